@@ -10,6 +10,8 @@ Tensors are borrowed for the call and results are written in place, as in the re
     `Runtime.blocking` is set to False (the reference always synchronises, _C.cpp:1182);
   * `attention` and `rope_and_cache` accept keyword-only `k_scale` / `v_scale` for a quantised KV cache
     (int8 or float8_e4m3fn, one fp32 scale per token and kv head).
+Beyond the reference: `tree_attention`, `verify_tree` (drafted trees), `attention_weights`, `select_kept` (caches kept
+to a budget) and `compact_kv_cache` (both).
 PyTorch is used only to own device memory and streams.
 """
 from __future__ import annotations
@@ -22,6 +24,7 @@ import torch
 from . import _lib
 
 _DT = {torch.float16: 0, torch.bfloat16: 1}
+_LOGIT_DT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 # element types of a quantised KV cache (one byte per element, fp32 scale per token and kv head)
 _KV_DT = {torch.int8: 1, torch.float8_e4m3fn: 2}
 
@@ -140,6 +143,17 @@ class Runtime:
         if _raw_stream is not None:
             return ctypes.c_void_p(_raw_stream(self.devid))
         return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def call(self, name: str, *args) -> None:
+        """One library call with this Runtime's device current (launches go to the current device, whatever their
+        stream's), and the wait of a blocking Runtime."""
+        fn = getattr(self._lib, name)
+        if torch.cuda.current_device() == self.devid:
+            _lib.check(fn(*args))
+        else:
+            with torch.cuda.device(self.devid):
+                _lib.check(fn(*args))
+        self.finish()
 
     def finish(self) -> None:
         if self.blocking:
@@ -646,6 +660,172 @@ def mla_prepare(rt: Runtime, attn_qkvc: torch.Tensor, q_norm: torch.Tensor, q_no
         rope_head_dim, block_size, _ptr(k_cache) if block_size else None, _ptr(pe_cache) if block_size else None,
         _ptr(slot_mapping) if block_size else None, float(norm_eps), dt))
     rt.finish()
+
+
+def _on(rt: Runtime, name: str, what: str, t: Optional[torch.Tensor], dtype=None) -> None:
+    """A contiguous tensor of `dtype` on the Runtime's device."""
+    if isinstance(t, torch.Tensor) and t.device == rt.device and t.is_contiguous() and (dtype is None or t.dtype == dtype):
+        return
+    _dev("%s: %s" % (name, what), t, dtype)
+    raise RuntimeError("%s: %s: expected a tensor on %s, got %s" % (name, what, rt.device, t.device))
+
+
+def _cache_type(rt: Runtime, name: str, act: torch.dtype, n_kv_heads: int, head_dim: int, block_size: int, caches, scales) -> int:
+    """Checks paged caches (name, tensor) of one shape and their scales; the kv_dtype code."""
+    _req(n_kv_heads > 0 and head_dim > 0 and block_size > 0, "%s: head counts, head_dim and block_size must be positive" % name)
+    quant = any(t is not None for _, t in scales)
+    for n, t in caches:
+        _on(rt, name, n, t)
+        if quant:
+            _req(t.dtype in _KV_DT and t.dtype == caches[0][1].dtype,
+                 "%s: scales given but the caches are neither int8 nor float8_e4m3fn" % name)
+        elif t.dtype != act:
+            raise RuntimeError("%s: %s %s unsupported! (expected %s)" % (name, n, t.dtype, act))
+        _req(t.numel() % (block_size * n_kv_heads * head_dim) == 0 and t.numel() == caches[0][1].numel(), "%s: cache shape mismatch" % name)
+    for n, t in scales:
+        if quant:
+            _req(t is not None, "%s: quantised caches need %s" % (name, n))
+            _on(rt, name, n, t, torch.float32)
+            _req(t.numel() * head_dim == caches[0][1].numel(), "%s: one scale per (block, slot, kv head) expected" % name)
+    return _KV_DT[caches[0][1].dtype] if quant else 0
+
+
+def _step_lists(rt: Runtime, name: str, batch: int, max_num_block: int, block_tables, **lists) -> None:
+    _req(batch >= 0 and max_num_block > 0, "%s: batch and max_num_block must be positive" % name)
+    for n, t in lists.items():
+        _on(rt, name, n, t, torch.int32)
+        _req(t.numel() >= batch, "%s: %s shorter than batch" % (name, n))
+    _on(rt, name, "block_tables", block_tables, torch.int32)
+    _req(block_tables.numel() >= batch * max_num_block, "%s: block_tables shorter than batch * max_num_block" % name)
+
+
+def tree_attention(rt: Runtime, qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, output: torch.Tensor,
+                   tree_mask: torch.Tensor, query_start_loc: torch.Tensor, lens: torch.Tensor, cached_lens: torch.Tensor,
+                   block_tables: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, block_size: int, batch: int,
+                   max_num_block: int, *, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+    """Paged GQA attention of drafted trees (not part of the reference API). The rows of a step are the nodes of one
+    tree per sequence, already in the cache at positions cached_lens[i] + node; a row sees every cached position and the
+    nodes whose bit its row of `tree_mask` [total_tokens, words] int32 has (`gvirt_amd.mha.prepare_tree` builds it). A
+    row that sees nothing gets zeros."""
+    name = "tree_attention"
+    _on(rt, name, "qkv", qkv)
+    _on(rt, name, "output", output)
+    dt = _act_dtype(name, qkv, output)
+    _req(n_kv_heads > 0 and n_heads > 0 and n_heads % n_kv_heads == 0, "tree_attention: n_heads must be a multiple of n_kv_heads")
+    kv = _cache_type(rt, name, qkv.dtype, n_kv_heads, head_dim, block_size, (("k_cache", k_cache), ("v_cache", v_cache)),
+                     (("k_scale", k_scale), ("v_scale", v_scale)))
+    _step_lists(rt, name, batch, max_num_block, block_tables, query_start_loc=query_start_loc, lens=lens, cached_lens=cached_lens)
+    T = qkv.shape[0]
+    _req(qkv.numel() == T * (n_heads + 2 * n_kv_heads) * head_dim, "tree_attention: qkv shape mismatch")
+    _req(output.numel() == T * n_heads * head_dim, "tree_attention: output shape mismatch")
+    _on(rt, name, "tree_mask", tree_mask, torch.int32)
+    _req(tree_mask.dim() == 2 and tree_mask.shape[0] == T and tree_mask.shape[1] > 0, "tree_attention: tree_mask must be [total_tokens, words]")
+    need = rt._lib.xlite_hip_tree_attention_workspace_bytes(T, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, kv)
+    ws = rt.workspace(need)
+    rt.call("xlite_hip_tree_attention", rt.stream(), _ptr(qkv), _ptr(k_cache), _ptr(v_cache), _ptr(output), _ptr(tree_mask),
+            tree_mask.shape[1], _ptr(query_start_loc), _ptr(lens), _ptr(cached_lens), _ptr(block_tables), T, n_heads, n_kv_heads,
+            head_dim, block_size, batch, max_num_block, dt, kv, _ptr(k_scale), _ptr(v_scale), _ptr(ws), ws.numel())
+
+
+def verify_tree(rt: Runtime, logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, accepted: torch.Tensor,
+                n_accepted: torch.Tensor, next_token: torch.Tensor, query_start_loc: torch.Tensor, lens: torch.Tensor,
+                batch: int) -> None:
+    """Greedy verification of drafted trees (not part of the reference API): from node 0 of every sequence on, the token
+    of the largest logit (lowest index of equal ones) of the node's row of `logits` [total_tokens, vocab] (fp16, bf16 or
+    fp32) chooses the child that goes on. `accepted` [batch, max_path] gets the path's nodes, then -1; `n_accepted`
+    [batch] its length; `next_token` [batch] the token behind its last node. `accepted` and `n_accepted` are the lists
+    of `compact_kv_cache` with starts=cached_lens."""
+    name = "verify_tree"
+    _on(rt, name, "logits", logits)
+    if logits.dtype not in _LOGIT_DT:
+        raise RuntimeError("verify_tree: logits dtype %s unsupported!" % logits.dtype)
+    _req(logits.dim() == 2, "verify_tree: logits must be [total_tokens, vocab]")
+    T, vocab = logits.shape
+    for n, t, least in (("tokens", tokens, T), ("parents", parents, T), ("n_accepted", n_accepted, batch),
+                        ("next_token", next_token, batch), ("query_start_loc", query_start_loc, batch), ("lens", lens, batch)):
+        _on(rt, name, n, t, torch.int32)
+        _req(t.numel() >= least, "verify_tree: %s too short" % n)
+    _on(rt, name, "accepted", accepted, torch.int32)
+    _req(accepted.dim() == 2 and accepted.shape[0] >= batch and accepted.shape[1] > 0, "verify_tree: accepted must be [batch, max_path]")
+    ws = rt.workspace(rt._lib.xlite_hip_verify_tree_workspace_bytes(T))
+    rt.call("xlite_hip_verify_tree", rt.stream(), _ptr(logits), _ptr(tokens), _ptr(parents), _ptr(accepted), _ptr(n_accepted),
+            _ptr(next_token), _ptr(query_start_loc), _ptr(lens), T, vocab, batch, accepted.shape[1], _LOGIT_DT[logits.dtype],
+            _ptr(ws), ws.numel())
+
+
+def attention_weights(rt: Runtime, qkv: torch.Tensor, k_cache: torch.Tensor, weights: torch.Tensor,
+                      query_start_loc: torch.Tensor, lens: torch.Tensor, cached_lens: torch.Tensor, block_tables: torch.Tensor,
+                      n_heads: int, n_kv_heads: int, head_dim: int, block_size: int, batch: int, max_num_block: int,
+                      window: int = 0, *, k_scale: Optional[torch.Tensor] = None) -> None:
+    """Accumulated attention weight of every cached position (not part of the reference API): `weights` [num_blocks,
+    block_size, n_kv_heads] fp32 gets, for every position and kv head, the sum of the softmax probabilities that the
+    step's rows (the last `window` of every sequence, 0: all) and the kv head's query heads give it, causal as in
+    `attention`. Added to what earlier steps left for cached positions; the step's own positions start at zero."""
+    name = "attention_weights"
+    _on(rt, name, "qkv", qkv)
+    dt = _act_dtype(name, qkv)
+    _req(n_kv_heads > 0 and n_heads > 0 and n_heads % n_kv_heads == 0, "attention_weights: n_heads must be a multiple of n_kv_heads")
+    kv = _cache_type(rt, name, qkv.dtype, n_kv_heads, head_dim, block_size, (("k_cache", k_cache),), (("k_scale", k_scale),))
+    _step_lists(rt, name, batch, max_num_block, block_tables, query_start_loc=query_start_loc, lens=lens, cached_lens=cached_lens)
+    T = qkv.shape[0]
+    _req(qkv.numel() == T * (n_heads + 2 * n_kv_heads) * head_dim, "attention_weights: qkv shape mismatch")
+    _on(rt, name, "weights", weights, torch.float32)
+    _req(weights.numel() * head_dim == k_cache.numel(), "attention_weights: one weight per (block, slot, kv head) expected")
+    _req(window >= 0, "attention_weights: window must not be negative")
+    need = rt._lib.xlite_hip_attention_weights_workspace_bytes(T, n_heads, n_kv_heads, block_size, batch, max_num_block, window)
+    ws = rt.workspace(need)
+    rt.call("xlite_hip_attention_weights", rt.stream(), _ptr(qkv), _ptr(k_cache), _ptr(weights), _ptr(query_start_loc), _ptr(lens),
+            _ptr(cached_lens), _ptr(block_tables), T, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, window, dt, kv,
+            _ptr(k_scale), _ptr(ws), ws.numel())
+
+
+def select_kept(rt: Runtime, weights: torch.Tensor, kept: torch.Tensor, kept_lens: torch.Tensor, context_lens: torch.Tensor,
+                block_tables: torch.Tensor, n_kv_heads: int, block_size: int, batch: int, max_num_block: int, budget: int,
+                recent: int, sink: int = 0) -> None:
+    """Which positions a cache keeps (not part of the reference API): per sequence and kv head the first `sink`, the last
+    `recent` and the largest `weights` of the rest, `budget` in all (everything, if it fits; equal weights: the lower
+    position). `kept` [batch, n_kv_heads, budget] gets ascending positions, then -1, `kept_lens` [batch] their number:
+    the lists of `compact_kv_cache`."""
+    name = "select_kept"
+    _req(n_kv_heads > 0 and block_size > 0, "select_kept: n_kv_heads and block_size must be positive")
+    _on(rt, name, "weights", weights, torch.float32)
+    _req(weights.numel() % (block_size * n_kv_heads) == 0, "select_kept: weights shape mismatch")
+    _step_lists(rt, name, batch, max_num_block, block_tables, kept_lens=kept_lens, context_lens=context_lens)
+    _req(budget > 0 and recent >= 0 and sink >= 0 and recent + sink <= budget,
+         "select_kept: budget must be positive and hold recent + sink")
+    _on(rt, name, "kept", kept, torch.int32)
+    _req(kept.numel() == batch * n_kv_heads * budget, "select_kept: kept must be [batch, n_kv_heads, budget]")
+    rt.call("xlite_hip_select_kept", rt.stream(), _ptr(weights), _ptr(kept), _ptr(kept_lens), _ptr(context_lens), _ptr(block_tables),
+            n_kv_heads, block_size, batch, max_num_block, budget, recent, sink)
+
+
+def compact_kv_cache(rt: Runtime, k_cache: torch.Tensor, v_cache: torch.Tensor, kept: torch.Tensor, kept_lens: torch.Tensor,
+                     block_tables: torch.Tensor, n_kv_heads: int, head_dim: int, block_size: int, batch: int,
+                     max_num_block: int, *, starts: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                     k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+    """Moves cache rows to the front, in place (not part of the reference API): position starts[i] + n of sequence i
+    receives the rows of position starts[i] + kept[i, n], n < kept_lens[i]; kept[i, n] >= n. `kept` is [batch,
+    n_kv_heads, max_kept] (a list per kv head, `select_kept`) or [batch, max_kept] (one list, `verify_tree`). Scales and
+    `weights` move with their rows."""
+    name = "compact_kv_cache"
+    kv = _cache_type(rt, name, k_cache.dtype if isinstance(k_cache, torch.Tensor) else None, n_kv_heads, head_dim, block_size,
+                     (("k_cache", k_cache), ("v_cache", v_cache)), (("k_scale", k_scale), ("v_scale", v_scale)))
+    if kv == 0:
+        _act_dtype(name, k_cache, v_cache)
+    _step_lists(rt, name, batch, max_num_block, block_tables, kept_lens=kept_lens)
+    _on(rt, name, "kept", kept, torch.int32)
+    per_head = kept.dim() == 3
+    _req(kept.dim() in (2, 3) and kept.shape[0] >= batch and (not per_head or kept.shape[1] == n_kv_heads),
+         "compact_kv_cache: kept must be [batch, n_kv_heads, max_kept] or [batch, max_kept]")
+    if starts is not None:
+        _on(rt, name, "starts", starts, torch.int32)
+        _req(starts.numel() >= batch, "compact_kv_cache: starts shorter than batch")
+    if weights is not None:
+        _on(rt, name, "weights", weights, torch.float32)
+        _req(weights.numel() * head_dim == k_cache.numel(), "compact_kv_cache: one weight per (block, slot, kv head) expected")
+    rt.call("xlite_hip_compact_kv_cache", rt.stream(), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(weights),
+            _ptr(kept), _ptr(kept_lens), _ptr(starts), _ptr(block_tables), n_kv_heads, head_dim, block_size, batch, max_num_block,
+            kept.shape[-1], 1 if per_head else 0, kv)
 
 
 def get_tile_size_of_cached_kv(cached_lens: List[int], query_lens: List[int], head_num_in_group: int,

@@ -42,6 +42,15 @@ SIGNATURES = {
     "xlite_hip_layernorm": (_i32, [_vp] * 5 + [_u32] * 4 + [_f32, _i32]),
     "xlite_hip_muls": (_i32, [_vp] * 3 + [_u32] * 4 + [_f32, _i32]),
     "xlite_hip_rope_complex_and_cache": (_i32, [_vp] + [_u32] * 6 + [_vp, _vp, _u32, _u32, _vp, _vp, _u32, _vp, _vp, _i32]),
+    "xlite_hip_prepare_tree": (_i32, [_vp] * 3 + [_u32] * 2 + [_vp] * 2),
+    "xlite_hip_tree_attention_workspace_bytes": (_sz, [_u32] * 7 + [_i32]),
+    "xlite_hip_tree_attention": (_i32, [_vp] * 6 + [_u32] + [_vp] * 4 + [_u32] * 7 + [_i32, _i32] + [_vp] * 3 + [_sz]),
+    "xlite_hip_verify_tree_workspace_bytes": (_sz, [_u32]),
+    "xlite_hip_verify_tree": (_i32, [_vp] * 9 + [_u32] * 4 + [_i32, _vp, _sz]),
+    "xlite_hip_attention_weights_workspace_bytes": (_sz, [_u32] * 7),
+    "xlite_hip_attention_weights": (_i32, [_vp] * 8 + [_u32] * 8 + [_i32, _i32, _vp, _vp, _sz]),
+    "xlite_hip_select_kept": (_i32, [_vp] * 6 + [_u32] * 7),
+    "xlite_hip_compact_kv_cache": (_i32, [_vp] * 10 + [_u32] * 6 + [_i32, _i32]),
 }
 
 _lib = None

@@ -26,8 +26,60 @@ struct AttentionArgs {
     // a bf16 model over the fp16 copy of a quantised cache, on a kernel that converts at its edges: dtype says
     // FP16 (the products), qkv and output are bf16
     bool io_bf16;
+    // a drafted tree per sequence: row r sees every cached position, and of the step's own positions those whose bit is
+    // set in its mask_words words (nullptr: causal)
+    const uint32_t *tree_mask;
+    uint32_t mask_words;
 };
 enum { kAllRows = 0, kOnlySingle = 1, kSkipSingle = 2 };
+
+// the low n bits (none below 0, all from 32 on)
+__device__ __forceinline__ uint32_t ones(int32_t n)
+{
+    return static_cast<uint32_t>((1ull << min(max(n, 0), 32)) - 1);
+}
+// Which of the positions j0 .. j0 + 31 a tree row sees, as bits. `words`: the row's mask, bit n = drafted node n, which sits
+// at position `cached` + n; every position below `cached` is seen, none at or beyond `cached` + `nodes`.
+__device__ __forceinline__ uint32_t tree_seen(const uint32_t *words, uint32_t n_words, uint32_t j0, uint32_t cached, uint32_t nodes)
+{
+    const int32_t off = static_cast<int32_t>(j0 - cached);   // the node of position j0; negative: cached positions
+    const int32_t i = off >> 5;
+    const uint32_t sh = static_cast<uint32_t>(off) & 31u;
+    // (loads from clamped indexes, selected afterwards: a load under a condition is awaited on its own)
+    const int32_t last = static_cast<int32_t>(n_words) - 1;
+    const uint32_t a = words[min(max(i, 0), last)], b = words[min(max(i + 1, 0), last)];
+    const uint64_t both = (i >= 0 && i <= last ? a : 0u) | (static_cast<uint64_t>(i + 1 >= 0 && i + 1 <= last ? b : 0u) << 32);
+    uint32_t seen = static_cast<uint32_t>(both >> sh);
+    seen |= ones(-off);
+    return seen & ones(static_cast<int32_t>(nodes) - off);   // (nodes - off: positions of the sequence from j0 on)
+}
+
+// 16-bit pairs with an infinity or a NaN in either half
+template <typename T>
+__device__ __forceinline__ bool not_finite2(uint32_t w)
+{
+    constexpr uint32_t e = T::kCode == XLITE_HIP_BF16 ? 0x7f80u : 0x7c00u;
+    return static_cast<uint32_t>((w & e) == e) | static_cast<uint32_t>((w & (e << 16)) == (e << 16));
+}
+
+// the pair with its infinities and NaNs as zeros
+template <typename T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w)
+{
+    constexpr uint32_t e = T::kCode == XLITE_HIP_BF16 ? 0x7f80u : 0x7c00u;
+    return ((w & e) == e ? 0u : w & 0xffffu) | ((w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u);
+}
+// eight 16-bit values as indicators (1 or 0) of +infinity (what = 0), -infinity (1) or NaN (2)
+template <typename T>
+__device__ __forceinline__ uint4 odd_values(const uint2 &lo, const uint2 &hi, int what)
+{
+    constexpr uint32_t e = T::kCode == XLITE_HIP_BF16 ? 0x7f80u : 0x7c00u, one = T::kCode == XLITE_HIP_BF16 ? 0x3f80u : 0x3c00u;
+    auto is = [&](uint32_t h) {
+        return what == 0 ? h == e : what == 1 ? h == (e | 0x8000u) : (h & 0x7fffu) > e;
+    };
+    auto pair = [&](uint32_t w) { return (is(w & 0xffffu) ? one : 0u) | (is(w >> 16) ? one << 16 : 0u); };
+    return make_uint4(pair(lo.x), pair(lo.y), pair(hi.x), pair(hi.y));
+}
 
 struct MlaArgs {
     const void *q_absorb;
@@ -62,6 +114,7 @@ size_t partial_bytes(uint32_t rows, uint32_t n_heads, uint32_t dv, uint32_t max_
 PartialBuffers carve_partials(void *workspace, uint32_t rows, uint32_t n_heads, uint32_t dv, uint32_t max_slots);
 int launch_merge(hipStream_t stream, int dtype, void *out, const PartialBuffers &b, uint32_t rows,
                  uint32_t n_heads, uint32_t dv, uint32_t max_slots);
+int launch_clear_counts(hipStream_t stream, const PartialBuffers &b, uint32_t rows, uint32_t n_heads);
 // Partials of the MLA decode kernel: a row's s-th segment sits in slot 2 c0 + (1 - first flag) for s = 0 and
 // 2 (c0 + s) after that (meta = segments, c0, first flag per row); acc holds O / l in the 16-bit activation type.
 int launch_merge_mla(hipStream_t stream, int dtype, void *out, const uint16_t *acc, const float *ml, const int32_t *meta,

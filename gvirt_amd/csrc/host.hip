@@ -234,3 +234,34 @@ extern "C" int xlite_hip_prepare_attn(const uint32_t *lens, const uint32_t *cach
     }
     return XLITE_HIP_OK;
 }
+
+// ---- drafted trees: rope positions and ancestor masks from the parents ----
+extern "C" int xlite_hip_prepare_tree(const uint32_t *lens, const uint32_t *cached_lens, const int32_t *parents, uint32_t batch,
+                                      uint32_t mask_words, int64_t *position, int32_t *tree_mask)
+{
+    XL_REQUIRE(batch > 0, "invalid batchSize: 0");
+    XL_REQUIRE(lens && cached_lens && parents, "null input");
+    XL_REQUIRE(position && tree_mask, "null output");
+    XL_REQUIRE(mask_words > 0, "mask_words must be positive");
+    size_t first = 0;   // of the sequence's nodes
+    for (uint32_t i = 0; i < batch; i++) {
+        const uint32_t n = lens[i];
+        XL_REQUIRE(ceil_div(n, 32) <= mask_words, "mask_words too small for a tree of " + std::to_string(n) + " nodes");
+        for (uint32_t r = 0; r < n; r++) {
+            const int32_t up = parents[first + r];
+            XL_REQUIRE(up >= -1 && up < static_cast<int32_t>(r),
+                       "a node's parent must stand before it (node " + std::to_string(r) + ", parent " + std::to_string(up) + ")");
+            int32_t *row = tree_mask + (first + r) * mask_words;
+            if (up >= 0) {
+                std::copy(row - (r - up) * static_cast<size_t>(mask_words), row - (r - up) * static_cast<size_t>(mask_words) + mask_words, row);
+                position[first + r] = position[first + up] + 1;
+            } else {
+                std::fill(row, row + mask_words, 0);
+                position[first + r] = static_cast<int64_t>(cached_lens[i]);
+            }
+            row[r / 32] = static_cast<int32_t>(static_cast<uint32_t>(row[r / 32]) | 1u << (r % 32));
+        }
+        first += n;
+    }
+    return XLITE_HIP_OK;
+}

@@ -441,6 +441,24 @@ PartialBuffers carve_partials(void *workspace, uint32_t rows, uint32_t n_heads, 
     return b;
 }
 
+__global__ void __launch_bounds__(256)
+clear_counts_kernel(int32_t *cnt, uint64_t n)
+{
+    const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i < n) {
+        cnt[i] = 0;
+    }
+}
+
+// "nothing to merge" for every row: those of no sequence (a batch padded with rows behind its last one) are nobody's
+int launch_clear_counts(hipStream_t stream, const PartialBuffers &b, uint32_t rows, uint32_t n_heads)
+{
+    const uint64_t n = static_cast<uint64_t>(rows) * n_heads;
+    clear_counts_kernel<<<static_cast<uint32_t>((n + 255) / 256), 256, 0, stream>>>(b.cnt, n);
+    XL_LAUNCH_CHECK();
+    return XLITE_HIP_OK;
+}
+
 int launch_merge(hipStream_t stream, int dtype, void *out, const PartialBuffers &b, uint32_t rows,
                  uint32_t n_heads, uint32_t dv, uint32_t max_slots)
 {

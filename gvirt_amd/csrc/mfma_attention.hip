@@ -18,6 +18,8 @@
 //
 // Replaces attention.h / flash_attention.h for batches with multi-token queries
 // (xlite/csrc/kernels/attention.h:308-492) and mla_v2.h / flash_mla_v2.h / mla_v3.h.
+#include <type_traits>
+
 #include "attention_common.h"
 
 namespace xlite {
@@ -76,6 +78,8 @@ struct MfmaParams {
     uint32_t max_splits;
     float scale_log2e;
     uint32_t table_in_lds;   // 1: the launch reserved LDS for the sequence's block-table row (max_num_block words)
+    const uint32_t *tree_mask;   // trees: [token][mask_words], which of the step's own positions a row sees
+    uint32_t mask_words;
 };
 
 // position inside a 16-token group at which token offset o is stored in the transposed V tile, so
@@ -85,7 +89,8 @@ __device__ __forceinline__ uint32_t vt_pos(uint32_t o)
     return (o & ~15u) | (((o >> 2) & 1u) << 3) | (((o >> 3) & 1u) << 2) | (o & 3u);
 }
 
-template <typename T, int DQ0, int DQ1, int DV, int BN, bool SEPARATE_V>
+// TREE (with a separate value cache): the step's rows are drafted trees, see tree_seen
+template <typename T, int DQ0, int DQ1, int DV, int BN, bool SEPARATE_V, bool TREE = false>
 __global__ void __launch_bounds__(kThreads)
 mfma_attention_kernel(const MfmaParams p)
 {
@@ -145,7 +150,7 @@ mfma_attention_kernel(const MfmaParams p)
     const uint32_t total_kv = dense ? min(static_cast<uint32_t>(clen + qlen), p.dense_len)
                                     : static_cast<uint32_t>(clen + qlen);
     // keys visible to at least one row of the tile
-    const uint32_t limit_max = dense ? total_kv : static_cast<uint32_t>(clen) + m_last / G + 1;
+    const uint32_t limit_max = dense || TREE ? total_kv : static_cast<uint32_t>(clen) + m_last / G + 1;
     const uint32_t n_splits = ceil_div(limit_max, p.split_len);
     if (split >= n_splits) {
         return;
@@ -384,12 +389,30 @@ mfma_attention_kernel(const MfmaParams p)
 
         // ---- online softmax over the tile -----------------------------------------------------------------
         float mx = -INFINITY;
+        // (a tile below the cached length is seen whole: the words of the mask are read behind a uniform condition)
+        [[maybe_unused]] const bool own_positions = TREE && j0 + BN > static_cast<uint32_t>(clen);
+        [[maybe_unused]] uint32_t seen[NT];
+        if constexpr (TREE) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                seen[nt] = 0xffffffffu;
+                if (own_positions) {
+                    seen[nt] = tree_seen(p.tree_mask + static_cast<uint64_t>(tok) * p.mask_words, p.mask_words, j0 + nt * 32,
+                                         static_cast<uint32_t>(clen), static_cast<uint32_t>(qlen));
+                }
+                seen[nt] = m_valid ? seen[nt] >> (4 * half) : 0u;
+            }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int k = 0; k < 16; k++) {
                 const uint32_t t = j0 + nt * 32 + (k / 4) * 8 + half * 4 + (k % 4);
-                const float s = t < vis ? S[nt][k] * p.scale_log2e : -INFINITY;
+                bool ok = t < vis;
+                if constexpr (TREE) {
+                    ok = (seen[nt] >> ((k / 4) * 8 + (k % 4))) & 1u;
+                }
+                const float s = ok ? S[nt][k] * p.scale_log2e : -INFINITY;
                 S[nt][k] = s;
                 mx = fmaxf(mx, s);
             }
@@ -434,7 +457,35 @@ mfma_attention_kernel(const MfmaParams p)
             for (int kk = 0; kk < 2; kk++) {
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
-                    const uint4 a = *reinterpret_cast<const uint4 *>(Vt + (dt * 32 + col) * VSTRIDE + nt * 32 + kk * 16 + half * 8);
+                    uint4 a = *reinterpret_cast<const uint4 *>(Vt + (dt * 32 + col) * VSTRIDE + nt * 32 + kk * 16 + half * 8);
+                    if constexpr (TREE) {
+                        // infinities and NaNs in V rows that some rows of the tile do not see (as in the prefill kernel)
+                        if (own_positions && __any(not_finite2<T>(a.x) | not_finite2<T>(a.y) | not_finite2<T>(a.z) | not_finite2<T>(a.w))) {
+                            uint32_t sw[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int k = kk * 8 + 2 * e;
+                                sw[e] = T::pack((seen[nt] >> ((k / 4) * 8 + (k % 4))) & 1u ? 1.f : 0.f,
+                                                (seen[nt] >> (((k + 1) / 4) * 8 + ((k + 1) % 4))) & 1u ? 1.f : 0.f);
+                            }
+#pragma unroll 1
+                            for (int what = 0; what < 3; what++) {
+                                f32x16_t hit;
+#pragma unroll
+                                for (int k = 0; k < 16; k++) {
+                                    hit[k] = 0.f;
+                                }
+                                hit = Mfma<T>::run(odd_values<T>(make_uint2(a.x, a.y), make_uint2(a.z, a.w), what),
+                                                   make_uint4(sw[0], sw[1], sw[2], sw[3]), hit);
+                                const float odd = what == 0 ? INFINITY : what == 1 ? -INFINITY : NAN;
+#pragma unroll
+                                for (int k = 0; k < 16; k++) {
+                                    O[dt][k] += hit[k] > 0.f ? odd : 0.f;
+                                }
+                            }
+                            a = make_uint4(finite_only<T>(a.x), finite_only<T>(a.y), finite_only<T>(a.z), finite_only<T>(a.w));
+                        }
+                    }
                     O[dt] = Mfma<T>::run(a, pb[nt][kk], O[dt]);
                 }
             }
@@ -486,7 +537,7 @@ constexpr size_t lds_bytes()
     return static_cast<size_t>(BN) * (DQK + 8) * 2 + static_cast<size_t>(DV) * (BN + 8) * 2 + BN * 8;
 }
 
-template <typename T, int DQ0, int DQ1, int DV, int BN, bool SEPARATE_V>
+template <typename T, int DQ0, int DQ1, int DV, int BN, bool SEPARATE_V, bool TREE = false>
 int launch_kernel(hipStream_t stream, const MfmaParams &p_in, dim3 grid)
 {
     MfmaParams p = p_in;
@@ -496,7 +547,7 @@ int launch_kernel(hipStream_t stream, const MfmaParams &p_in, dim3 grid)
     if (p.table_in_lds) {
         lds += static_cast<size_t>(p.max_num_block) * 4;
     }
-    auto kernel = mfma_attention_kernel<T, DQ0, DQ1, DV, BN, SEPARATE_V>;
+    auto kernel = mfma_attention_kernel<T, DQ0, DQ1, DV, BN, SEPARATE_V, TREE>;
     if (lds > 64 * 1024) {
         if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds)) {
             return rc;
@@ -583,23 +634,33 @@ int launch_mfma_gqa(hipStream_t stream, const AttentionArgs &a)
     p.split_len = split_len;
     p.max_splits = max_splits;
     p.scale_log2e = kLog2e;
+    p.tree_mask = a.tree_mask;
+    p.mask_words = a.mask_words;
     const PartialBuffers pb = max_splits > 1 ? carve_partials(a.workspace, a.total_tokens, a.n_heads, a.head_dim, max_splits)
                                              : PartialBuffers{};
     fill_common(p, pb);
 
     dim3 grid(max_splits, m_tiles, a.n_kv_heads);
     const bool bf = a.dtype == XLITE_HIP_BF16;
-    int rc;
-    if (a.head_dim == 256) {
-        rc = bf ? launch_kernel<BF16, 256, 0, 256, BN, true>(stream, p, grid)
-                : launch_kernel<FP16, 256, 0, 256, BN, true>(stream, p, grid);
-    } else if (a.head_dim == 128) {
-        rc = bf ? launch_kernel<BF16, 128, 0, 128, BN, true>(stream, p, grid)
-                : launch_kernel<FP16, 128, 0, 128, BN, true>(stream, p, grid);
-    } else {
-        rc = bf ? launch_kernel<BF16, 64, 0, 64, BN, true>(stream, p, grid)
-                : launch_kernel<FP16, 64, 0, 64, BN, true>(stream, p, grid);
+    if (a.tree_mask != nullptr && max_splits > 1) {
+        if (const int rc = launch_clear_counts(stream, pb, a.total_tokens, a.n_heads)) {
+            return rc;
+        }
     }
+    auto of_type = [&](auto tree) {
+        constexpr bool TREE = decltype(tree)::value;
+        if (a.head_dim == 256) {
+            return bf ? launch_kernel<BF16, 256, 0, 256, BN, true, TREE>(stream, p, grid)
+                      : launch_kernel<FP16, 256, 0, 256, BN, true, TREE>(stream, p, grid);
+        }
+        if (a.head_dim == 128) {
+            return bf ? launch_kernel<BF16, 128, 0, 128, BN, true, TREE>(stream, p, grid)
+                      : launch_kernel<FP16, 128, 0, 128, BN, true, TREE>(stream, p, grid);
+        }
+        return bf ? launch_kernel<BF16, 64, 0, 64, BN, true, TREE>(stream, p, grid)
+                  : launch_kernel<FP16, 64, 0, 64, BN, true, TREE>(stream, p, grid);
+    };
+    const int rc = a.tree_mask != nullptr ? of_type(std::integral_constant<bool, true>{}) : of_type(std::integral_constant<bool, false>{});
     if (rc != XLITE_HIP_OK || max_splits == 1) {
         return rc;
     }

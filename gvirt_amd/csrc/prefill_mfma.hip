@@ -88,6 +88,8 @@ struct PrefillParams {
     unsigned long long *clock_probe;   // nullptr, or where workgroup 0 leaves its shader-clock and wall-clock stamps
     const float *k_scale;      // 8-bit caches read by the kernel itself: [slot][kv head] fp32
     const float *v_scale;
+    const uint32_t *tree_mask; // trees: [token][mask_words], which of the step's own positions a row sees
+    uint32_t mask_words;
 };
 
 // XOR pattern of the 16-byte chunk index of LDS row `row` (rows are 256 bytes = one bank window). The
@@ -142,7 +144,9 @@ __device__ __forceinline__ uint4 convert8(const uint4 &x)
 // then a wave loads the bytes and scales of its eight positions of a tile into registers, two tiles ahead, and writes
 // them to the tile's stage as fp16 (value x scale, the arithmetic of the dequantising copy in kv_dequant.hip: same
 // bits) one iteration later; everything behind the stages is the 16-bit kernel. head_dim 128, T = FP16.
-template <typename T, int D, typename TIO = T, int KVF = XLITE_HIP_KV_SAME>
+// TREE: the step's rows are drafted trees: a row sees every cached position and, of the step's own, those of its mask
+// (the unmasked tiles are those below the cached length, the range of every M tile ends with the sequence).
+template <typename T, int D, typename TIO = T, int KVF = XLITE_HIP_KV_SAME, bool TREE = false>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const PrefillParams p)
 {
@@ -281,7 +285,7 @@ prefill_kernel(const PrefillParams p)
     const uint32_t m_first = mt * kMTile;
     const uint32_t m_last = min(m_rows, m_first + kMTile) - 1;
     // keys visible to at least one row of the tile
-    const uint32_t range_end = static_cast<uint32_t>(clen) + m_last / G + 1;
+    const uint32_t range_end = static_cast<uint32_t>(clen) + (TREE ? static_cast<uint32_t>(qlen) : m_last / G + 1);
     // ---- this workgroup's run of KV tiles [first_tile, n_tiles): the whole range, or one of n_splits equal
     // runs of at least kMinSplitTiles tiles
     uint32_t n_tiles = ceil_div(range_end, static_cast<uint32_t>(BN));
@@ -309,7 +313,7 @@ prefill_kernel(const PrefillParams p)
     const uint32_t tok = static_cast<uint32_t>(qstart) + qpos;
     const uint32_t vis = m_valid ? static_cast<uint32_t>(clen) + qpos + 1 : 0u;   // causal: keys [0, vis)
     // tiles wholly below every row's limit need no mask; first tile that does (uniform per wave)
-    const uint32_t wave_min_vis = static_cast<uint32_t>(clen) + min(m_first + wave * 32, m_rows - 1) / G + 1;
+    const uint32_t wave_min_vis = static_cast<uint32_t>(clen) + (TREE ? 0u : min(m_first + wave * 32, m_rows - 1) / G + 1);
 
     uint4 qreg[KS];   // the lane's query row as the B operand of the first product; loaded by the set-up below
     f32x16_t O[DT];
@@ -366,7 +370,7 @@ prefill_kernel(const PrefillParams p)
     // rows apart, so one lookup and one base address serve both: a third of the loop's scalar instructions)
     const bool one_lookup = CPT == 2 && (p.block_size & 7u) == 0;
     const uint32_t c_voff_second = c_voff[CPT - 1] + PPC * row_bytes;
-    auto issue = [&](uint32_t tile) {
+    auto issue = [&](uint32_t tile) __attribute__((always_inline)) {
         const uint32_t st = smem_addr + (tile % kStages) * STAGE;
         if (one_lookup && tile * BN + PPC * CPT * (wave + 1) - 1 < range_end) {
             const uint32_t pos = PPC * CPT * wave;
@@ -451,7 +455,9 @@ prefill_kernel(const PrefillParams p)
     // ---- one step of 32 positions. Register k of S holds position j0 + 8 (k / 4) + 4 half + k % 4. The
     // running maximum is kept in raw score units; q arrives scaled by head_dim^-0.5 (rope_and_cache), so the
     // only factor is log2(e), folded into the exponent's multiply-add.
-    auto step = [&](uint32_t stage_off, int h, uint32_t j0, uint32_t next_stage_off, int next_h, auto mask_tag) {
+    // (always inlined: as a function of its own it would take the kernel's registers through memory, and the copies' scalar
+    // addresses with them)
+    auto step = [&](uint32_t stage_off, int h, uint32_t j0, uint32_t next_stage_off, int next_h, auto mask_tag) __attribute__((always_inline)) {
         constexpr bool MASK = decltype(mask_tag)::value;
         // ---- S^T = K . Q^T (one accumulation chain: the SIMD's other wave fills the issue gaps between
         // dependent products, and a second chain would cost 16 more vector instructions of this wave's issue time)
@@ -484,7 +490,16 @@ prefill_kernel(const PrefillParams p)
         // issue slots are sparse, and this wave's vector instructions go first (1 % on the chunked-prefill step;
         // raising the priority around the products instead costs 4 %)
         __builtin_amdgcn_s_setprio(2);
-        if constexpr (MASK) {
+        [[maybe_unused]] uint32_t seen = 0;
+        if constexpr (MASK && TREE) {
+            seen = tree_seen(p.tree_mask + static_cast<uint64_t>(tok) * p.mask_words, p.mask_words, j0,
+                             static_cast<uint32_t>(clen), static_cast<uint32_t>(qlen)) >> (4 * half);
+            seen = m_valid ? seen : 0u;
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                S[k] = (seen >> ((k / 4) * 8 + (k % 4))) & 1u ? S[k] : -INFINITY;
+            }
+        } else if constexpr (MASK) {
             const uint32_t rem = vis > j0 + half * 4 ? vis - (j0 + half * 4) : 0u;
 #pragma unroll
             for (int k = 0; k < 16; k++) {
@@ -532,6 +547,58 @@ prefill_kernel(const PrefillParams p)
             }
         }
         __builtin_amdgcn_s_setprio(0);
+        if constexpr (MASK && TREE) {
+            // A row that does not see a position has probability zero there, and zero times an infinity or a NaN in that
+            // position's V row would still poison it (rows of other branches share the tile). Such values are taken out of
+            // the operands; the rows that do see them get them back through three products of indicators.
+            bool odd = false;
+#pragma unroll
+            for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                    for (int h2 = 0; h2 < 2; h2++) {
+                        odd |= not_finite2<T>(vop[kk][dt][h2].x) | not_finite2<T>(vop[kk][dt][h2].y);
+                    }
+                }
+            }
+            if (__any(odd)) {
+                uint32_t sw[8];
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    sw[k / 2] = T::pack((seen >> ((k / 4) * 8 + (k % 4))) & 1u ? 1.f : 0.f,
+                                        (seen >> (((k + 1) / 4) * 8 + ((k + 1) % 4))) & 1u ? 1.f : 0.f);
+                }
+                const uint4 sb[2] = {make_uint4(sw[0], sw[1], sw[2], sw[3]), make_uint4(sw[4], sw[5], sw[6], sw[7])};
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                    for (int what = 0; what < 3; what++) {   // +inf, -inf, NaN
+                        f32x16_t hit;
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            hit[k] = 0.f;
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < 2; kk++) {
+                            hit = Mfma32<T>::run(odd_values<T>(vop[kk][dt][0], vop[kk][dt][1], what), sb[kk], hit);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            O[dt][k] += hit[k] > 0.f ? (what == 0 ? INFINITY : what == 1 ? -INFINITY : NAN) : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+                        for (int h2 = 0; h2 < 2; h2++) {
+                            vop[kk][dt][h2].x = finite_only<T>(vop[kk][dt][h2].x);
+                            vop[kk][dt][h2].y = finite_only<T>(vop[kk][dt][h2].y);
+                        }
+                    }
+                }
+            }
+        }
         __builtin_amdgcn_sched_barrier(0);
         // K operands of the next step: in flight during the second product
         fetch_k(next_stage_off, next_h);
@@ -601,7 +668,7 @@ prefill_kernel(const PrefillParams p)
     fetch_k((first_tile % kStages) * STAGE, 0);
     using MaskOn = std::integral_constant<bool, true>;
     using MaskOff = std::integral_constant<bool, false>;
-    auto tile_iter = [&](uint32_t tile, auto mask_tag) {
+    auto tile_iter = [&](uint32_t tile, auto mask_tag) __attribute__((always_inline)) {
         const uint32_t so = (tile % kStages) * STAGE;
         const uint32_t so_next = (min(tile + 1, last) % kStages) * STAGE;
         const uint32_t j0 = tile * BN;
@@ -810,6 +877,8 @@ int launch_prefill_mfma(hipStream_t stream, const AttentionArgs &a)
     p.skip_single = a.rows_mode == kSkipSingle ? 1u : 0u;
     p.k_scale = a.k_scale;
     p.v_scale = a.v_scale;
+    p.tree_mask = a.tree_mask;
+    p.mask_words = a.mask_words;
     const bool kv8 = a.kv_dtype != XLITE_HIP_KV_SAME;
     XL_REQUIRE(!kv8 || prefill_kv8_supported(a), "8-bit caches: shape not served by the prefill kernel");
     uint32_t splits = prefill_mfma_pick_splits(a.total_tokens, G, a.batch, a.n_kv_heads, a.max_num_block * a.block_size, a.head_dim);
@@ -857,9 +926,15 @@ int launch_prefill_mfma(hipStream_t stream, const AttentionArgs &a)
     } else {
         n_wg = a.n_kv_heads * p.n_mtiles;
     }
+    if (a.tree_mask != nullptr && splits > 1) {
+        if (const int rc = launch_clear_counts(stream, pb, a.total_tokens, a.n_heads)) {
+            return rc;
+        }
+    }
     const dim3 grid(n_wg, splits, 1);
     const int rc_launch = with_kernel([&](auto t, auto d, auto tio, auto kvf) -> int {
-        auto kernel = prefill_kernel<decltype(t), decltype(d)::value, decltype(tio), decltype(kvf)::value>;
+        auto kernel = p.tree_mask != nullptr ? prefill_kernel<decltype(t), decltype(d)::value, decltype(tio), decltype(kvf)::value, true>
+                                             : prefill_kernel<decltype(t), decltype(d)::value, decltype(tio), decltype(kvf)::value>;
         if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds)) {
             return rc;
         }

@@ -28,6 +28,9 @@ class StepMeta:
     block_tables: torch.Tensor      # [batch * max_num_blocks] int32
     position: torch.Tensor          # [batched_tokens] int64
     slot_mapping: torch.Tensor      # [batched_tokens] int32
+    # drafted trees only: the nodes' ancestor masks [batched_tokens, words] and parents [batched_tokens], int32
+    tree_mask: Optional[torch.Tensor] = None
+    parents: Optional[torch.Tensor] = None
 
 
 def prepare_attn(lens: Sequence[int], cached_lens: Sequence[int], block_tables: Sequence[Sequence[int]],
@@ -77,6 +80,33 @@ def prepare_attn_meta(meta, block_size: int, device) -> StepMeta:
     raise RuntimeError("prepare_attn: invalid attnMeta version: " + type(meta).__name__)
 
 
+def prepare_tree(lens: Sequence[int], cached_lens: Sequence[int], block_tables: Sequence[Sequence[int]], block_size: int,
+                 parents: Sequence[Sequence[int]], device, positions: Optional[Sequence[int]] = None) -> StepMeta:
+    """`prepare_attn` of a step whose rows are drafted trees: `parents[i]` lists the parent of every node of sequence i
+    (-1: the node hangs on the cached positions alone; a parent stands before its children). A node's rope position is
+    the sequence's `positions[i]` (default: its cached length; a cache that was cut down holds fewer rows than the
+    sequence has positions) plus the node's depth, its slot is cached_lens[i] + node."""
+    lib = _lib.load()
+    batch = len(lens)
+    if batch == 0 or len(parents) != batch or any(len(p) != int(l) for p, l in zip(parents, lens)):
+        raise RuntimeError("prepare_tree: one parent per node of every sequence expected")
+    flat = [int(x) for p in parents for x in p]
+    if not flat:
+        raise RuntimeError("prepare_tree: a step without nodes")
+    u32 = ctypes.c_uint32 * batch
+    words = max(1, (max(int(l) for l in lens) + 31) // 32)
+    host_parents = torch.tensor(flat, dtype=torch.int32)
+    mask = torch.empty(len(flat), words, dtype=torch.int32)
+    pos = torch.empty(len(flat), dtype=torch.int64)
+    base = cached_lens if positions is None else positions
+    _lib.check(lib.xlite_hip_prepare_tree(u32(*[int(x) for x in lens]), u32(*[int(x) for x in base]),
+                                          ctypes.c_void_p(host_parents.data_ptr()), batch, words,
+                                          ctypes.c_void_p(pos.data_ptr()), ctypes.c_void_p(mask.data_ptr())))
+    meta = prepare_attn(lens, cached_lens, block_tables, block_size, device, positions=pos)
+    meta.tree_mask, meta.parents = mask.to(device), host_parents.to(device)
+    return meta
+
+
 @dataclass
 class MhaConfig:
     hidden: int
@@ -100,7 +130,9 @@ class MhaLayer:
             raise RuntimeError("MhaLayer: qk_norm needs q_norm and k_norm")
 
     def forward(self, rt: _C.Runtime, hidden: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, meta: StepMeta,
-                cosin: torch.Tensor) -> torch.Tensor:
+                cosin: torch.Tensor, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """`weights` [num_blocks, block_size, n_kv_heads] fp32: accumulates what every cached position was attended to
+        (not for drafted trees, whose rows may not stand)."""
         c = self.cfg
         qkv = torch.matmul(hidden, self.wqkv)
         if self.bqkv is not None:
@@ -110,9 +142,21 @@ class MhaLayer:
             _C.qk_rms_norm(rt, qkv, self.q_norm, None, self.k_norm, None, qkv, c.norm_eps, c.head_dim, c.n_heads,
                            c.head_dim, c.n_kv_heads, c.n_heads * c.head_dim)
         attn = torch.empty(hidden.shape[0], c.n_heads * c.head_dim, dtype=hidden.dtype, device=hidden.device)
+        if meta.tree_mask is not None:
+            if weights is not None:
+                raise RuntimeError("MhaLayer: weights are not accumulated over drafted trees")
+            _C.rope_and_cache(rt, qkv, k_cache, v_cache, meta.position, cosin, meta.slot_mapping, c.n_heads, c.n_kv_heads,
+                              c.head_dim, c.rot_dim, c.block_size, True)
+            _C.tree_attention(rt, qkv, k_cache, v_cache, attn, meta.tree_mask, meta.query_start_loc, meta.lens,
+                              meta.cached_lens, meta.block_tables, c.n_heads, c.n_kv_heads, c.head_dim, c.block_size,
+                              meta.batch, meta.max_num_blocks)
+            return torch.matmul(attn, self.wo)
         # rope_and_cache, then attention (xlite/csrc/model.cpp:544-571), from one call into the library: a single
         # kernel launch for decode steps over short contexts, the two launches otherwise, the same bits either way
         _C.decode_step(rt, qkv, k_cache, v_cache, attn, meta.position, cosin, meta.slot_mapping, meta.query_start_loc,
                        meta.lens, meta.cached_lens, meta.block_tables, c.n_heads, c.n_kv_heads, c.head_dim, c.rot_dim,
                        c.block_size, meta.batch, meta.max_num_blocks)
+        if weights is not None:
+            _C.attention_weights(rt, qkv, k_cache, weights, meta.query_start_loc, meta.lens, meta.cached_lens, meta.block_tables,
+                                 c.n_heads, c.n_kv_heads, c.head_dim, c.block_size, meta.batch, meta.max_num_blocks)
         return torch.matmul(attn, self.wo)

@@ -32,6 +32,7 @@ extern "C" {
 /* element types (same order as xlite/csrc/base.h XDtype FP16/BF16) */
 #define XLITE_HIP_FP16 0
 #define XLITE_HIP_BF16 1
+#define XLITE_HIP_FP32 2 /* logits of verify_tree only */
 /* KV cache element types: the activation dtype, or int8 / fp8 (OCP e4m3) with fp32 scales */
 #define XLITE_HIP_KV_SAME 0
 #define XLITE_HIP_KV_INT8 1
@@ -433,6 +434,117 @@ int xlite_hip_attention_noalloc(void *stream, const void *qkv, const void *k_cac
                                 uint32_t head_dim, uint32_t block_size, uint32_t batch,
                                 uint32_t max_num_block, int dtype, int kv_dtype, const float *k_scale,
                                 const float *v_scale);
+
+/* ------------------------------------------------------------------------
+ * Drafted trees (speculative decoding; no counterpart in the reference). A step's rows are the
+ * nodes of one tree per sequence: node 0 is the sequence's last token, every other node a drafted
+ * one whose parent stands before it. Node n of sequence i sits at cache position
+ * cached_lens[i] + n (rope_and_cache has written it there, rotated for position
+ * cached_lens[i] + depth).
+ *
+ * prepare_tree: host arrays in, host arrays out. parents [sum lens]: a node's parent inside its
+ * sequence, -1 for a node that hangs on the cached positions alone; parents[n] < n (EINVAL
+ * otherwise). position [sum lens] = cached + depth (the tokens' rope positions), tree_mask
+ * [sum lens, mask_words]: bit n % 32 of word n / 32 of row r is set when node n is r or one of
+ * its ancestors. mask_words >= ceil(max lens / 32).
+ * ---------------------------------------------------------------------- */
+int xlite_hip_prepare_tree(const uint32_t *lens, const uint32_t *cached_lens, const int32_t *parents,
+                           uint32_t batch, uint32_t mask_words, int64_t *position, int32_t *tree_mask);
+
+/* ------------------------------------------------------------------------
+ * tree_attention - attention in which row r of sequence i sees every cached position
+ * 0 .. cached_lens[i] - 1 and, of the step's own positions cached_lens[i] + n (n < lens[i]), those
+ * whose bit n is set in its row of tree_mask [total_tokens, mask_words] (any mask: not only
+ * ancestors; bits from lens[i] on are ignored, nodes from 32 * mask_words on are seen by nobody).
+ * A row that sees nothing gets zeros. Infinities and NaNs in rows that a row does not see do not
+ * reach it. Everything else as in xlite_hip_attention (quantised caches: head_dim 64 or 128).
+ * workspace: xlite_hip_tree_attention_workspace_bytes(); with less the KV axis is not split
+ * (a batch over a quantised cache that needs a 16-bit copy fails with XLITE_HIP_ENOSPC).
+ * ---------------------------------------------------------------------- */
+size_t xlite_hip_tree_attention_workspace_bytes(uint32_t total_tokens, uint32_t n_heads,
+                                                uint32_t n_kv_heads, uint32_t head_dim,
+                                                uint32_t block_size, uint32_t batch,
+                                                uint32_t max_num_block, int kv_dtype);
+int xlite_hip_tree_attention(void *stream, const void *qkv, const void *k_cache, const void *v_cache,
+                             void *output, const int32_t *tree_mask, uint32_t mask_words,
+                             const int32_t *query_start_loc, const int32_t *lens,
+                             const int32_t *cached_lens, const int32_t *block_tables,
+                             uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
+                             uint32_t head_dim, uint32_t block_size, uint32_t batch,
+                             uint32_t max_num_block, int dtype, int kv_dtype, const float *k_scale,
+                             const float *v_scale, void *workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------
+ * verify_tree - the path of every sequence's tree that greedy decoding takes: from node 0 on, the
+ * token of the largest logit of the node's row (NaN above everything, the lowest index of equal
+ * ones); the path goes on at the lowest child node with that token, or ends and the token is the
+ * sequence's next one.
+ * logits       [total_tokens, vocab] fp16, bf16 or fp32
+ * tokens, parents [total_tokens] int32, as in prepare_tree (only children behind their parent count)
+ * accepted     [batch, max_path]: the path's nodes, 0 first, then -1; a path ends when it is full
+ * n_accepted   [batch]: its length (0 for a sequence without rows)
+ * next_token   [batch]: the model's token behind the path's last node (-1 without rows)
+ * accepted and n_accepted are the lists of compact_kv_cache with starts = cached_lens.
+ * ---------------------------------------------------------------------- */
+size_t xlite_hip_verify_tree_workspace_bytes(uint32_t total_tokens);
+int xlite_hip_verify_tree(void *stream, const void *logits, const int32_t *tokens, const int32_t *parents,
+                          int32_t *accepted, int32_t *n_accepted, int32_t *next_token,
+                          const int32_t *query_start_loc, const int32_t *lens, uint32_t total_tokens,
+                          uint32_t vocab, uint32_t batch, uint32_t max_path, int dtype, void *workspace,
+                          size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------
+ * attention_weights - what every cached position was attended to (no counterpart in the reference):
+ * weights [num_blocks, block_size, n_kv_heads] fp32; for position j of sequence i and kv head g
+ *   sum over the counted rows r and the heads of g of softmax(q_r . k)[j], row r seeing positions
+ *   0 .. cached_lens[i] + r as in attention,
+ * is added to the position's weight if j < cached_lens[i], and replaces it if the step itself
+ * appended the position. window: only the last `window` rows of every sequence count (0: all).
+ * Sums are fp32, in the same order in every run. A block may stand in one sequence's table only.
+ * Sequences without rows are left as they are. 16-bit caches, or quantised ones (K bytes and
+ * k_scale, head_dim 64 or 128). workspace: xlite_hip_attention_weights_workspace_bytes() (required).
+ * ---------------------------------------------------------------------- */
+size_t xlite_hip_attention_weights_workspace_bytes(uint32_t total_tokens, uint32_t n_heads,
+                                                   uint32_t n_kv_heads, uint32_t block_size,
+                                                   uint32_t batch, uint32_t max_num_block,
+                                                   uint32_t window);
+int xlite_hip_attention_weights(void *stream, const void *qkv, const void *k_cache, float *weights,
+                                const int32_t *query_start_loc, const int32_t *lens,
+                                const int32_t *cached_lens, const int32_t *block_tables,
+                                uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
+                                uint32_t head_dim, uint32_t block_size, uint32_t batch,
+                                uint32_t max_num_block, uint32_t window, int dtype, int kv_dtype,
+                                const float *k_scale, void *workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------
+ * select_kept - which positions a cache keeps. For sequence i with context_lens[i] cached positions
+ * and every kv head: all of them if they fit the budget; otherwise the first `sink`, the last
+ * `recent` and, of those between, the budget - sink - recent with the largest weights (NaN counts as
+ * the largest; equal weights: the lower position). recent + sink <= budget.
+ * kept      [batch, n_kv_heads, budget]: positions in ascending order, then -1
+ * kept_lens [batch] = min(context_lens, budget)
+ * ---------------------------------------------------------------------- */
+int xlite_hip_select_kept(void *stream, const float *weights, int32_t *kept, int32_t *kept_lens,
+                          const int32_t *context_lens, const int32_t *block_tables, uint32_t n_kv_heads,
+                          uint32_t block_size, uint32_t batch, uint32_t max_num_block, uint32_t budget,
+                          uint32_t recent, uint32_t sink);
+
+/* ------------------------------------------------------------------------
+ * compact_kv_cache - moves cache rows to the front, in place: position starts[i] + n of sequence i
+ * receives the rows that position starts[i] + kept[n] held before the call, n < kept_lens[i] (at
+ * most max_kept). kept[n] >= n (as in any ascending list); other entries, and positions outside
+ * the block table, are ignored.
+ * kept   [batch, n_kv_heads, max_kept] (per_head != 0) or [batch, max_kept] (one list for all heads)
+ * starts [batch] or NULL (0)
+ * K and V rows, and with them k_scale / v_scale (quantised caches) and, if not NULL, weights
+ * [num_blocks, block_size, n_kv_heads]. Rows not named by n < kept_lens[i] stay as they are.
+ * A block may stand in one sequence's table only. head_dim x element size: a multiple of 16 bytes.
+ * ---------------------------------------------------------------------- */
+int xlite_hip_compact_kv_cache(void *stream, void *k_cache, void *v_cache, float *k_scale, float *v_scale,
+                               float *weights, const int32_t *kept, const int32_t *kept_lens,
+                               const int32_t *starts, const int32_t *block_tables, uint32_t n_kv_heads,
+                               uint32_t head_dim, uint32_t block_size, uint32_t batch,
+                               uint32_t max_num_block, uint32_t max_kept, int per_head, int kv_dtype);
 
 #ifdef __cplusplus
 }
