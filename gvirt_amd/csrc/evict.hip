@@ -11,19 +11,22 @@ namespace {
 // ---- select_kept ------------------------------------------------------------------------------------------------------
 // Per (sequence, kv head): the first `sink` and the last `recent` positions, and of the positions between them the n =
 // budget - sink - recent with the largest weights; equal weights go to the lower position. A radix selection: the n-th
-// largest key is found 8 bits at a time with a histogram in LDS, then one pass in position order writes the positions
-// whose key is larger, and the first ones that equal it. Counts only, so the result does not depend on any order.
+// largest key is found 8 bits at a time with histograms in LDS (one per wave: most weights share their top byte), then the
+// positions whose key is larger, and the first ones that equal it, are written in position order. Counts only, so the result
+// does not depend on any order. One workgroup per (sequence, kv head); the keys are read once, into registers.
+// A weight's neighbours in memory belong to the other kv heads: the heads of a sequence run on one XCD, at the same time, so
+// that its lines come from memory once and from that XCD's L2 for the other heads.
 constexpr int kSelThreads = 1024;
+constexpr int kSelWaves = kSelThreads / 64;
+constexpr uint32_t kXcds = 8;
 
-// weights in the order of a descending sort: NaN first, -0 and +0 alike
+// weights in the order of a descending sort: NaN first, -0 and +0 alike; never 0, which stands for "no weight"
 __device__ __forceinline__ uint32_t weight_key(float w)
 {
     w += 0.0f;
-    if (w != w) {
-        return 0xffffffffu;
-    }
     const uint32_t b = __builtin_bit_cast(uint32_t, w);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t k = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+    return w != w ? 0xffffffffu : k;
 }
 
 struct SelectParams {
@@ -32,20 +35,88 @@ struct SelectParams {
     int32_t *kept_lens;
     const int32_t *context_lens;
     const int32_t *block_tables;
-    uint32_t n_kv_heads, block_size, max_num_block, budget, recent, sink;
+    uint32_t n_kv_heads, block_size, max_num_block, budget, recent, sink, batch;
+    uint32_t block_magic;   // floor(2^32 / block_size) + 1 while positions * block_size stay below 2^32, otherwise 0
 };
 
+// The n-th largest of the keys (n > 0, at least n of them) and how many of those equal to it are among the n largest.
+// each(f) calls f for every key of the thread (0: none).
+template <typename EACH>
+__device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, uint32_t (*hist)[256], uint32_t *found, uint32_t *threshold, uint32_t *equal)
+{
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t left = n, prefix = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            hist[wave][lane + 64 * i] = 0;
+        }
+        // (a wave's own histogram: its LDS operations are carried out in order)
+        each([&](uint32_t k) {
+            const bool in = shift == 24 ? k != 0 : (k >> (shift + 8)) == prefix;
+            if (in) {
+                atomicAdd(&hist[wave][(k >> shift) & 255u], 1u);
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x < 256) {
+            uint32_t sum = 0;
+#pragma unroll
+            for (int w = 0; w < kSelWaves; w++) {
+                sum += hist[w][threadIdx.x];
+            }
+            hist[0][threadIdx.x] = sum;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            // lane l: bins 255 - 4 l .. 252 - 4 l, in descending order
+            uint32_t c[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                c[e] = hist[0][255 - 4 * lane - e];
+                sum += c[e];
+            }
+            uint32_t incl = sum;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t up = __shfl_up(incl, d);
+                incl += lane >= static_cast<uint32_t>(d) ? up : 0u;
+            }
+            uint32_t above = incl - sum;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (above < left && left <= above + c[e]) {   // exactly one bin of one lane
+                    found[0] = 255 - 4 * lane - e;
+                    found[1] = above;
+                }
+                above += c[e];
+            }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | found[0];
+        left -= found[1];
+    }
+    *threshold = prefix;
+    *equal = left;
+}
+
+// KPT: keys a thread holds in registers (the context fits KPT * 1024 positions); 0: any length, the keys are read again in
+// every pass
+template <int KPT>
 __global__ void __launch_bounds__(kSelThreads)
 select_kept_kernel(const SelectParams p)
 {
-    constexpr int WAVES = kSelThreads / 64;
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t found[2];            // the digit, and how many keys of the bins above it were taken
-    __shared__ uint2 wave_count[WAVES];
-    const uint32_t seq = blockIdx.x / p.n_kv_heads, kvh = blockIdx.x % p.n_kv_heads;
+    __shared__ uint32_t hist[kSelWaves][256];
+    __shared__ uint32_t found[2];            // the digit, and how many keys lie in the bins above it
+    __shared__ uint2 counts[(KPT > 0 ? KPT : 1) * kSelWaves];   // (above, equal) of a wave's 64 positions, then the sums before them
+    const uint32_t xcd = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
+    const uint32_t seq = place / p.n_kv_heads * kXcds + xcd, kvh = place % p.n_kv_heads;
+    if (seq >= p.batch) {
+        return;
+    }
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t length = min(static_cast<uint32_t>(max(p.context_lens[seq], 0)), p.max_num_block * p.block_size);
-    int32_t *out = p.kept + static_cast<uint64_t>(blockIdx.x) * p.budget;
+    int32_t *out = p.kept + (static_cast<uint64_t>(seq) * p.n_kv_heads + kvh) * p.budget;
     const uint32_t count = min(length, p.budget);
     if (kvh == 0 && threadIdx.x == 0) {
         p.kept_lens[seq] = static_cast<int32_t>(count);
@@ -61,60 +132,12 @@ select_kept_kernel(const SelectParams p)
     }
     const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
     auto key_at = [&](uint32_t pos) {
-        const uint32_t b = pos / p.block_size;
+        const uint32_t b = p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size;
         const uint64_t slot = static_cast<uint64_t>(static_cast<uint32_t>(table[b])) * p.block_size + (pos - b * p.block_size);
         return weight_key(p.weights[slot * p.n_kv_heads + kvh]);
     };
     const uint32_t lo = p.sink, hi = length - p.recent;   // the judged positions
     const uint32_t n = p.budget - p.sink - p.recent;      // fewer than hi - lo: length > budget
-    // ---- the n-th largest key, and how many of the keys equal to it are taken
-    uint32_t threshold = 0, equal = 0;
-    if (n > 0) {
-        uint32_t left = n, prefix = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (threadIdx.x < 256) {
-                hist[threadIdx.x] = 0;
-            }
-            __syncthreads();
-            for (uint32_t i = lo + threadIdx.x; i < hi; i += kSelThreads) {
-                const uint32_t k = key_at(i);
-                if (shift == 24 || (k >> (shift + 8)) == prefix) {
-                    atomicAdd(&hist[(k >> shift) & 255u], 1u);
-                }
-            }
-            __syncthreads();
-            if (wave == 0) {
-                // lane l: bins 255 - 4 l .. 252 - 4 l, in descending order
-                uint32_t c[4], sum = 0;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    c[e] = hist[255 - 4 * lane - e];
-                    sum += c[e];
-                }
-                uint32_t incl = sum;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const uint32_t up = __shfl_up(incl, d);
-                    incl += lane >= static_cast<uint32_t>(d) ? up : 0u;
-                }
-                uint32_t above = incl - sum;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (above < left && left <= above + c[e]) {   // exactly one bin of one lane
-                        found[0] = 255 - 4 * lane - e;
-                        found[1] = above;
-                    }
-                    above += c[e];
-                }
-            }
-            __syncthreads();
-            prefix = prefix << 8 | found[0];
-            left -= found[1];
-        }
-        threshold = prefix;
-        equal = left;
-    }
-    // ---- the kept positions in order
     for (uint32_t i = threadIdx.x; i < p.sink; i += kSelThreads) {
         out[i] = static_cast<int32_t>(i);
     }
@@ -124,31 +147,97 @@ select_kept_kernel(const SelectParams p)
     if (n == 0) {
         return;
     }
-    uint32_t above_before = 0, equal_before = 0;
-    for (uint32_t i0 = lo; i0 < hi; i0 += kSelThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        const uint32_t k = key_at(min(i, hi - 1));
-        const bool is_above = i < hi && k > threshold, is_equal = i < hi && k == threshold;
-        const uint64_t above_mask = __ballot(is_above), equal_mask = __ballot(is_equal);
-        __syncthreads();
-        if (lane == 0) {
-            wave_count[wave] = make_uint2(__builtin_popcountll(above_mask), __builtin_popcountll(equal_mask));
-        }
-        __syncthreads();
-        uint32_t a = above_before, e = equal_before;
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t threshold, equal;
+    if constexpr (KPT > 0) {
+        uint32_t key[KPT];
 #pragma unroll
-        for (uint32_t w = 0; w < WAVES; w++) {
-            const uint2 c = wave_count[w];
-            a += w < wave ? c.x : 0u;
-            e += w < wave ? c.y : 0u;
-            above_before += c.x;
-            equal_before += c.y;
+        for (int j = 0; j < KPT; j++) {
+            const uint32_t i = lo + j * kSelThreads + threadIdx.x;
+            key[j] = key_at(min(i, hi - 1));
+            key[j] = i < hi ? key[j] : 0u;
         }
-        const uint64_t below = (1ull << lane) - 1;
-        a += __builtin_popcountll(above_mask & below);
-        e += __builtin_popcountll(equal_mask & below);
-        if (is_above || (is_equal && e < equal)) {
-            out[p.sink + a + min(e, equal)] = static_cast<int32_t>(i);
+        nth_largest([&](auto &&f) {
+#pragma unroll
+            for (int j = 0; j < KPT; j++) {
+                f(key[j]);
+            }
+        }, n, hist, found, &threshold, &equal);
+#pragma unroll
+        for (int j = 0; j < KPT; j++) {
+            const uint64_t a = __ballot(key[j] > threshold), e = __ballot(key[j] == threshold);
+            if (lane == 0) {
+                counts[j * kSelWaves + wave] = make_uint2(__builtin_popcountll(a), __builtin_popcountll(e));
+            }
+        }
+        __syncthreads();
+        if (wave == 0) {   // exclusive sums in position order: lane l owns KPT / 4 consecutive entries
+            constexpr int PER = (KPT * kSelWaves + 63) / 64;
+            uint2 sum = make_uint2(0, 0);
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const uint2 c = counts[lane * PER + i];
+                sum.x += c.x;
+                sum.y += c.y;
+            }
+            uint2 incl = sum;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t ux = __shfl_up(incl.x, d), uy = __shfl_up(incl.y, d);
+                incl.x += lane >= static_cast<uint32_t>(d) ? ux : 0u;
+                incl.y += lane >= static_cast<uint32_t>(d) ? uy : 0u;
+            }
+            uint2 before = make_uint2(incl.x - sum.x, incl.y - sum.y);
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const uint2 c = counts[lane * PER + i];
+                counts[lane * PER + i] = before;
+                before.x += c.x;
+                before.y += c.y;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < KPT; j++) {
+            const bool is_above = key[j] > threshold, is_equal = key[j] == threshold;
+            const uint64_t am = __ballot(is_above), em = __ballot(is_equal);
+            const uint2 before = counts[j * kSelWaves + wave];
+            const uint32_t a = before.x + __builtin_popcountll(am & below), e = before.y + __builtin_popcountll(em & below);
+            if (is_above || (is_equal && e < equal)) {
+                out[p.sink + a + min(e, equal)] = static_cast<int32_t>(lo + j * kSelThreads + threadIdx.x);
+            }
+        }
+    } else {
+        nth_largest([&](auto &&f) {
+            for (uint32_t i = lo + threadIdx.x; i < hi; i += kSelThreads) {
+                f(key_at(i));
+            }
+        }, n, hist, found, &threshold, &equal);
+        uint32_t above_before = 0, equal_before = 0;
+        for (uint32_t i0 = lo; i0 < hi; i0 += kSelThreads) {
+            const uint32_t i = i0 + threadIdx.x;
+            const uint32_t k = key_at(min(i, hi - 1));
+            const bool is_above = i < hi && k > threshold, is_equal = i < hi && k == threshold;
+            const uint64_t above_mask = __ballot(is_above), equal_mask = __ballot(is_equal);
+            __syncthreads();
+            if (lane == 0) {
+                counts[wave] = make_uint2(__builtin_popcountll(above_mask), __builtin_popcountll(equal_mask));
+            }
+            __syncthreads();
+            uint32_t a = above_before, e = equal_before;
+#pragma unroll
+            for (uint32_t w = 0; w < kSelWaves; w++) {
+                const uint2 c = counts[w];
+                a += w < wave ? c.x : 0u;
+                e += w < wave ? c.y : 0u;
+                above_before += c.x;
+                equal_before += c.y;
+            }
+            a += __builtin_popcountll(above_mask & below);
+            e += __builtin_popcountll(equal_mask & below);
+            if (is_above || (is_equal && e < equal)) {
+                out[p.sink + a + min(e, equal)] = static_cast<int32_t>(i);
+            }
         }
     }
 }
@@ -156,11 +245,11 @@ select_kept_kernel(const SelectParams p)
 // ---- compact_kv_cache ---------------------------------------------------------------------------------------------------
 // Position start + i of a sequence receives the row of position start + kept[i], kept[i] >= i, in place. The columns of a
 // row are independent, so a workgroup owns a slice of the rows' bytes (or one fp32 per row: scales, weights) and walks the
-// list in order, kBatch entries at a time: all of a batch is read before any of it is written, and what later batches read
-// lies above everything written so far (kept[i] >= i), so one barrier per batch is all the order there is. Bound by
-// memory: every moved row is read and written once.
-constexpr int kMoveThreads = 256;
+// list in order, a batch of entries at a time: all of a batch is read before any of it is written (a barrier), and what later
+// batches read lies above everything written so far (kept[i] >= i), so the next batch is read ahead of that barrier. Bound
+// by memory: every moved row is read and written once.
 constexpr int kMoveUnroll = 4;
+constexpr uint32_t kMoveTable = 4096;   // block-table entries kept in LDS (longer tables are read from memory)
 
 struct CompactParams {
     unsigned char *k_cache, *v_cache;
@@ -170,6 +259,7 @@ struct CompactParams {
     const int32_t *starts;              // nullptr: 0
     const int32_t *block_tables;
     uint32_t n_kv_heads, block_size, max_num_block, max_kept;
+    uint32_t block_magic;               // as in SelectParams
     uint32_t per_head;                  // 1: a list per kv head, 0: one for all of them
     uint32_t row_bytes;                 // of a cache row that moves as one: a kv head's, or a position's
     uint32_t slices;                    // of a cache row
@@ -178,69 +268,102 @@ struct CompactParams {
 };
 
 // the walk: `lanes` threads per row, each with its own V at `column`
-template <typename V>
-__device__ __forceinline__ void move_rows(const CompactParams &p, V *data, uint64_t pitch, uint64_t column, uint32_t lanes,
-                                          const int32_t *list, uint32_t count, uint32_t start, const int32_t *table)
+template <typename V, typename ROW>
+__device__ __forceinline__ void move_rows(V *data, uint64_t pitch, uint64_t column, uint32_t lanes, const int32_t *list, uint32_t count,
+                                          uint32_t start, uint32_t capacity, ROW &&row_of)
 {
-    const uint32_t rows = kMoveThreads / lanes;          // rows of one instruction
+    constexpr int U = kMoveUnroll;
+    const uint32_t rows = blockDim.x / lanes;          // rows of one instruction
     const uint32_t mine = threadIdx.x / lanes;
-    const uint32_t capacity = p.max_num_block * p.block_size;
-    const uint64_t at = column + threadIdx.x % lanes;
-    auto row_of = [&](uint32_t pos) {
-        const uint32_t b = pos / p.block_size;
-        return static_cast<uint64_t>(static_cast<uint32_t>(table[b])) * p.block_size + (pos - b * p.block_size);
-    };
-    for (uint32_t i0 = 0; i0 < count; i0 += rows * kMoveUnroll) {
-        uint32_t src[kMoveUnroll];
-        bool ok[kMoveUnroll];
-        V x[kMoveUnroll];
+    V *base = data + column + threadIdx.x % lanes;
+    const uint32_t batch = rows * U;
+    uint32_t src[U];
+    V x[U], y[U];
+    bool ok[U], ok_next[U];
+    auto read_list = [&](uint32_t i0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; u++) {
-            const uint32_t i = i0 + u * rows + mine;
-            src[u] = static_cast<uint32_t>(list[min(i, count - 1)]);
-            // (a row that stays where it is, and entries that break the rules: nothing is read or written)
-            ok[u] = i < count && src[u] > i && src[u] < capacity - start;
+        for (int u = 0; u < U; u++) {
+            src[u] = static_cast<uint32_t>(list[min(i0 + u * rows + mine, count - 1)]);
         }
+    };
+    // (a row that stays where it is, and entries that break the rules: nothing is written, and the load is one of the row
+    // that stands there, whatever it holds)
+    auto read_rows = [&](uint32_t i0, V (&v)[U], bool (&good)[U]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; u++) {
-            if (ok[u]) {
-                x[u] = data[row_of(start + src[u]) * pitch + at];
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + u * rows + mine;
+            good[u] = i < count && src[u] > i && src[u] < capacity - start;
+            v[u] = base[row_of(start + (good[u] ? src[u] : 0u)) * pitch];
+        }
+    };
+    read_list(0);
+    read_rows(0, x, ok);
+    read_list(min(batch, count - 1));
+    for (uint32_t i0 = 0; i0 < count; i0 += batch) {
+        read_rows(i0 + batch, y, ok_next);
+        read_list(min(i0 + 2 * batch, count - 1));
+        // this batch's values are here, not only asked for, before anyone writes
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if constexpr (sizeof(V) == 16) {
+                asm volatile("" : "+v"(x[u].x), "+v"(x[u].y), "+v"(x[u].z), "+v"(x[u].w));
+            } else {
+                asm volatile("" : "+v"(x[u]));
             }
         }
-        __builtin_amdgcn_s_waitcnt(0);   // the values are here, not only asked for, before anyone writes
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kMoveUnroll; u++) {
-            if (ok[u]) {
-                data[row_of(start + i0 + u * rows + mine) * pitch + at] = x[u];
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + u * rows + mine;
+            if (ok[u] && start + i < capacity) {
+                base[row_of(start + i) * pitch] = x[u];
             }
+            x[u] = y[u];
+            ok[u] = ok_next[u];
         }
     }
 }
 
-__global__ void __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(1024)
 compact_kernel(const CompactParams p)
 {
+    __shared__ uint32_t table_lds[kMoveTable];
     const uint32_t lists = p.per_head ? p.n_kv_heads : 1u;
     const uint32_t seq = blockIdx.y / lists, head = blockIdx.y % lists;
     const uint32_t count = min(static_cast<uint32_t>(max(p.kept_lens[seq], 0)), p.max_kept);
     const uint32_t start = p.starts != nullptr ? static_cast<uint32_t>(max(p.starts[seq], 0)) : 0u;
-    if (count == 0 || start >= p.max_num_block * p.block_size) {
+    const uint32_t capacity = p.max_num_block * p.block_size;
+    if (count == 0 || start >= capacity) {
         return;
     }
     const int32_t *list = p.kept + static_cast<uint64_t>(blockIdx.y) * p.max_kept;
     const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
     const uint32_t part = blockIdx.x;
+    const uint32_t first = start / p.block_size;
+    for (uint32_t i = threadIdx.x; i < min(p.max_num_block - first, kMoveTable); i += blockDim.x) {
+        table_lds[i] = static_cast<uint32_t>(table[first + i]);
+    }
+    __syncthreads();
+    auto row_of = [&](uint32_t pos) {
+        const uint32_t b = p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size;
+        const uint32_t entry = b - first < kMoveTable ? table_lds[b - first] : static_cast<uint32_t>(table[b]);
+        return static_cast<uint64_t>(entry) * p.block_size + (pos - b * p.block_size);
+    };
     if (part < 2 * p.slices) {
         unsigned char *cache = part < p.slices ? p.k_cache : p.v_cache;
         const uint64_t pitch = static_cast<uint64_t>(p.row_bytes) * (p.per_head ? p.n_kv_heads : 1u) / 16;
         const uint64_t column = (static_cast<uint64_t>(head) * p.row_bytes + (part % p.slices) * p.slice_bytes) / 16;
-        move_rows<uint4>(p, reinterpret_cast<uint4 *>(cache), pitch, column, p.slice_bytes / 16, list, count, start, table);
+        move_rows<uint4>(reinterpret_cast<uint4 *>(cache), pitch, column, p.slice_bytes / 16, list, count, start, capacity, row_of);
     } else {
         const uint32_t c = part - 2 * p.slices;
         const uint32_t per_array = p.per_head ? 1u : p.n_kv_heads;
-        move_rows<float>(p, p.scalars[c / per_array], p.n_kv_heads, p.per_head ? head : c % per_array, 1, list, count, start, table);
+        move_rows<float>(p.scalars[c / per_array], p.n_kv_heads, p.per_head ? head : c % per_array, 1, list, count, start, capacity, row_of);
     }
+}
+
+uint32_t magic_of(uint32_t block_size, uint32_t max_num_block)
+{
+    return static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32) ? static_cast<uint32_t>((1ull << 32) / block_size) + 1 : 0u;
 }
 
 }  // namespace
@@ -262,9 +385,22 @@ extern "C" int xlite_hip_select_kept(void *stream, const float *weights, int32_t
     XL_REQUIRE(static_cast<uint64_t>(max_num_block) * block_size < (1ull << 31), "block tables reach beyond 2^31 positions");
     XL_REQUIRE(budget > 0 && budget < (1u << 31), "budget must be positive");
     XL_REQUIRE(static_cast<uint64_t>(recent) + sink <= budget, "recent + sink must not exceed budget");
-    XL_REQUIRE(static_cast<uint64_t>(batch) * n_kv_heads < (1ull << 31), "more lists than one launch takes");
-    SelectParams p{weights, kept, kept_lens, context_lens, block_tables, n_kv_heads, block_size, max_num_block, budget, recent, sink};
-    select_kept_kernel<<<batch * n_kv_heads, kSelThreads, 0, as_stream(stream)>>>(p);
+    XL_REQUIRE((static_cast<uint64_t>(batch) + kXcds) * n_kv_heads < (1ull << 31), "more lists than one launch takes");
+    SelectParams p{weights, kept, kept_lens, context_lens, block_tables, n_kv_heads, block_size, max_num_block,
+                   budget, recent, sink, batch, magic_of(block_size, max_num_block)};
+    const uint64_t grid = (static_cast<uint64_t>(batch) + kXcds - 1) / kXcds * kXcds * n_kv_heads;
+    const uint32_t judged = max_num_block * block_size - std::min(max_num_block * block_size, sink + recent);   // at most
+    hipStream_t s = as_stream(stream);
+    const dim3 g(static_cast<uint32_t>(grid));
+    if (judged <= 4 * kSelThreads) {
+        select_kept_kernel<4><<<g, kSelThreads, 0, s>>>(p);
+    } else if (judged <= 16 * kSelThreads) {
+        select_kept_kernel<16><<<g, kSelThreads, 0, s>>>(p);
+    } else if (judged <= 40 * kSelThreads) {
+        select_kept_kernel<40><<<g, kSelThreads, 0, s>>>(p);
+    } else {
+        select_kept_kernel<0><<<g, kSelThreads, 0, s>>>(p);
+    }
     XL_LAUNCH_CHECK();
     return XLITE_HIP_OK;
 }
@@ -303,8 +439,9 @@ extern "C" int xlite_hip_compact_kv_cache(void *stream, void *k_cache, void *v_c
     const uint64_t row = head_bytes * (per_head ? 1u : n_kv_heads);
     XL_REQUIRE(row < (1ull << 31), "a position's row is too long");
     p.row_bytes = static_cast<uint32_t>(row);
-    // slices of 128 bytes (a cache line), or less where the row is no multiple of it
-    p.slice_bytes = row % 128 == 0 ? 128u : row % 64 == 0 ? 64u : row % 32 == 0 ? 32u : 16u;
+    p.block_magic = magic_of(block_size, max_num_block);
+    // slices of 256 bytes, or the largest power of two below that divides the row
+    p.slice_bytes = std::min(256u, p.row_bytes & (~p.row_bytes + 1u));
     p.slices = p.row_bytes / p.slice_bytes;
     uint32_t arrays = 0;
     for (float *x : {kv_dtype == XLITE_HIP_KV_SAME ? nullptr : k_scale, kv_dtype == XLITE_HIP_KV_SAME ? nullptr : v_scale, weights}) {
@@ -315,7 +452,9 @@ extern "C" int xlite_hip_compact_kv_cache(void *stream, void *k_cache, void *v_c
     p.n_scalars = arrays * (per_head ? 1u : n_kv_heads);
     const uint64_t lists = static_cast<uint64_t>(batch) * (per_head ? n_kv_heads : 1u);
     XL_REQUIRE(lists <= 65535, "more lists than one launch takes");
-    compact_kernel<<<dim3(2 * p.slices + p.n_scalars, static_cast<uint32_t>(lists)), kMoveThreads, 0, as_stream(stream)>>>(p);
+    // long lists: 16 waves keep a compute unit's share of the memory busy; a path's few rows fit 4
+    const uint32_t threads = max_kept > 64 ? 1024u : 256u;
+    compact_kernel<<<dim3(2 * p.slices + p.n_scalars, static_cast<uint32_t>(lists)), threads, 0, as_stream(stream)>>>(p);
     XL_LAUNCH_CHECK();
     return XLITE_HIP_OK;
 }
