@@ -772,7 +772,8 @@ def attention_weights(rt: Runtime, qkv: torch.Tensor, k_cache: torch.Tensor, wei
     _on(rt, name, "weights", weights, torch.float32)
     _req(weights.numel() * head_dim == k_cache.numel(), "attention_weights: one weight per (block, slot, kv head) expected")
     _req(window >= 0, "attention_weights: window must not be negative")
-    need = rt._lib.xlite_hip_attention_weights_workspace_bytes(T, n_heads, n_kv_heads, block_size, batch, max_num_block, window)
+    need = rt._lib.xlite_hip_attention_weights_workspace_bytes(T, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block,
+                                                                   window)
     ws = rt.workspace(need)
     rt.call("xlite_hip_attention_weights", rt.stream(), _ptr(qkv), _ptr(k_cache), _ptr(weights), _ptr(query_start_loc), _ptr(lens),
             _ptr(cached_lens), _ptr(block_tables), T, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, window, dt, kv,

@@ -47,7 +47,7 @@ SIGNATURES = {
     "xlite_hip_tree_attention": (_i32, [_vp] * 6 + [_u32] + [_vp] * 4 + [_u32] * 7 + [_i32, _i32] + [_vp] * 3 + [_sz]),
     "xlite_hip_verify_tree_workspace_bytes": (_sz, [_u32]),
     "xlite_hip_verify_tree": (_i32, [_vp] * 9 + [_u32] * 4 + [_i32, _vp, _sz]),
-    "xlite_hip_attention_weights_workspace_bytes": (_sz, [_u32] * 7),
+    "xlite_hip_attention_weights_workspace_bytes": (_sz, [_u32] * 8),
     "xlite_hip_attention_weights": (_i32, [_vp] * 8 + [_u32] * 8 + [_i32, _i32, _vp, _vp, _sz]),
     "xlite_hip_select_kept": (_i32, [_vp] * 6 + [_u32] * 7),
     "xlite_hip_compact_kv_cache": (_i32, [_vp] * 10 + [_u32] * 6 + [_i32, _i32]),

@@ -3,13 +3,14 @@
 // (c cached positions; row r sees positions 0 .. c + r; j <= c + r). Positions of the step itself start at zero, older ones
 // keep what earlier steps left. No value of V is involved.
 //
-// Two kernels over the scores, which are formed twice instead of stored (a chunk of 2048 rows behind 6144 positions has
-// 0.9 G of them, 3.7 GB in fp32):
-//   row statistics: log2 of every row's normaliser. A wave owns 32 M rows (an M row: a counted row and one query head of the
+// A batch of few rows per sequence (decode steps, short windows) is bound by reading K: the scores are formed once, stored in
+// fp32 (a few per cent of the bytes of K) with every row's maximum and sum per chunk of positions, and summed up in a second
+// pass over them. A batch of many rows is bound by the exponentials and forms the scores twice instead of storing them (a
+// chunk of 2048 rows behind 6144 positions has 0.9 G of them, 3.7 GB in fp32):
+//   row statistics: log2 of every row's normaliser. A wave owns 64 M rows (an M row: a counted row and one query head of the
 //     kv head) as the columns of S^T = K Q^T, so a row's running maximum and sum live in one lane pair.
-//   column sums: a wave owns 32 positions as the columns of S = Q K^T and walks the M rows, so a position's sum lives in
-//     one lane pair: no atomics, one owner per weight, the same order of additions in every run.
-// Both are bound by the exponentials (one per score in each) and the vector instructions around them.
+//   column sums: a wave owns 64 positions as the columns of S = Q K^T and walks the M rows, so a position's sum lives in one
+//     lane pair: no atomics, one owner per weight, the same order of additions in every run.
 #include <algorithm>
 #include <type_traits>
 
@@ -21,11 +22,13 @@ namespace xlite {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
-constexpr uint32_t kRowTile = kWaves * 32;    // M rows of a workgroup of the first kernel
-constexpr uint32_t kPosTile = kWaves * 32;    // positions of a workgroup of the second one
-constexpr uint32_t kMinSplit = 256;           // positions a split of the first kernel walks at least
+constexpr int kThreads = 256;
+constexpr uint32_t kRowTile = 4 * 64;         // M rows of a workgroup of the row statistics
+// tiles of 32 positions that a wave of the column sums owns (head_dim 256: the registers hold one)
+template <int D>
+constexpr int kPosTiles = D == 256 ? 1 : 2;
+constexpr uint32_t kMinSplit = 256;           // positions a split of the row statistics walks at least
+constexpr uint32_t kStoredRows = 32;          // M rows per sequence, on average, up to which the scores are stored
 
 template <typename T>
 __device__ __forceinline__ f32x16_t mfma32(const uint4 &a, const uint4 &b, f32x16_t c)
@@ -54,6 +57,9 @@ struct WeightsParams {
     uint32_t tiles_per_seq;        // row tiles of a sequence when a window bounds them (0: ids from the prefix sums)
     uint32_t m_total;              // total_tokens * G
     uint32_t splits, split_len;
+    uint32_t block_magic;          // floor(2^32 / block_size) + 1 while positions * block_size stay below 2^32, otherwise 0
+    float *scores;                 // stored scores: [kv head][M row][pitch], in units of log2
+    uint32_t pitch;                // positions of a stored row, a multiple of 64
 };
 
 // what a workgroup knows about its sequence
@@ -75,7 +81,7 @@ __device__ __forceinline__ Sequence sequence_of(const WeightsParams &p, uint32_t
 
 __device__ __forceinline__ uint64_t slot_of(const WeightsParams &p, const int32_t *table, uint32_t pos)
 {
-    const uint32_t b = pos / p.block_size;
+    const uint32_t b = p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size;
     return static_cast<uint64_t>(static_cast<uint32_t>(table[b])) * p.block_size + (pos - b * p.block_size);
 }
 
@@ -90,14 +96,31 @@ __device__ __forceinline__ uint4 cache_chunk(const unsigned char *row, uint32_t 
     }
 }
 
+// M row m of a sequence, walked in steps of 32: token and head without a division per step
+struct RowCursor {
+    uint32_t r, h, dr, dh, group;
+    __device__ __forceinline__ RowCursor(uint32_t m, uint32_t g) : r(m / g), h(m - m / g * g), dr(32u / g), dh(32u - 32u / g * g), group(g) {}
+    __device__ __forceinline__ void step()
+    {
+        h += dh;
+        r += dr;
+        const bool over = h >= group;
+        h -= over ? group : 0u;
+        r += over ? 1u : 0u;
+    }
+};
+
 template <typename T, int D, int KVF>
 __global__ void __launch_bounds__(kThreads)
 row_stats_kernel(const WeightsParams p)
 {
     constexpr int KS = D / 16;
-    constexpr uint32_t ROWB = D * (KVF == XLITE_HIP_KV_SAME ? 2 : 1);
+    constexpr int RT = D == 256 ? 1 : 2;      // tiles of 32 rows of a wave (head_dim 256: the registers hold one)
+    constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
+    constexpr uint32_t ROWB = D * (KV8 ? 1 : 2);
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.z, split = blockIdx.y, G = p.group;
+    constexpr uint32_t TILE = 4 * 32 * RT;
 
     // ---- which rows: the tiles of a sequence are numbered from floor(start * G / tile) + i (a formula of the prefix sums,
     // at least as many ids as it has tiles), or evenly when a window bounds the counted rows
@@ -107,7 +130,7 @@ row_stats_kernel(const WeightsParams p)
         mt = blockIdx.x % p.tiles_per_seq;
     } else {
         auto first_id = [&](uint32_t i) {
-            return static_cast<uint32_t>(static_cast<uint64_t>(p.query_start_loc[i]) * G / kRowTile) + i;
+            return static_cast<uint32_t>(static_cast<uint64_t>(p.query_start_loc[i]) * G / TILE) + i;
         };
         uint32_t hi = p.batch;
         while (hi - seq > 1) {
@@ -121,81 +144,127 @@ row_stats_kernel(const WeightsParams p)
         mt = blockIdx.x - first_id(seq);
     }
     const Sequence s = sequence_of(p, seq);
-    const uint32_t m_wave = mt * kRowTile + wave * 32;
+    const uint32_t m_wave = mt * TILE + wave * 32 * RT;
     if (m_wave >= s.m_rows) {
         return;
     }
-    const uint32_t m = min(m_wave + col, s.m_rows - 1);
-    const uint32_t r = s.first + m / G;
-    const uint32_t vis = s.cached + r + 1;                                       // of this lane's row
+    uint32_t vis[RT];                                                            // of this lane's rows
     const uint32_t vis_first = s.cached + s.first + m_wave / G + 1;              // of the wave's first row, the least
-    const uint32_t vis_last = s.cached + s.first + min(m_wave + 31, s.m_rows - 1) / G + 1;
+    const uint32_t vis_last = s.cached + s.first + min(m_wave + 32 * RT - 1, s.m_rows - 1) / G + 1;
     const uint32_t begin = split * p.split_len, end = min(vis_last, begin + p.split_len);
     const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
 
-    float m_run = -INFINITY, l_run = 0.f;
-    if (begin < end) {
-        uint4 qreg[KS];
+    float m_run[RT], l_run[RT];
+    uint4 qreg[RT][KS];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const uint32_t m = min(m_wave + rt * 32 + col, s.m_rows - 1);
+        const uint32_t r = s.first + m / G;
+        vis[rt] = s.cached + r + 1;
+        m_run[rt] = -INFINITY;
+        l_run[rt] = 0.f;
         const uint16_t *src = p.q + static_cast<uint64_t>(s.start + r) * p.q_tok_stride + static_cast<uint64_t>(kvh * G + m % G) * D;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            qreg[ks] = *reinterpret_cast<const uint4 *>(src + ks * 16 + half * 8);
+            qreg[rt][ks] = *reinterpret_cast<const uint4 *>(src + ks * 16 + half * 8);
         }
-        for (uint32_t t0 = begin; t0 < end; t0 += 32) {
-            // (positions past the end repeat the last one; their scores are masked)
-            const uint64_t at = slot_of(p, table, min(t0 + col, end - 1)) * p.n_kv_heads + kvh;
+    }
+    if (begin < end) {
+        // a tile's K chunks are requested one tile ahead, its block-table entries two (positions past the end repeat the
+        // last one; their scores are masked)
+        typedef typename std::conditional<KV8, uint2, uint4>::type raw_t;
+        raw_t next[KS];
+        float scale_next = 1.f;
+        auto slot_ahead = [&](uint32_t t0) __attribute__((always_inline)) { return slot_of(p, table, min(t0 + col, end - 1)) * p.n_kv_heads + kvh; };
+        auto request = [&](uint64_t at) __attribute__((always_inline)) {
             const unsigned char *row = p.k_cache + at * ROWB;
-            f32x16_t S;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                S[k] = 0.f;
+            for (int ks = 0; ks < KS; ks++) {
+                next[ks] = *reinterpret_cast<const raw_t *>(row + (2 * ks + half) * sizeof(raw_t));
+            }
+            if constexpr (KV8) {
+                scale_next = p.k_scale[at];
+            }
+        };
+        request(slot_ahead(begin));
+        uint64_t at_next = slot_ahead(begin + 32);
+        for (uint32_t t0 = begin; t0 < end; t0 += 32) {
+            uint4 kop[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if constexpr (KV8) {
+                    kop[ks] = dequant8<T, KVF>(next[ks], 1.0f);
+                } else {
+                    kop[ks] = next[ks];
+                }
+            }
+            const float scale = scale_next;
+            request(at_next);
+            at_next = slot_ahead(t0 + 64);
+            f32x16_t S[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    S[rt][k] = 0.f;
+                }
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                S = mfma32<T>(cache_chunk<T, KVF>(row, 2 * ks + half), qreg[ks], S);
-            }
-            if constexpr (KVF != XLITE_HIP_KV_SAME) {
-                const float scale = p.k_scale[at];   // of position t0 + col; register k holds another one
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    S[k] *= __shfl(scale, static_cast<int>((k / 4) * 8 + half * 4 + (k % 4)));
+                for (int rt = 0; rt < RT; rt++) {
+                    S[rt] = mfma32<T>(kop[ks], qreg[rt][ks], S[rt]);
                 }
             }
-            const uint32_t lim = min(vis, end);
-            if (t0 + 32 > min(vis_first, end)) {
+            const bool masked = t0 + 32 > min(vis_first, end);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                if constexpr (KV8) {   // the scale of position t0 + col; register k holds another one
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        S[rt][k] *= __shfl(scale, static_cast<int>((k / 4) * 8 + half * 4 + (k % 4)));
+                    }
+                }
+                if (masked) {
+                    const uint32_t lim = min(vis[rt], end);
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        S[rt][k] = t0 + (k / 4) * 8 + half * 4 + (k % 4) < lim ? S[rt][k] : -INFINITY;
+                    }
+                }
+                float mx = m_run[rt];
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
-                    S[k] = t0 + (k / 4) * 8 + half * 4 + (k % 4) < lim ? S[k] : -INFINITY;
+                    mx = fmaxf(mx, S[rt][k]);
                 }
-            }
-            float mx = m_run;
+                const float m_safe = mx == -INFINITY ? 0.f : mx;
+                const float neg = -m_safe * kLog2e;
+                float sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                mx = fmaxf(mx, S[k]);
+                for (int k = 0; k < 16; k++) {
+                    sum += fast_exp2(__builtin_fmaf(S[rt][k], kLog2e, neg));
+                }
+                l_run[rt] = l_run[rt] * fast_exp2((m_run[rt] - m_safe) * kLog2e) + sum;
+                m_run[rt] = mx;
             }
-            const float m_safe = mx == -INFINITY ? 0.f : mx;
-            const float neg = -m_safe * kLog2e;
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-                sum += fast_exp2(__builtin_fmaf(S[k], kLog2e, neg));
-            }
-            l_run = l_run * fast_exp2((m_run - m_safe) * kLog2e) + sum;
-            m_run = mx;
         }
     }
-    // the two halves of a row's positions
-    const float m_other = __shfl_xor(m_run, 32), l_other = __shfl_xor(l_run, 32);
-    const float m_all = fmaxf(m_run, m_other);
-    const float m_safe = m_all == -INFINITY ? 0.f : m_all;
-    const float l_all = l_run * fast_exp2((m_run - m_safe) * kLog2e) + l_other * fast_exp2((m_other - m_safe) * kLog2e);
-    if (half == 0 && m_wave + col < s.m_rows) {
-        const uint64_t i = static_cast<uint64_t>(kvh) * p.m_total + static_cast<uint64_t>(s.start + s.first) * G + m_wave + col;
-        if (p.splits == 1) {
-            p.norm[i] = -(m_all * kLog2e + __log2f(l_all));
-        } else {
-            *reinterpret_cast<float2 *>(p.stats + (static_cast<uint64_t>(split) * p.n_kv_heads * p.m_total + i) * 2) =
-                make_float2(m_all * kLog2e, l_all);
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        // the two halves of a row's positions
+        const float m_other = __shfl_xor(m_run[rt], 32), l_other = __shfl_xor(l_run[rt], 32);
+        const float m_all = fmaxf(m_run[rt], m_other);
+        const float m_safe = m_all == -INFINITY ? 0.f : m_all;
+        const float l_all = l_run[rt] * fast_exp2((m_run[rt] - m_safe) * kLog2e) + l_other * fast_exp2((m_other - m_safe) * kLog2e);
+        const uint32_t m = m_wave + rt * 32 + col;
+        if (half == 0 && m < s.m_rows) {
+            const uint64_t i = static_cast<uint64_t>(kvh) * p.m_total + static_cast<uint64_t>(s.start + s.first) * G + m;
+            if (p.splits == 1) {
+                p.norm[i] = -(m_all * kLog2e + __log2f(l_all));
+            } else {
+                *reinterpret_cast<float2 *>(p.stats + (static_cast<uint64_t>(split) * p.n_kv_heads * p.m_total + i) * 2) =
+                    make_float2(m_all * kLog2e, l_all);
+            }
         }
     }
 }
@@ -219,97 +288,383 @@ join_stats_kernel(const float *__restrict__ stats, float *__restrict__ norm, uin
 }
 
 template <typename T, int D, int KVF>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(2 * kThreads)
 column_sums_kernel(const WeightsParams p)
 {
     constexpr int KS = D / 16;
+    constexpr int PT = kPosTiles<D>;          // tiles of 32 positions of a wave
+    constexpr uint32_t WG = 4 * 32 * PT;      // positions of the workgroup: two waves for each 32 PT of them
     constexpr uint32_t ROWB = D * (KVF == XLITE_HIP_KV_SAME ? 2 : 1);
+    __shared__ float other[4][32 * PT];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.z, seq = blockIdx.y, G = p.group;
+    const uint32_t mine = wave & 3u, turn = wave >> 2;   // which 64 positions, and which of the M tiles: even or odd ones
     const Sequence s = sequence_of(p, seq);
     const uint32_t total = s.cached + s.nodes;
-    const uint32_t p0 = blockIdx.x * kPosTile + wave * 32;   // the wave's first position
-    if (s.nodes == 0 || p0 >= total) {
+    if (s.nodes == 0 || blockIdx.x * WG >= total) {
         return;
     }
+    const uint32_t p0 = blockIdx.x * WG + mine * 32 * PT;   // the wave's first position
     const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
-    const uint32_t t = p0 + col;
-    const uint64_t at = slot_of(p, table, min(t, total - 1)) * p.n_kv_heads + kvh;
-    const unsigned char *row = p.k_cache + at * ROWB;
-    uint4 kreg[KS];
+    uint64_t at[PT];
+    uint4 kreg[PT][KS];
+    float mul[PT], acc[PT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-        kreg[ks] = cache_chunk<T, KVF>(row, 2 * ks + half);
-    }
-    float mul = kLog2e;
-    if constexpr (KVF != XLITE_HIP_KV_SAME) {
-        mul *= p.k_scale[at];
+    for (int pt = 0; pt < PT; pt++) {
+        at[pt] = slot_of(p, table, min(p0 + pt * 32 + col, total - 1)) * p.n_kv_heads + kvh;
+        const unsigned char *row = p.k_cache + at[pt] * ROWB;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            kreg[pt][ks] = cache_chunk<T, KVF>(row, 2 * ks + half);
+        }
+        mul[pt] = kLog2e;
+        acc[pt] = 0.f;
+        if constexpr (KVF != XLITE_HIP_KV_SAME) {
+            mul[pt] *= p.k_scale[at[pt]];
+        }
     }
     // the first row that sees the wave's first position (rows before it see none of its positions)
     const uint32_t first_seen = p0 > s.cached + s.first ? (p0 - s.cached - s.first) * G : 0u;
     const uint64_t tok0 = s.start + s.first;
     const float *norm = p.norm + static_cast<uint64_t>(kvh) * p.m_total + tok0 * G;
-    float acc = 0.f;
-    for (uint32_t m0 = first_seen & ~31u; m0 < s.m_rows; m0 += 32) {
-        const uint32_t m = min(m0 + col, s.m_rows - 1);
-        const uint16_t *src = p.q + (tok0 + m / G) * p.q_tok_stride + static_cast<uint64_t>(kvh * G + m % G) * D;
-        uint4 qop[KS];
+    const uint16_t *q0 = p.q + tok0 * p.q_tok_stride + static_cast<uint64_t>(kvh * G) * D + half * 8;
+    const uint32_t m_begin = (first_seen & ~31u) + 32 * turn;
+    if (m_begin < s.m_rows && p0 < total) {
+        RowCursor cursor(m_begin + col, G);
+        uint4 next[KS];
+        // a tile's query rows are requested one tile ahead (rows past the end repeat the last one)
+        auto request = [&](uint32_t m0) __attribute__((always_inline)) {
+            const bool in = m0 + col < s.m_rows;
+            const uint32_t r = in ? cursor.r : (s.m_rows - 1) / G, h = in ? cursor.h : G - 1;
+            const uint16_t *src = q0 + static_cast<uint64_t>(r) * p.q_tok_stride + h * D;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            qop[ks] = *reinterpret_cast<const uint4 *>(src + ks * 16 + half * 8);
-        }
-        float n[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++) {
-            n[k] = norm[min(m0 + (k / 4) * 8 + half * 4 + (k % 4), s.m_rows - 1)];
-        }
-        f32x16_t S;
-#pragma unroll
-        for (int k = 0; k < 16; k++) {
-            S[k] = 0.f;
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            S = mfma32<T>(qop[ks], kreg[ks], S);
-        }
-        float sum = 0.f;
-        if (m0 + 32 > s.m_rows || p0 + 31 > s.cached + s.first + m0 / G) {
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const uint32_t mk = m0 + (k / 4) * 8 + half * 4 + (k % 4);
-                const float e = fast_exp2(__builtin_fmaf(S[k], mul, n[k]));
-                sum += mk < s.m_rows && t <= s.cached + s.first + mk / G ? e : 0.f;
+            for (int ks = 0; ks < KS; ks++) {
+                next[ks] = *reinterpret_cast<const uint4 *>(src + ks * 16);
             }
-        } else {
+        };
+        request(m_begin);
+        for (uint32_t m0 = m_begin; m0 < s.m_rows; m0 += 64) {
+            uint4 qop[KS];
+            float n[16];
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                sum += fast_exp2(__builtin_fmaf(S[k], mul, n[k]));
+            for (int ks = 0; ks < KS; ks++) {
+                qop[ks] = next[ks];
+            }
+            // this tile's normalisers ahead of the next tile's rows: memory answers in order
+            if (m0 + 32 <= s.m_rows) {
+                typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const f4 x = *reinterpret_cast<const f4 *>(norm + m0 + g * 8 + half * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        n[4 * g + e] = x[e];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    n[k] = norm[min(m0 + (k / 4) * 8 + half * 4 + (k % 4), s.m_rows - 1)];
+                }
+            }
+            if (m0 + 64 < s.m_rows) {
+                cursor.step();
+                cursor.step();
+                request(m0 + 64);
+            }
+            f32x16_t S[PT];
+#pragma unroll
+            for (int pt = 0; pt < PT; pt++) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    S[pt][k] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+                for (int pt = 0; pt < PT; pt++) {
+                    S[pt] = mfma32<T>(qop[ks], kreg[pt][ks], S[pt]);
+                }
+            }
+            const bool masked = m0 + 32 > s.m_rows || p0 + 32 * PT - 1 > s.cached + s.first + m0 / G;
+#pragma unroll
+            for (int pt = 0; pt < PT; pt++) {
+                float sum = 0.f;
+                if (masked) {
+                    const uint32_t t = p0 + pt * 32 + col;
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const uint32_t mk = m0 + (k / 4) * 8 + half * 4 + (k % 4);
+                        const float e = fast_exp2(__builtin_fmaf(S[pt][k], mul[pt], n[k]));
+                        sum += mk < s.m_rows && t <= s.cached + s.first + mk / G ? e : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        sum += fast_exp2(__builtin_fmaf(S[pt][k], mul[pt], n[k]));
+                    }
+                }
+                acc[pt] += sum;   // (a tile's sum first: 16 additions, then one per tile, not one chain over every row)
             }
         }
-        acc += sum;   // (a tile's sum first: 16 additions, then one per tile, instead of one chain over every row)
     }
-    acc += __shfl_xor(acc, 32);
-    if (half == 0 && t < total) {
-        p.weights[at] = t < s.cached ? p.weights[at] + acc : acc;
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+        acc[pt] += __shfl_xor(acc[pt], 32);
+        if (turn == 1 && half == 0) {
+            other[mine][pt * 32 + col] = acc[pt];
+        }
+    }
+    __syncthreads();
+    if (turn == 0 && half == 0) {
+#pragma unroll
+        for (int pt = 0; pt < PT; pt++) {
+            const uint32_t t = p0 + pt * 32 + col;
+            if (t < total) {
+                const float sum = acc[pt] + other[mine][pt * 32 + col];
+                p.weights[at[pt]] = t < s.cached ? p.weights[at[pt]] + sum : sum;
+            }
+        }
     }
 }
 
-// KV splits of the row statistics: enough workgroups for four per compute unit
-uint32_t stat_tiles(uint32_t total_tokens, uint32_t group, uint32_t batch, uint32_t window, uint32_t *per_seq)
+// ---- few rows: scores stored ------------------------------------------------------------------------------------------------
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4v_t;
+template <typename T>
+__device__ __forceinline__ f32x4v_t mfma16(const uint4 &a, const uint4 &b, f32x4v_t c)
 {
-    const uint64_t bounded = window == 0 ? 0 : static_cast<uint64_t>(std::min(window, total_tokens)) * group;
-    *per_seq = static_cast<uint32_t>((bounded + kRowTile - 1) / kRowTile);
-    const uint32_t by_prefix = ceil_div(total_tokens * group, kRowTile) + batch;
-    if (*per_seq != 0 && static_cast<uint64_t>(*per_seq) * batch <= by_prefix) {
-        return *per_seq * batch;
+    if constexpr (T::kCode == XLITE_HIP_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
     }
-    *per_seq = 0;
-    return by_prefix;
 }
-uint32_t stat_splits(uint32_t tiles, uint32_t n_kv_heads, uint32_t max_ctx)
+
+// where a sequence's stored rows begin (in M rows of a kv head): window rows per sequence, or its tokens
+__device__ __forceinline__ uint32_t stored_base(const WeightsParams &p, uint32_t seq, const Sequence &s)
 {
-    const uint32_t want = ceil_div(1024u, std::max(1u, tiles * n_kv_heads));
-    return std::max(1u, std::min(want, max_ctx / kMinSplit));
+    return (p.window != 0 ? seq * p.window : s.start) * p.group;
+}
+
+// A wave takes the positions of one kv head, 64 at a time, of the workgroup's chunk [chunk * split_len, + split_len): K rows
+// straight from memory as the A operand (a lane reads its row's chunk of 16 bytes, four lanes a row's 64 consecutive bytes),
+// the next 64 in flight; 16 M rows as the columns. It leaves the scores and every row's maximum and sum over the chunk.
+// Waves of a workgroup: the kv heads side by side, so that they read a position's whole row together, and where there are
+// fewer than eight heads, neighbouring chunks.
+template <typename T, int D, int KVF>
+__global__ void __launch_bounds__(512)
+store_scores_kernel(const WeightsParams p)
+{
+    constexpr int KS = D / 32;
+    constexpr int NT = D == 256 ? 2 : 4;      // tiles of 16 positions of an iteration
+    constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
+    constexpr uint32_t ROWB = D * (KV8 ? 1 : 2);
+    typedef typename std::conditional<KV8, uint2, uint4>::type raw_t;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, jq = lane >> 4;
+    const uint32_t heads = min(p.n_kv_heads, 8u), per_wg = 8u / heads;       // kv heads and chunks of a workgroup
+    if (wave >= heads * per_wg) {
+        return;
+    }
+    const uint32_t kvh = blockIdx.z * heads + wave % heads, chunk = blockIdx.x * per_wg + wave / heads, seq = blockIdx.y, G = p.group;
+    const Sequence s = sequence_of(p, seq);
+    const uint32_t total = s.cached + s.nodes;
+    const uint32_t begin = chunk * p.split_len, end = min(total, begin + p.split_len);
+    if (kvh >= p.n_kv_heads || s.nodes == 0 || chunk >= p.splits) {
+        return;
+    }
+    const uint32_t base = stored_base(p, seq, s);
+    const uint64_t rows0 = static_cast<uint64_t>(kvh) * p.m_total + base;
+    const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
+    for (uint32_t m0 = 0; m0 < s.m_rows; m0 += 16) {
+        const uint32_t m = min(m0 + col, s.m_rows - 1);
+        const uint32_t r = s.first + m / G;
+        const uint32_t lim = s.cached + r + 1;
+        float m_run = -INFINITY, l_run = 0.f;
+        if (begin < end) {
+            const uint16_t *src = p.q + static_cast<uint64_t>(s.start + r) * p.q_tok_stride + static_cast<uint64_t>(kvh * G + m % G) * D;
+            uint4 qreg[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                qreg[ks] = *reinterpret_cast<const uint4 *>(src + ks * 32 + jq * 8);
+            }
+            raw_t next[NT][KS];
+            float scale_next[NT];
+            auto request = [&](uint32_t t0) __attribute__((always_inline)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const uint64_t at = slot_of(p, table, min(t0 + nt * 16 + col, end - 1)) * p.n_kv_heads + kvh;
+                    const unsigned char *row = p.k_cache + at * ROWB;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        next[nt][ks] = *reinterpret_cast<const raw_t *>(row + (4 * ks + jq) * sizeof(raw_t));
+                    }
+                    if constexpr (KV8) {
+                        scale_next[nt] = p.k_scale[at];
+                    }
+                }
+            };
+            float *out = p.scores + (rows0 + m0 + col) * p.pitch;
+            request(begin);
+            for (uint32_t t0 = begin; t0 < end; t0 += 16 * NT) {
+                raw_t now[NT][KS];
+                float scale[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        now[nt][ks] = next[nt][ks];
+                    }
+                    if constexpr (KV8) {
+                        scale[nt] = scale_next[nt];
+                    }
+                }
+                if (t0 + 16 * NT < end) {
+                    request(t0 + 16 * NT);
+                }
+                f32x4v_t S[NT];
+                float mx = m_run;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    S[nt] = f32x4v_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        if constexpr (KV8) {
+                            S[nt] = mfma16<T>(dequant8<T, KVF>(now[nt][ks], 1.0f), qreg[ks], S[nt]);
+                        } else {
+                            S[nt] = mfma16<T>(now[nt][ks], qreg[ks], S[nt]);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t o = nt * 16 + 4 * jq + e;
+                        float x = S[nt][e] * kLog2e;
+                        if constexpr (KV8) {   // the scale of position t0 + 16 nt + col; register e holds another one
+                            x *= __shfl(scale[nt], static_cast<int>(4 * jq + e));
+                        }
+                        S[nt][e] = x;
+                        mx = fmaxf(mx, t0 + o < lim ? x : -INFINITY);
+                    }
+                    if (m0 + col < s.m_rows) {   // (positions past the end: inside the row's pitch, nobody reads them)
+                        *reinterpret_cast<float4 *>(out + t0 + nt * 16 + 4 * jq) = make_float4(S[nt][0], S[nt][1], S[nt][2], S[nt][3]);
+                    }
+                }
+                const float m_safe = mx == -INFINITY ? 0.f : mx;
+                float sum = 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float x = fast_exp2(S[nt][e] - m_safe);
+                        sum += t0 + nt * 16 + 4 * jq + e < lim ? x : 0.f;
+                    }
+                }
+                l_run = l_run * fast_exp2(m_run - m_safe) + sum;
+                m_run = mx;
+            }
+        }
+        // the row's four lanes
+#pragma unroll
+        for (int d = 16; d <= 32; d <<= 1) {
+            const float m_other = __shfl_xor(m_run, d), l_other = __shfl_xor(l_run, d);
+            const float m_all = fmaxf(m_run, m_other);
+            const float m_safe = m_all == -INFINITY ? 0.f : m_all;
+            l_run = l_run * fast_exp2(m_run - m_safe) + l_other * fast_exp2(m_other - m_safe);
+            m_run = m_all;
+        }
+        if (jq == 0 && m0 + col < s.m_rows) {
+            *reinterpret_cast<float2 *>(p.stats + (static_cast<uint64_t>(chunk) * p.n_kv_heads * p.m_total + rows0 + m0 + col) * 2) =
+                make_float2(m_run, l_run);
+        }
+    }
+}
+
+// a thread per position: the stored scores of its kv heads' rows
+__global__ void __launch_bounds__(kThreads)
+sum_scores_kernel(const WeightsParams p)
+{
+    const uint32_t seq = blockIdx.y, G = p.group;
+    const Sequence s = sequence_of(p, seq);
+    const uint32_t total = s.cached + s.nodes, t = blockIdx.x * kThreads + threadIdx.x;
+    if (s.nodes == 0 || t >= total) {
+        return;
+    }
+    const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
+    float *w = p.weights + slot_of(p, table, t) * p.n_kv_heads;
+    const uint32_t base = stored_base(p, seq, s);
+    // rows that see the position: from the first counted row r with s.cached + r >= t on
+    const uint32_t m_first = t > s.cached + s.first ? (t - s.cached - s.first) * G : 0u;
+    for (uint32_t kvh = blockIdx.z; kvh < p.n_kv_heads; kvh += gridDim.z) {
+        const uint64_t rows0 = static_cast<uint64_t>(kvh) * p.m_total + base;
+        const float *norm = p.norm + rows0;
+        const float *score = p.scores + rows0 * p.pitch + t;
+        const float old = w[kvh];
+        float acc = 0.f;
+        for (uint32_t m0 = 0; m0 < s.m_rows; m0 += 8) {
+            float x[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                x[u] = score[static_cast<uint64_t>(min(m0 + u, s.m_rows - 1)) * p.pitch];
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float e = fast_exp2(x[u] + norm[min(m0 + u, s.m_rows - 1)]);
+                sum += m0 + u >= m_first && m0 + u < s.m_rows ? e : 0.f;
+            }
+            acc += sum;
+        }
+        w[kvh] = t < s.cached ? old + acc : acc;
+    }
+}
+
+// ---- the plan of a call: which kernels, how many pieces, how much scratch -----------------------------------------------------
+struct Plan {
+    bool stored;                 // the scores are stored
+    uint32_t rows;               // M rows of a kv head that the scratch is laid out for
+    uint32_t tiles, tiles_per_seq, splits, split_len, pitch, window;
+    size_t bytes;
+};
+
+Plan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
+             uint32_t max_num_block, uint32_t window)
+{
+    Plan plan{};
+    plan.window = window = window >= total_tokens ? 0u : window;   // (as many rows as there are: all of them)
+    const uint32_t G = n_heads / n_kv_heads, max_ctx = max_num_block * block_size;
+    // counted rows: at most `window` per sequence, at most every row
+    const uint64_t bounded = window == 0 ? total_tokens : static_cast<uint64_t>(window) * batch;
+    const uint64_t counted = std::min<uint64_t>(bounded, total_tokens);
+    plan.stored = counted * G <= static_cast<uint64_t>(kStoredRows) * batch && bounded * n_heads < (1ull << 31);
+    if (plan.stored) {
+        plan.rows = static_cast<uint32_t>(bounded) * G;
+        plan.pitch = ceil_div(max_ctx, 64u) * 64u;
+        // chunks of 64 to 256 positions: as long as there are four workgroups (of eight waves) per compute unit
+        const uint64_t waves64 = static_cast<uint64_t>(batch) * ceil_div(max_ctx, 64u) * n_kv_heads;
+        plan.split_len = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(4, waves64 / 8192))) * 64u;
+        plan.splits = ceil_div(max_ctx, plan.split_len);
+        const size_t rows = static_cast<size_t>(plan.rows) * n_kv_heads;
+        plan.bytes = ((rows + 3) / 4 * 4 + rows * plan.pitch + 2 * rows * plan.splits) * sizeof(float);
+        return plan;
+    }
+    plan.rows = total_tokens * G;
+    const uint32_t tile = head_dim == 256 ? kRowTile / 2 : kRowTile;
+    const uint64_t of_window = window == 0 ? 0 : static_cast<uint64_t>(std::min(window, total_tokens)) * G;
+    plan.tiles_per_seq = static_cast<uint32_t>((of_window + tile - 1) / tile);
+    const uint32_t by_prefix = ceil_div(total_tokens * G, tile) + batch;
+    if (plan.tiles_per_seq != 0 && static_cast<uint64_t>(plan.tiles_per_seq) * batch <= by_prefix) {
+        plan.tiles = plan.tiles_per_seq * batch;
+    } else {
+        plan.tiles_per_seq = 0;
+        plan.tiles = by_prefix;
+    }
+    // splits of the row statistics: enough workgroups (of four waves) for four per compute unit
+    const uint32_t want = ceil_div(1024u, std::max(1u, plan.tiles * n_kv_heads));
+    plan.splits = std::max(1u, std::min(want, max_ctx / kMinSplit));
+    plan.split_len = ceil_div(ceil_div(max_ctx, plan.splits), 32u) * 32u;
+    const size_t rows = static_cast<size_t>(total_tokens) * n_heads;
+    plan.bytes = (rows + (plan.splits > 1 ? 2 * plan.splits * rows : 0)) * sizeof(float);
+    return plan;
 }
 
 }  // namespace
@@ -319,17 +674,13 @@ uint32_t stat_splits(uint32_t tiles, uint32_t n_kv_heads, uint32_t max_ctx)
 using namespace xlite;
 
 extern "C" size_t xlite_hip_attention_weights_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
-                                                              uint32_t block_size, uint32_t batch, uint32_t max_num_block,
-                                                              uint32_t window)
+                                                              uint32_t head_dim, uint32_t block_size, uint32_t batch,
+                                                              uint32_t max_num_block, uint32_t window)
 {
     if (total_tokens == 0 || batch == 0 || n_kv_heads == 0 || n_heads % n_kv_heads != 0) {
         return 0;
     }
-    uint32_t per_seq;
-    const uint32_t tiles = stat_tiles(total_tokens, n_heads / n_kv_heads, batch, window, &per_seq);
-    const uint64_t splits = stat_splits(tiles, n_kv_heads, max_num_block * block_size);
-    const uint64_t rows = static_cast<uint64_t>(total_tokens) * n_heads;
-    return static_cast<size_t>((rows + (splits > 1 ? 2 * splits * rows : 0)) * sizeof(float));
+    return plan_of(total_tokens, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, window).bytes;
 }
 
 extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const void *k_cache, float *weights,
@@ -354,10 +705,9 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
     XL_REQUIRE(kv_dtype == XLITE_HIP_KV_SAME || head_dim != 256, "quantised KV caches: head_dim must be 64 or 128");
     XL_REQUIRE(static_cast<uint64_t>(total_tokens) * n_heads < (1ull << 31) && batch <= 65535 && n_kv_heads <= 65535,
                "more rows than one launch takes");
-    const size_t need = xlite_hip_attention_weights_workspace_bytes(total_tokens, n_heads, n_kv_heads, block_size, batch,
-                                                                    max_num_block, window);
-    if (workspace == nullptr || workspace_bytes < need) {
-        return fail(XLITE_HIP_ENOSPC, __func__, "workspace too small: need " + std::to_string(need) + " bytes, have " +
+    const Plan plan = plan_of(total_tokens, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, window);
+    if (workspace == nullptr || workspace_bytes < plan.bytes) {
+        return fail(XLITE_HIP_ENOSPC, __func__, "workspace too small: need " + std::to_string(plan.bytes) + " bytes, have " +
                                                     std::to_string(workspace == nullptr ? 0 : workspace_bytes));
     }
     hipStream_t s = as_stream(stream);
@@ -377,24 +727,42 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
     p.batch = batch;
     p.block_size = block_size;
     p.max_num_block = max_num_block;
-    p.window = window;
-    p.m_total = total_tokens * G;
-    const uint32_t tiles = stat_tiles(total_tokens, G, batch, window, &p.tiles_per_seq);
-    p.splits = stat_splits(tiles, n_kv_heads, max_ctx);
-    p.split_len = ceil_div(ceil_div(max_ctx, p.splits), 32u) * 32u;
-    const uint32_t rows = total_tokens * n_heads;
+    p.window = plan.window;
+    p.m_total = plan.rows;
+    p.tiles_per_seq = plan.tiles_per_seq;
+    p.splits = plan.splits;
+    p.split_len = plan.split_len;
+    p.block_magic = static_cast<uint64_t>(max_ctx) * block_size < (1ull << 32) ? static_cast<uint32_t>((1ull << 32) / block_size) + 1 : 0u;
+    const uint32_t rows = plan.rows * n_kv_heads;
     p.norm = static_cast<float *>(workspace);
-    p.stats = p.norm + rows;
+    if (plan.stored) {
+        p.scores = p.norm + (static_cast<size_t>(rows) + 3) / 4 * 4;   // (16-byte stores)
+        p.pitch = plan.pitch;
+        p.stats = p.scores + static_cast<size_t>(rows) * plan.pitch;
+    } else {
+        p.stats = p.norm + rows;
+    }
     auto launch = [&](auto t, auto d, auto kvf) -> int {
         using T = decltype(t);
         constexpr int D = decltype(d)::value, KVF = decltype(kvf)::value;
-        row_stats_kernel<T, D, KVF><<<dim3(tiles, p.splits, n_kv_heads), kThreads, 0, s>>>(p);
+        if (plan.stored) {
+            const uint32_t heads = std::min(n_kv_heads, 8u);
+            store_scores_kernel<T, D, KVF><<<dim3(ceil_div(plan.splits, 8u / heads), batch, ceil_div(n_kv_heads, heads)), 512, 0, s>>>(p);
+        } else {
+            row_stats_kernel<T, D, KVF><<<dim3(plan.tiles, plan.splits, n_kv_heads), kThreads, 0, s>>>(p);
+        }
         XL_LAUNCH_CHECK();
-        if (p.splits > 1) {
-            join_stats_kernel<<<ceil_div(rows, 256u), 256, 0, s>>>(p.stats, p.norm, rows, p.splits);
+        if (plan.stored || plan.splits > 1) {
+            join_stats_kernel<<<ceil_div(rows, 256u), 256, 0, s>>>(p.stats, p.norm, rows, plan.splits);
             XL_LAUNCH_CHECK();
         }
-        column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, kPosTile), batch, n_kv_heads), kThreads, 0, s>>>(p);
+        if (plan.stored) {
+            const uint32_t tiles = ceil_div(max_ctx, static_cast<uint32_t>(kThreads));
+            const uint32_t z = std::max(1u, std::min(n_kv_heads, 512u / std::max(1u, tiles * batch)));   // few positions: the heads side by side
+            sum_scores_kernel<<<dim3(tiles, batch, z), kThreads, 0, s>>>(p);
+        } else {
+            column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 128u * kPosTiles<D>), batch, n_kv_heads), 2 * kThreads, 0, s>>>(p);
+        }
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;
     };

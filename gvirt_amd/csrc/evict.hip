@@ -11,7 +11,7 @@ namespace {
 // ---- select_kept ------------------------------------------------------------------------------------------------------
 // Per (sequence, kv head): the first `sink` and the last `recent` positions, and of the positions between them the n =
 // budget - sink - recent with the largest weights; equal weights go to the lower position. A radix selection: the n-th
-// largest key is found 8 bits at a time with histograms in LDS (one per wave: most weights share their top byte), then the
+// largest key is found digit by digit with histograms in LDS, then the
 // positions whose key is larger, and the first ones that equal it, are written in position order. Counts only, so the result
 // does not depend on any order. One workgroup per (sequence, kv head); the keys are read once, into registers.
 // A weight's neighbours in memory belong to the other kv heads: the heads of a sequence run on one XCD, at the same time, so
@@ -40,61 +40,69 @@ struct SelectParams {
 };
 
 // The n-th largest of the keys (n > 0, at least n of them) and how many of those equal to it are among the n largest.
-// each(f) calls f for every key of the thread (0: none).
+// each(f) calls f for every key of the thread (0: none). Digits of 11, 11 and 10 bits: the first one holds the sign, the
+// exponent and two bits of the mantissa, so that few lanes of a wave meet in one bin (with 8 bits a dozen did, and the
+// first pass took longer than the rest of the kernel together).
+constexpr int kHistCopies = 4;
+struct SelectScratch {
+    uint32_t hist[kHistCopies][2048];
+    uint32_t wave_sum[kSelWaves];
+    uint32_t found[2];   // the digit, and how many keys lie in the bins above it
+};
 template <typename EACH>
-__device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, uint32_t (*hist)[256], uint32_t *found, uint32_t *threshold, uint32_t *equal)
+__device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScratch &s, uint32_t *threshold, uint32_t *equal)
 {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t *mine = s.hist[wave % kHistCopies];
     uint32_t left = n, prefix = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            hist[wave][lane + 64 * i] = 0;
+    for (int pass = 0; pass < 3; pass++) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t bits = pass == 2 ? 10u : 11u;
+#pragma unroll
+        for (int i = 0; i < kHistCopies * 2048 / kSelThreads; i++) {
+            (&s.hist[0][0])[threadIdx.x + i * kSelThreads] = 0;
         }
-        // (a wave's own histogram: its LDS operations are carried out in order)
+        __syncthreads();
         each([&](uint32_t k) {
-            const bool in = shift == 24 ? k != 0 : (k >> (shift + 8)) == prefix;
-            if (in) {
-                atomicAdd(&hist[wave][(k >> shift) & 255u], 1u);
+            if (pass == 0 ? k != 0 : (k >> (shift + bits)) == prefix) {
+                atomicAdd(&mine[(k >> shift) & ((1u << bits) - 1)], 1u);
             }
         });
         __syncthreads();
-        if (threadIdx.x < 256) {
-            uint32_t sum = 0;
+        // thread t: bins 2047 - 2 t and 2046 - 2 t, in descending order
+        uint32_t c[2] = {0, 0};
 #pragma unroll
-            for (int w = 0; w < kSelWaves; w++) {
-                sum += hist[w][threadIdx.x];
-            }
-            hist[0][threadIdx.x] = sum;
+        for (int h = 0; h < kHistCopies; h++) {
+            c[0] += s.hist[h][2047 - 2 * threadIdx.x];
+            c[1] += s.hist[h][2046 - 2 * threadIdx.x];
+        }
+        uint32_t incl = c[0] + c[1];
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(incl, d);
+            incl += lane >= static_cast<uint32_t>(d) ? up : 0u;
+        }
+        if (lane == 63) {
+            s.wave_sum[wave] = incl;
         }
         __syncthreads();
-        if (wave == 0) {
-            // lane l: bins 255 - 4 l .. 252 - 4 l, in descending order
-            uint32_t c[4], sum = 0;
+        uint32_t above = incl - c[0] - c[1];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                c[e] = hist[0][255 - 4 * lane - e];
-                sum += c[e];
-            }
-            uint32_t incl = sum;
+        for (uint32_t w = 0; w < kSelWaves; w++) {
+            above += w < wave ? s.wave_sum[w] : 0u;
+        }
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t up = __shfl_up(incl, d);
-                incl += lane >= static_cast<uint32_t>(d) ? up : 0u;
+        for (int e = 0; e < 2; e++) {
+            if (above < left && left <= above + c[e]) {   // exactly one bin of one thread
+                s.found[0] = 2047 - 2 * threadIdx.x - e;
+                s.found[1] = above;
             }
-            uint32_t above = incl - sum;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (above < left && left <= above + c[e]) {   // exactly one bin of one lane
-                    found[0] = 255 - 4 * lane - e;
-                    found[1] = above;
-                }
-                above += c[e];
-            }
+            above += c[e];
         }
         __syncthreads();
-        prefix = prefix << 8 | found[0];
-        left -= found[1];
+        prefix = prefix << bits | s.found[0];
+        left -= s.found[1];
     }
     *threshold = prefix;
     *equal = left;
@@ -106,8 +114,7 @@ template <int KPT>
 __global__ void __launch_bounds__(kSelThreads)
 select_kept_kernel(const SelectParams p)
 {
-    __shared__ uint32_t hist[kSelWaves][256];
-    __shared__ uint32_t found[2];            // the digit, and how many keys lie in the bins above it
+    __shared__ SelectScratch scratch;
     __shared__ uint2 counts[(KPT > 0 ? KPT : 1) * kSelWaves];   // (above, equal) of a wave's 64 positions, then the sums before them
     const uint32_t xcd = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
     const uint32_t seq = place / p.n_kv_heads * kXcds + xcd, kvh = place % p.n_kv_heads;
@@ -162,7 +169,7 @@ select_kept_kernel(const SelectParams p)
             for (int j = 0; j < KPT; j++) {
                 f(key[j]);
             }
-        }, n, hist, found, &threshold, &equal);
+        }, n, scratch, &threshold, &equal);
 #pragma unroll
         for (int j = 0; j < KPT; j++) {
             const uint64_t a = __ballot(key[j] > threshold), e = __ballot(key[j] == threshold);
@@ -212,7 +219,7 @@ select_kept_kernel(const SelectParams p)
             for (uint32_t i = lo + threadIdx.x; i < hi; i += kSelThreads) {
                 f(key_at(i));
             }
-        }, n, hist, found, &threshold, &equal);
+        }, n, scratch, &threshold, &equal);
         uint32_t above_before = 0, equal_before = 0;
         for (uint32_t i0 = lo; i0 < hi; i0 += kSelThreads) {
             const uint32_t i = i0 + threadIdx.x;

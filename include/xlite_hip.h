@@ -505,9 +505,9 @@ int xlite_hip_verify_tree(void *stream, const void *logits, const int32_t *token
  * k_scale, head_dim 64 or 128). workspace: xlite_hip_attention_weights_workspace_bytes() (required).
  * ---------------------------------------------------------------------- */
 size_t xlite_hip_attention_weights_workspace_bytes(uint32_t total_tokens, uint32_t n_heads,
-                                                   uint32_t n_kv_heads, uint32_t block_size,
-                                                   uint32_t batch, uint32_t max_num_block,
-                                                   uint32_t window);
+                                                   uint32_t n_kv_heads, uint32_t head_dim,
+                                                   uint32_t block_size, uint32_t batch,
+                                                   uint32_t max_num_block, uint32_t window);
 int xlite_hip_attention_weights(void *stream, const void *qkv, const void *k_cache, float *weights,
                                 const int32_t *query_start_loc, const int32_t *lens,
                                 const int32_t *cached_lens, const int32_t *block_tables,
