@@ -16,6 +16,7 @@
 
 #include "attention_common.h"
 #include "kv8.h"
+#include "stage.h"
 
 namespace xlite {
 
@@ -269,6 +270,188 @@ row_stats_kernel(const WeightsParams p)
     }
 }
 
+// The same for 16-bit caches of head_dim 64 and 128, K tiles of 64 positions copied straight into LDS (a ring of four) and
+// shared by the four waves. Read from memory by every wave, as above, a K chunk of 32 positions touches 32 lines per
+// instruction and every line four times: the vector cache's look-ups took longer than the products and the exponentials.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2)
+row_stats_staged_kernel(const WeightsParams p)
+{
+    constexpr int KS = D / 16, RT = 2, BN = 64, STAGES = 4;
+    constexpr uint32_t ROWB = D * 2, STAGE = BN * ROWB, TILE = 4 * 32 * RT;
+    constexpr int PPC = 1024 / ROWB;           // positions per copy
+    constexpr int CPW = BN / PPC / 4;          // copies per wave and tile
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    uint32_t *tbl = reinterpret_cast<uint32_t *>(smem + STAGES * STAGE);
+    const uint32_t smem_addr = stage::lds_address(smem);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const uint32_t kvh = blockIdx.z, split = blockIdx.y, G = p.group;
+    uint32_t seq = 0, mt;
+    if (p.tiles_per_seq != 0) {
+        seq = blockIdx.x / p.tiles_per_seq;
+        mt = blockIdx.x % p.tiles_per_seq;
+    } else {
+        auto first_id = [&](uint32_t i) {
+            return static_cast<uint32_t>(static_cast<uint64_t>(p.query_start_loc[i]) * G / TILE) + i;
+        };
+        uint32_t hi = p.batch;
+        while (hi - seq > 1) {
+            const uint32_t mid = (seq + hi) >> 1;
+            if (first_id(mid) <= blockIdx.x) {
+                seq = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        mt = blockIdx.x - first_id(seq);
+    }
+    const Sequence s = sequence_of(p, seq);
+    const uint32_t m_first = mt * TILE;
+    if (m_first >= s.m_rows) {
+        return;
+    }
+    const uint32_t m_wave = min(m_first + wave * 32 * RT, s.m_rows - 1);         // (a wave without rows repeats the last one)
+    uint32_t vis[RT];
+    const uint32_t vis_first = s.cached + s.first + m_wave / G + 1;
+    // the workgroup's range: what its last row sees
+    const uint32_t vis_last = s.cached + s.first + min(m_first + TILE - 1, s.m_rows - 1) / G + 1;
+    const uint32_t begin = split * p.split_len, end = min(vis_last, begin + p.split_len);
+    const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
+    float m_run[RT], l_run[RT];
+    uint4 qreg[RT][KS];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const uint32_t m = min(m_wave + rt * 32 + col, s.m_rows - 1);
+        const uint32_t r = s.first + m / G;
+        vis[rt] = s.cached + r + 1;
+        m_run[rt] = -INFINITY;
+        l_run[rt] = 0.f;
+        const uint16_t *src = p.q + static_cast<uint64_t>(s.start + r) * p.q_tok_stride + static_cast<uint64_t>(kvh * G + m % G) * D;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            qreg[rt][ks] = *reinterpret_cast<const uint4 *>(src + ks * 16 + half * 8);
+        }
+    }
+    if (begin < end) {
+        const uint32_t blk0 = begin / p.block_size, blk1 = (end - 1) / p.block_size;
+        for (uint32_t i = threadIdx.x; i <= blk1 - blk0; i += kThreads) {
+            tbl[i] = static_cast<uint32_t>(table[blk0 + i]);
+        }
+        // complete these loads before any copy is issued
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                asm volatile("" : "+v"(qreg[rt][ks].x), "+v"(qreg[rt][ks].y), "+v"(qreg[rt][ks].z), "+v"(qreg[rt][ks].w));
+            }
+        }
+        __syncthreads();
+        const uint32_t pitch = p.n_kv_heads * ROWB;
+        uint32_t c_row[CPW], c_off[CPW];
+#pragma unroll
+        for (int i = 0; i < CPW; i++) {
+            uint32_t chunk;
+            stage::copy_source<D>(lane, PPC * (CPW * wave + i), &c_row[i], &chunk);
+            c_off[i] = chunk << 4;
+        }
+        // copies of tile `tile` of the range into stage tile % 4; the positions of a copy share a block, those past the end
+        // repeat the last one (their scores are masked)
+        auto issue = [&](uint32_t tile) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < CPW; i++) {
+                const uint32_t pos = PPC * (CPW * wave + i);
+                const uint32_t t_raw = begin + tile * BN + pos, lim = end - 1;
+                const uint32_t t = min(t_raw, lim) & ~static_cast<uint32_t>(PPC - 1);
+                const uint32_t rel = min(t_raw + c_row[i], lim) - t;
+                const uint32_t blk = __umulhi(t, p.block_magic);
+                const uint32_t phys = __builtin_amdgcn_readfirstlane(tbl[blk - blk0]);
+                const uint64_t row0 = static_cast<uint64_t>(phys) * p.block_size + (t - blk * p.block_size);
+                const char *kb = reinterpret_cast<const char *>(p.k_cache) + row0 * pitch + kvh * ROWB;
+                stage::copy_1k(smem_addr + (tile % STAGES) * STAGE + pos * ROWB, rel * pitch + c_off[i], kb);
+            }
+        };
+        const uint32_t n_tiles = ceil_div(end - begin, static_cast<uint32_t>(BN));
+        const uint32_t row_off = D == 128 ? col * 256 : (col >> 1) * 256;
+        const uint32_t x = D == 128 ? (half ^ stage::pattern<D>(col)) << 4 : ((((col & 1) << 3) | half) ^ stage::pattern<D>(col >> 1)) << 4;
+        issue(0);
+        issue(1);
+        issue(2);
+        for (uint32_t tile = 0; tile < n_tiles; tile++) {
+            stage::wait<2 * CPW>();   // this wave's share of `tile` has landed
+            __syncthreads();          // ... and everybody else's; stage (tile - 1) % 4 is free
+            issue(tile + 3);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t t0 = begin + tile * BN + h * 32;
+                const unsigned char *base = smem + (tile % STAGES) * STAGE + h * 32 * ROWB + row_off;
+                uint4 kop[KS];
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    kop[ks] = *reinterpret_cast<const uint4 *>(base + (((2 * ks) << 4) ^ x));
+                }
+                f32x16_t S[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        S[rt][k] = 0.f;
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        S[rt] = mfma32<T>(kop[ks], qreg[rt][ks], S[rt]);
+                    }
+                }
+                const bool masked = t0 + 32 > min(vis_first, end);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    if (masked) {
+                        const uint32_t lim = min(vis[rt], end);
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            S[rt][k] = t0 + (k / 4) * 8 + half * 4 + (k % 4) < lim ? S[rt][k] : -INFINITY;
+                        }
+                    }
+                    float mx = m_run[rt];
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        mx = fmaxf(mx, S[rt][k]);
+                    }
+                    const float m_safe = mx == -INFINITY ? 0.f : mx;
+                    const float neg = -m_safe * kLog2e;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        sum += fast_exp2(__builtin_fmaf(S[rt][k], kLog2e, neg));
+                    }
+                    l_run[rt] = l_run[rt] * fast_exp2((m_run[rt] - m_safe) * kLog2e) + sum;
+                    m_run[rt] = mx;
+                }
+            }
+        }
+        stage::wait<0>();   // (nothing is left on its way into LDS when the workgroup ends)
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const float m_other = __shfl_xor(m_run[rt], 32), l_other = __shfl_xor(l_run[rt], 32);
+        const float m_all = fmaxf(m_run[rt], m_other);
+        const float m_safe = m_all == -INFINITY ? 0.f : m_all;
+        const float l_all = l_run[rt] * fast_exp2((m_run[rt] - m_safe) * kLog2e) + l_other * fast_exp2((m_other - m_safe) * kLog2e);
+        const uint32_t m = m_first + wave * 32 * RT + rt * 32 + col;
+        if (half == 0 && m < s.m_rows) {
+            const uint64_t i = static_cast<uint64_t>(kvh) * p.m_total + static_cast<uint64_t>(s.start + s.first) * G + m;
+            if (p.splits == 1) {
+                p.norm[i] = -(m_all * kLog2e + __log2f(l_all));
+            } else {
+                *reinterpret_cast<float2 *>(p.stats + (static_cast<uint64_t>(split) * p.n_kv_heads * p.m_total + i) * 2) =
+                    make_float2(m_all * kLog2e, l_all);
+            }
+        }
+    }
+}
+
 // joins the splits of every row (rows that nobody counted hold whatever the workspace held; nobody reads them)
 __global__ void __launch_bounds__(256)
 join_stats_kernel(const float *__restrict__ stats, float *__restrict__ norm, uint32_t rows, uint32_t splits)
@@ -409,6 +592,183 @@ column_sums_kernel(const WeightsParams p)
             }
         }
     }
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+        acc[pt] += __shfl_xor(acc[pt], 32);
+        if (turn == 1 && half == 0) {
+            other[mine][pt * 32 + col] = acc[pt];
+        }
+    }
+    __syncthreads();
+    if (turn == 0 && half == 0) {
+#pragma unroll
+        for (int pt = 0; pt < PT; pt++) {
+            const uint32_t t = p0 + pt * 32 + col;
+            if (t < total) {
+                const float sum = acc[pt] + other[mine][pt * 32 + col];
+                p.weights[at[pt]] = t < s.cached ? p.weights[at[pt]] + sum : sum;
+            }
+        }
+    }
+}
+
+// The same for head_dim 64 and 128 with the query rows copied straight into LDS, 64 M rows at a time (32 for each half of
+// the waves), and their normalisers with them.
+template <typename T, int D, int KVF>
+__global__ void __launch_bounds__(2 * kThreads)
+column_sums_staged_kernel(const WeightsParams p)
+{
+    constexpr int KS = D / 16, PT = 2, STAGES = 3;
+    constexpr uint32_t ROWB = D * (KVF == XLITE_HIP_KV_SAME ? 2 : 1), QROWB = D * 2;
+    constexpr uint32_t QBYTES = 64 * QROWB, STAGE = QBYTES + 8 * 256;   // the rows, then the normalisers once per wave
+    constexpr int RPC = 1024 / QROWB, CPW = 64 / RPC / 8;               // rows per copy, copies per wave
+    constexpr uint32_t WG = 4 * 32 * PT;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    __shared__ float other[4][32 * PT];
+    const uint32_t smem_addr = stage::lds_address(smem);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const uint32_t kvh = blockIdx.z, seq = blockIdx.y, G = p.group;
+    const uint32_t mine = wave & 3u, turn = wave >> 2;   // which 64 positions, and which half of the staged rows
+    const Sequence s = sequence_of(p, seq);
+    const uint32_t total = s.cached + s.nodes;
+    const uint32_t wg0 = blockIdx.x * WG;
+    if (s.nodes == 0 || wg0 >= total) {
+        return;
+    }
+    const uint32_t p0 = wg0 + mine * 32 * PT;   // the wave's first position
+    const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
+    uint64_t at[PT];
+    uint4 kreg[PT][KS];
+    float mul[PT], acc[PT];
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+        at[pt] = slot_of(p, table, min(p0 + pt * 32 + col, total - 1)) * p.n_kv_heads + kvh;
+        const unsigned char *row = p.k_cache + at[pt] * ROWB;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            kreg[pt][ks] = cache_chunk<T, KVF>(row, 2 * ks + half);
+        }
+        mul[pt] = kLog2e;
+        acc[pt] = 0.f;
+        if constexpr (KVF != XLITE_HIP_KV_SAME) {
+            mul[pt] *= p.k_scale[at[pt]];
+        }
+    }
+    // complete these loads before any copy is issued
+#pragma unroll
+    for (int pt = 0; pt < PT; pt++) {
+        asm volatile("" : "+v"(mul[pt]));
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            asm volatile("" : "+v"(kreg[pt][ks].x), "+v"(kreg[pt][ks].y), "+v"(kreg[pt][ks].z), "+v"(kreg[pt][ks].w));
+        }
+    }
+    // from the first row that sees the workgroup's first position on (rows before it see none of its positions)
+    const uint32_t m_begin = (wg0 > s.cached + s.first ? (wg0 - s.cached - s.first) * G : 0u) & ~63u;
+    const uint32_t rows = s.m_rows - m_begin, n_it = ceil_div(rows, 64u);   // (the last row sees every position: rows > 0)
+    const uint64_t tok0 = s.start + s.first;
+    const float *norm = p.norm + static_cast<uint64_t>(kvh) * p.m_total + tok0 * G + m_begin;
+    const uint16_t *q0 = p.q + tok0 * p.q_tok_stride + static_cast<uint64_t>(kvh * G) * D;
+    // a lane's rows of the copies: M row m_begin + 64 it + c_row, as (token, head); rows past the end repeat the last one
+    uint32_t c_m[CPW], c_r[CPW], c_h[CPW], c_chunk[CPW];
+#pragma unroll
+    for (int i = 0; i < CPW; i++) {
+        const uint32_t first = RPC * (CPW * wave + i);
+        uint32_t row;
+        stage::copy_source<D>(lane, first, &row, &c_chunk[i]);
+        c_m[i] = first + row;
+        c_r[i] = (m_begin + c_m[i]) / G;
+        c_h[i] = (m_begin + c_m[i]) - c_r[i] * G;
+    }
+    const uint32_t dr = 64u / G, dh = 64u - dr * G, r_last = (s.m_rows - 1) / G;
+    uint32_t m_ahead = 0;   // M rows (from m_begin) that the next copies start at
+    auto issue = [&](uint32_t slot) __attribute__((always_inline)) {
+        const uint32_t st = smem_addr + slot * STAGE;
+#pragma unroll
+        for (int i = 0; i < CPW; i++) {
+            const bool in = m_ahead + c_m[i] < rows;
+            const uint32_t r = in ? c_r[i] : r_last, h = in ? c_h[i] : G - 1;
+            stage::copy_lanes_16(st + RPC * (CPW * wave + i) * QROWB, q0 + static_cast<uint64_t>(r) * p.q_tok_stride + h * D + c_chunk[i] * 8);
+            c_h[i] += dh;
+            c_r[i] += dr;
+            const bool over = c_h[i] >= G;
+            c_h[i] -= over ? G : 0u;
+            c_r[i] += over ? 1u : 0u;
+        }
+        stage::copy_lanes_4(st + QBYTES + wave * 256, norm + min(m_ahead + lane, rows - 1));
+        m_ahead += 64;
+    };
+    const uint32_t row_off = D == 128 ? col * 256 : (col >> 1) * 256;
+    const uint32_t x = D == 128 ? (half ^ stage::pattern<D>(col)) << 4 : ((((col & 1) << 3) | half) ^ stage::pattern<D>(col >> 1)) << 4;
+    uint32_t slot = 0;
+    issue(0);
+    issue(1);
+    for (uint32_t it = 0; it < n_it; it++) {
+        stage::wait<CPW + 1>();   // this wave's share of the stage has landed
+        __syncthreads();          // ... and everybody else's; the stage before it is free
+        issue(slot == 0 ? 2u : slot - 1);
+        const unsigned char *st = smem + slot * STAGE;
+        slot = slot == 2 ? 0u : slot + 1;
+        const uint32_t m0 = m_begin + it * 64 + turn * 32;
+        // (a tile of rows that see none of the wave's positions, and one past the end)
+        if (m0 >= s.m_rows || s.cached + s.first + (m0 + 31) / G < p0) {
+            continue;
+        }
+        uint4 qop[KS];
+        const unsigned char *base = st + turn * 32 * QROWB + row_off;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            qop[ks] = *reinterpret_cast<const uint4 *>(base + (((2 * ks) << 4) ^ x));
+        }
+        float n[16];
+        const float *nl = reinterpret_cast<const float *>(st + QBYTES + wave * 256) + turn * 32 + half * 4;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const float4 v = *reinterpret_cast<const float4 *>(nl + g * 8);
+            n[4 * g] = v.x;
+            n[4 * g + 1] = v.y;
+            n[4 * g + 2] = v.z;
+            n[4 * g + 3] = v.w;
+        }
+        f32x16_t S[PT];
+#pragma unroll
+        for (int pt = 0; pt < PT; pt++) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                S[pt][k] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+            for (int pt = 0; pt < PT; pt++) {
+                S[pt] = mfma32<T>(qop[ks], kreg[pt][ks], S[pt]);
+            }
+        }
+        const bool masked = m0 + 32 > s.m_rows || p0 + 32 * PT - 1 > s.cached + s.first + m0 / G;
+#pragma unroll
+        for (int pt = 0; pt < PT; pt++) {
+            float sum = 0.f;
+            if (masked) {
+                // of the lane's rows, those from the first one that sees the position on
+                const uint32_t t = p0 + pt * 32 + col;
+                const uint32_t from = t > s.cached + s.first ? (t - s.cached - s.first) * G : 0u;
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const uint32_t mk = m0 + (k / 4) * 8 + half * 4 + (k % 4);
+                    const float e = fast_exp2(__builtin_fmaf(S[pt][k], mul[pt], n[k]));
+                    sum += mk < s.m_rows && mk >= from ? e : 0.f;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    sum += fast_exp2(__builtin_fmaf(S[pt][k], mul[pt], n[k]));
+                }
+            }
+            acc[pt] += sum;   // (a tile's sum first: 16 additions, then one per tile, not one chain over every row)
+        }
+    }
+    stage::wait<0>();
 #pragma unroll
     for (int pt = 0; pt < PT; pt++) {
         acc[pt] += __shfl_xor(acc[pt], 32);
@@ -749,7 +1109,22 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
             const uint32_t heads = std::min(n_kv_heads, 8u);
             store_scores_kernel<T, D, KVF><<<dim3(ceil_div(plan.splits, 8u / heads), batch, ceil_div(n_kv_heads, heads)), 512, 0, s>>>(p);
         } else {
-            row_stats_kernel<T, D, KVF><<<dim3(plan.tiles, plan.splits, n_kv_heads), kThreads, 0, s>>>(p);
+            // K through LDS: 16-bit caches whose copies (four positions of 128 elements, eight of 64) lie in one block, and a
+            // split's block-table entries behind the stages
+            bool staged = false;
+            if constexpr (D != 256 && KVF == XLITE_HIP_KV_SAME) {
+                const size_t lds = 4 * 64 * D * 2 + (static_cast<size_t>(plan.split_len / block_size) + 2) * sizeof(uint32_t);
+                staged = block_size % (512 / D) == 0 && p.block_magic != 0 && lds <= 80 * 1024;
+                if (staged) {
+                    if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(row_stats_staged_kernel<T, D>), lds)) {
+                        return rc;
+                    }
+                    row_stats_staged_kernel<T, D><<<dim3(plan.tiles, plan.splits, n_kv_heads), kThreads, lds, s>>>(p);
+                }
+            }
+            if (!staged) {
+                row_stats_kernel<T, D, KVF><<<dim3(plan.tiles, plan.splits, n_kv_heads), kThreads, 0, s>>>(p);
+            }
         }
         XL_LAUNCH_CHECK();
         if (plan.stored || plan.splits > 1) {
@@ -761,7 +1136,16 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
             const uint32_t z = std::max(1u, std::min(n_kv_heads, 512u / std::max(1u, tiles * batch)));   // few positions: the heads side by side
             sum_scores_kernel<<<dim3(tiles, batch, z), kThreads, 0, s>>>(p);
         } else {
-            column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 128u * kPosTiles<D>), batch, n_kv_heads), 2 * kThreads, 0, s>>>(p);
+const dim3 grid(ceil_div(max_ctx, 128u * kPosTiles<D>), batch, n_kv_heads);
+            if constexpr (D == 256) {
+                column_sums_kernel<T, D, KVF><<<grid, 2 * kThreads, 0, s>>>(p);
+            } else {
+                const size_t lds = 3 * (64 * D * 2 + 8 * 256);
+                if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(column_sums_staged_kernel<T, D, KVF>), lds)) {
+                    return rc;
+                }
+                column_sums_staged_kernel<T, D, KVF><<<grid, 2 * kThreads, lds, s>>>(p);
+            }
         }
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;
