@@ -25,9 +25,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256;
 constexpr uint32_t kRowTile = 4 * 64;         // M rows of a workgroup of the row statistics
-// tiles of 32 positions that a wave of the column sums owns (head_dim 256: the registers hold one)
-template <int D>
-constexpr int kPosTiles = D == 256 ? 1 : 2;
 constexpr uint32_t kMinSplit = 256;           // positions a split of the row statistics walks at least
 constexpr uint32_t kStoredRows = 32;          // M rows per sequence, on average, up to which the scores are stored
 
@@ -277,7 +274,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
 row_stats_staged_kernel(const WeightsParams p)
 {
-    constexpr int KS = D / 16, RT = 2, BN = 64, STAGES = 4;
+    constexpr int KS = D / 16, RT = 2, BN = 64, STAGES = 3;
     constexpr uint32_t ROWB = D * 2, STAGE = BN * ROWB, TILE = 4 * 32 * RT;
     constexpr int PPC = 1024 / ROWB;           // positions per copy
     constexpr int CPW = BN / PPC / 4;          // copies per wave and tile
@@ -354,7 +351,7 @@ row_stats_staged_kernel(const WeightsParams p)
             stage::copy_source<D>(lane, PPC * (CPW * wave + i), &c_row[i], &chunk);
             c_off[i] = chunk << 4;
         }
-        // copies of tile `tile` of the range into stage tile % 4; the positions of a copy share a block, those past the end
+        // copies of tile `tile` of the range into stage tile % 3; the positions of a copy share a block, those past the end
         // repeat the last one (their scores are masked)
         auto issue = [&](uint32_t tile) __attribute__((always_inline)) {
 #pragma unroll
@@ -375,11 +372,10 @@ row_stats_staged_kernel(const WeightsParams p)
         const uint32_t x = D == 128 ? (half ^ stage::pattern<D>(col)) << 4 : ((((col & 1) << 3) | half) ^ stage::pattern<D>(col >> 1)) << 4;
         issue(0);
         issue(1);
-        issue(2);
         for (uint32_t tile = 0; tile < n_tiles; tile++) {
-            stage::wait<2 * CPW>();   // this wave's share of `tile` has landed
-            __syncthreads();          // ... and everybody else's; stage (tile - 1) % 4 is free
-            issue(tile + 3);
+            stage::wait<CPW>();   // this wave's share of `tile` has landed
+            __syncthreads();      // ... and everybody else's; stage (tile - 1) % 3 is free
+            issue(tile + 2);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const uint32_t t0 = begin + tile * BN + h * 32;
@@ -414,20 +410,31 @@ row_stats_staged_kernel(const WeightsParams p)
                             S[rt][k] = t0 + (k / 4) * 8 + half * 4 + (k % 4) < lim ? S[rt][k] : -INFINITY;
                         }
                     }
-                    float mx = m_run[rt];
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        mx = fmaxf(mx, S[rt][k]);
-                    }
-                    const float m_safe = mx == -INFINITY ? 0.f : mx;
-                    const float neg = -m_safe * kLog2e;
+                    // The reference of a row's exponentials moves only when a tile's sum says so (the first tile's does): any
+                    // reference within 2^60 of the maximum gives the same sum in fp32, and finding every tile's maximum is
+                    // a tenth of the kernel's vector instructions.
                     float sum = 0.f;
+                    const float neg = -m_run[rt] * kLog2e;
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
                         sum += fast_exp2(__builtin_fmaf(S[rt][k], kLog2e, neg));
                     }
-                    l_run[rt] = l_run[rt] * fast_exp2((m_run[rt] - m_safe) * kLog2e) + sum;
-                    m_run[rt] = mx;
+                    if (__any(!(sum < 0x1p60f))) {   // (the first tile: the reference is -infinity, the sum infinite or NaN)
+                        float mx = m_run[rt];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            mx = fmaxf(mx, S[rt][k]);
+                        }
+                        const float m_safe = mx == -INFINITY ? 0.f : mx;
+                        sum = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            sum += fast_exp2(__builtin_fmaf(S[rt][k], kLog2e, -m_safe * kLog2e));
+                        }
+                        l_run[rt] *= fast_exp2((m_run[rt] - m_safe) * kLog2e);
+                        m_run[rt] = mx;
+                    }
+                    l_run[rt] += sum;
                 }
             }
         }
@@ -475,7 +482,7 @@ __global__ void __launch_bounds__(2 * kThreads)
 column_sums_kernel(const WeightsParams p)
 {
     constexpr int KS = D / 16;
-    constexpr int PT = kPosTiles<D>;          // tiles of 32 positions of a wave
+    constexpr int PT = 1;                     // tiles of 32 positions of a wave (the registers hold one)
     constexpr uint32_t WG = 4 * 32 * PT;      // positions of the workgroup: two waves for each 32 PT of them
     constexpr uint32_t ROWB = D * (KVF == XLITE_HIP_KV_SAME ? 2 : 1);
     __shared__ float other[4][32 * PT];
@@ -612,23 +619,27 @@ column_sums_kernel(const WeightsParams p)
     }
 }
 
-// The same for head_dim 64 and 128 with the query rows copied straight into LDS, 64 M rows at a time (32 for each half of
-// the waves), and their normalisers with them.
+// The same for head_dim 64 and 128 with the query rows copied straight into LDS, 32 M rows for each turn (four waves, 64
+// positions each) at a time, and their normalisers with them. As many turns as the registers hold waves: the exponentials of
+// a tile (96 vector instructions, 300 cycles with four waves on a SIMD, 410 with one) run beside the products of the others.
+template <int D>
+constexpr int kTurns = D == 128 ? 3 : 4;
+
 template <typename T, int D, int KVF>
-__global__ void __launch_bounds__(2 * kThreads)
+__global__ void __launch_bounds__(kTurns<D> * kThreads)
 column_sums_staged_kernel(const WeightsParams p)
 {
-    constexpr int KS = D / 16, PT = 2, STAGES = 3;
+    constexpr int KS = D / 16, PT = 2, STAGES = 3, TURNS = kTurns<D>, ROWS = 32 * TURNS;
     constexpr uint32_t ROWB = D * (KVF == XLITE_HIP_KV_SAME ? 2 : 1), QROWB = D * 2;
-    constexpr uint32_t QBYTES = 64 * QROWB, STAGE = QBYTES + 8 * 256;   // the rows, then the normalisers once per wave
-    constexpr int RPC = 1024 / QROWB, CPW = 64 / RPC / 8;               // rows per copy, copies per wave
+    constexpr uint32_t QBYTES = ROWS * QROWB, STAGE = QBYTES + 4 * TURNS * 256;   // the rows, then each wave's normalisers
+    constexpr int RPC = 1024 / QROWB, CPW = 8 / RPC;                    // rows per copy, copies per wave
     constexpr uint32_t WG = 4 * 32 * PT;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    __shared__ float other[4][32 * PT];
+    __shared__ float other[TURNS][4][32 * PT];
     const uint32_t smem_addr = stage::lds_address(smem);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.z, seq = blockIdx.y, G = p.group;
-    const uint32_t mine = wave & 3u, turn = wave >> 2;   // which 64 positions, and which half of the staged rows
+    const uint32_t mine = wave & 3u, turn = wave >> 2;   // which 64 positions, and which 32 of the staged rows
     const Sequence s = sequence_of(p, seq);
     const uint32_t total = s.cached + s.nodes;
     const uint32_t wg0 = blockIdx.x * WG;
@@ -664,12 +675,12 @@ column_sums_staged_kernel(const WeightsParams p)
         }
     }
     // from the first row that sees the workgroup's first position on (rows before it see none of its positions)
-    const uint32_t m_begin = (wg0 > s.cached + s.first ? (wg0 - s.cached - s.first) * G : 0u) & ~63u;
-    const uint32_t rows = s.m_rows - m_begin, n_it = ceil_div(rows, 64u);   // (the last row sees every position: rows > 0)
+    const uint32_t m_begin = (wg0 > s.cached + s.first ? (wg0 - s.cached - s.first) * G : 0u) & ~31u;
+    const uint32_t rows = s.m_rows - m_begin, n_it = ceil_div(rows, static_cast<uint32_t>(ROWS));   // (the last row sees every position: rows > 0)
     const uint64_t tok0 = s.start + s.first;
     const float *norm = p.norm + static_cast<uint64_t>(kvh) * p.m_total + tok0 * G + m_begin;
     const uint16_t *q0 = p.q + tok0 * p.q_tok_stride + static_cast<uint64_t>(kvh * G) * D;
-    // a lane's rows of the copies: M row m_begin + 64 it + c_row, as (token, head); rows past the end repeat the last one
+    // a lane's rows of the copies: M row m_begin + ROWS it + c_m, as (token, head); rows past the end repeat the last one
     uint32_t c_m[CPW], c_r[CPW], c_h[CPW], c_chunk[CPW];
 #pragma unroll
     for (int i = 0; i < CPW; i++) {
@@ -680,7 +691,7 @@ column_sums_staged_kernel(const WeightsParams p)
         c_r[i] = (m_begin + c_m[i]) / G;
         c_h[i] = (m_begin + c_m[i]) - c_r[i] * G;
     }
-    const uint32_t dr = 64u / G, dh = 64u - dr * G, r_last = (s.m_rows - 1) / G;
+    const uint32_t dr = ROWS / G, dh = ROWS - dr * G, r_last = (s.m_rows - 1) / G;
     uint32_t m_ahead = 0;   // M rows (from m_begin) that the next copies start at
     auto issue = [&](uint32_t slot) __attribute__((always_inline)) {
         const uint32_t st = smem_addr + slot * STAGE;
@@ -695,8 +706,8 @@ column_sums_staged_kernel(const WeightsParams p)
             c_h[i] -= over ? G : 0u;
             c_r[i] += over ? 1u : 0u;
         }
-        stage::copy_lanes_4(st + QBYTES + wave * 256, norm + min(m_ahead + lane, rows - 1));
-        m_ahead += 64;
+        stage::copy_lanes_4(st + QBYTES + wave * 256, norm + min(m_ahead + 32 * turn + (lane & 31u), rows - 1));
+        m_ahead += ROWS;
     };
     const uint32_t row_off = D == 128 ? col * 256 : (col >> 1) * 256;
     const uint32_t x = D == 128 ? (half ^ stage::pattern<D>(col)) << 4 : ((((col & 1) << 3) | half) ^ stage::pattern<D>(col >> 1)) << 4;
@@ -709,7 +720,7 @@ column_sums_staged_kernel(const WeightsParams p)
         issue(slot == 0 ? 2u : slot - 1);
         const unsigned char *st = smem + slot * STAGE;
         slot = slot == 2 ? 0u : slot + 1;
-        const uint32_t m0 = m_begin + it * 64 + turn * 32;
+        const uint32_t m0 = m_begin + it * ROWS + turn * 32;
         // (a tile of rows that see none of the wave's positions, and one past the end)
         if (m0 >= s.m_rows || s.cached + s.first + (m0 + 31) / G < p0) {
             continue;
@@ -721,7 +732,7 @@ column_sums_staged_kernel(const WeightsParams p)
             qop[ks] = *reinterpret_cast<const uint4 *>(base + (((2 * ks) << 4) ^ x));
         }
         float n[16];
-        const float *nl = reinterpret_cast<const float *>(st + QBYTES + wave * 256) + turn * 32 + half * 4;
+        const float *nl = reinterpret_cast<const float *>(st + QBYTES + wave * 256) + half * 4;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
             const float4 v = *reinterpret_cast<const float4 *>(nl + g * 8);
@@ -772,8 +783,8 @@ column_sums_staged_kernel(const WeightsParams p)
 #pragma unroll
     for (int pt = 0; pt < PT; pt++) {
         acc[pt] += __shfl_xor(acc[pt], 32);
-        if (turn == 1 && half == 0) {
-            other[mine][pt * 32 + col] = acc[pt];
+        if (turn != 0 && half == 0) {
+            other[turn][mine][pt * 32 + col] = acc[pt];
         }
     }
     __syncthreads();
@@ -782,7 +793,11 @@ column_sums_staged_kernel(const WeightsParams p)
         for (int pt = 0; pt < PT; pt++) {
             const uint32_t t = p0 + pt * 32 + col;
             if (t < total) {
-                const float sum = acc[pt] + other[mine][pt * 32 + col];
+                float sum = acc[pt];
+#pragma unroll
+                for (int u = 1; u < TURNS; u++) {
+                    sum += other[u][mine][pt * 32 + col];
+                }
                 p.weights[at[pt]] = t < s.cached ? p.weights[at[pt]] + sum : sum;
             }
         }
@@ -1019,7 +1034,7 @@ Plan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint3
         plan.tiles = by_prefix;
     }
     // splits of the row statistics: enough workgroups (of four waves) for four per compute unit
-    const uint32_t want = ceil_div(1024u, std::max(1u, plan.tiles * n_kv_heads));
+    const uint32_t want = ceil_div(2048u, std::max(1u, plan.tiles * n_kv_heads));
     plan.splits = std::max(1u, std::min(want, max_ctx / kMinSplit));
     plan.split_len = ceil_div(ceil_div(max_ctx, plan.splits), 32u) * 32u;
     const size_t rows = static_cast<size_t>(total_tokens) * n_heads;
@@ -1113,8 +1128,8 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
             // split's block-table entries behind the stages
             bool staged = false;
             if constexpr (D != 256 && KVF == XLITE_HIP_KV_SAME) {
-                const size_t lds = 4 * 64 * D * 2 + (static_cast<size_t>(plan.split_len / block_size) + 2) * sizeof(uint32_t);
-                staged = block_size % (512 / D) == 0 && p.block_magic != 0 && lds <= 80 * 1024;
+                const size_t lds = 3 * 64 * D * 2 + (static_cast<size_t>(plan.split_len / block_size) + 2) * sizeof(uint32_t);
+                staged = block_size % (512 / D) == 0 && p.block_magic != 0 && lds <= 64 * 1024;
                 if (staged) {
                     if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(row_stats_staged_kernel<T, D>), lds)) {
                         return rc;
@@ -1136,15 +1151,14 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
             const uint32_t z = std::max(1u, std::min(n_kv_heads, 512u / std::max(1u, tiles * batch)));   // few positions: the heads side by side
             sum_scores_kernel<<<dim3(tiles, batch, z), kThreads, 0, s>>>(p);
         } else {
-const dim3 grid(ceil_div(max_ctx, 128u * kPosTiles<D>), batch, n_kv_heads);
             if constexpr (D == 256) {
-                column_sums_kernel<T, D, KVF><<<grid, 2 * kThreads, 0, s>>>(p);
+                column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 128u), batch, n_kv_heads), 2 * kThreads, 0, s>>>(p);
             } else {
-                const size_t lds = 3 * (64 * D * 2 + 8 * 256);
+                const size_t lds = 3 * kTurns<D> * (32 * D * 2 + 4 * 256);
                 if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(column_sums_staged_kernel<T, D, KVF>), lds)) {
                     return rc;
                 }
-                column_sums_staged_kernel<T, D, KVF><<<grid, 2 * kThreads, lds, s>>>(p);
+                column_sums_staged_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 256u), batch, n_kv_heads), kTurns<D> * kThreads, lds, s>>>(p);
             }
         }
         XL_LAUNCH_CHECK();
