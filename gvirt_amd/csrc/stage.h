@@ -16,6 +16,12 @@ __device__ __forceinline__ void copy_1k(uint32_t lds_addr, uint32_t voff, const 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
                  :: "s"(lds_addr), "v"(voff), "s"(base) : "memory", "m0");
 }
+// the same for bytes that nobody reads again: they displace nothing on their way through the caches
+__device__ __forceinline__ void copy_1k_once(uint32_t lds_addr, uint32_t voff, const void *base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\t"
+                 :: "s"(lds_addr), "v"(voff), "s"(base) : "memory", "m0");
+}
 // the same from an address per lane, 16 or 4 bytes each
 __device__ __forceinline__ void copy_lanes_16(uint32_t lds_addr, const void *src)
 {

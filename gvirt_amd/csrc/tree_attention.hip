@@ -2,8 +2,9 @@
 // nodes of one drafted tree per sequence, already written to the cache behind the cached positions; a row sees every
 // cached position and those nodes whose bit its mask has:
 //     out_r = sum_j [seen(r, j)] exp(q_r . k_j) v_j / sum_j [seen(r, j)] exp(q_r . k_j),   0 where nothing is seen.
-// The walk is that of a prefill chunk with another mask, and only tiles that reach into the tree look at it, so the
-// prefill kernels serve it with a mask of their own (prefill_mfma.hip, mfma_attention.hip: TREE).
+// head_dim 128 over 16-bit caches: a kernel of its own that streams the cache past all rows of a tree (tree_stream.hip).
+// Other shapes: the walk is that of a prefill chunk with another mask, and only tiles that reach into the tree look at it, so
+// the prefill kernels serve them with a mask of their own (prefill_mfma.hip, mfma_attention.hip: TREE).
 #include <algorithm>
 
 #include "attention_common.h"
@@ -36,6 +37,9 @@ extern "C" size_t xlite_hip_tree_attention_workspace_bytes(uint32_t total_tokens
         return 0;
     }
     size_t need = tree_bytes_16(total_tokens, n_heads, n_kv_heads, head_dim, batch, max_num_block * block_size);
+    if (tree_stream_supported(n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, kv_dtype)) {
+        need = std::max(need, tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, batch, block_size, max_num_block));
+    }
     if (kv_dtype != XLITE_HIP_KV_SAME) {
         need += kv_dequant_bytes(n_kv_heads, head_dim, block_size, batch, max_num_block);
         need += kv_dequant_f16_io_bytes(total_tokens, n_heads, n_kv_heads, head_dim);   // bf16 models (the size does not know)
@@ -76,6 +80,10 @@ extern "C" int xlite_hip_tree_attention(void *stream, const void *qkv, const voi
     a.mask_words = mask_words;
     hipStream_t s = as_stream(stream);
     if (kv_dtype == XLITE_HIP_KV_SAME) {
+        if (tree_stream_supported(n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, kv_dtype) && workspace != nullptr &&
+            workspace_bytes >= tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, batch, block_size, max_num_block)) {
+            return launch_tree_stream(s, a);
+        }
         return run_16(s, a);
     }
     // a cache of bytes: read by the prefill kernel itself (head_dim 128; a tree is a short chunk), otherwise through an

@@ -1,0 +1,664 @@
+// Attention over drafted trees for head_dim 128 and 16-bit caches: the cache streamed once, past all rows of a tree.
+//
+// A tree has few rows (nodes x query heads of a kv head: an M row each), so its attention is bound by reading K and V. The
+// prefill kernel gives a workgroup one kv head: its copies are 256-byte rows up to two kilobytes apart, which memory serves
+// at two thirds of the rate of longer runs, and four of its eight waves have no rows. Here a workgroup takes two kv heads
+// times 128 M rows or one times 256, a wave 32 M rows of one head (the most that queries, results and operands
+// leave registers for at two waves per SIMD), and copies of 1 KiB fetch the heads of a position together:
+//     S^T[pos][m]  = K[pos][:] . Q[m][:]           v_mfma_f32_32x32x16 (A = K rows, ds_read_b128; B = Q)
+//     O^T[d][m]   += V^T[d][pos] . P^T[pos][m]     v_mfma_f32_32x32x16 (A = V^T, ds_read_b64_tr_b16; B = P)
+// Four stages of 32 KiB: one is consumed while three are on their way (with two of 64 KiB half of what memory delivers in a
+// round trip was not asked for: 447 against XXX us for 64 trees of 32 over 8192 positions).
+//
+// Work split: a sequence owns ceil(len G / rows) M tiles of ceil((cached + len) / step) steps each; the steps of all M tiles laid
+// end to end are cut into equal chunks, one per workgroup, whatever the sequences' lengths (they live in device memory: every
+// workgroup forms the prefix sums itself). A chunk that crosses an M tile's end runs as several segments. Chunk c owns the
+// partial slots 2 c (its first segment) and 2 c + 1 (its last, when that is another one); an M tile cut into n segments from
+// chunk c0 on finds them at 2 c0 (+ 1 unless it is that chunk's first), 2 (c0 + 1), ..., which its meta entry tells the merge.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_common.h"
+#include "stage.h"
+
+namespace xlite {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleSlack = 2.0f / kLog2e;   // the reference maximum moves when a score exceeds it by a factor of 4
+constexpr int D = 128;
+constexpr int kWaves = 8;
+constexpr int kThreads = kWaves * 64;
+constexpr uint32_t kHalf = 16 * 1024;            // K or V of a stage: 32 positions of two kv heads, 64 of one
+constexpr uint32_t kStages = 4;
+template <int NH>
+constexpr uint32_t kRows = 32 * kWaves / NH;     // M rows of a workgroup, per kv head
+constexpr uint32_t kStage = 2 * kHalf;
+constexpr uint32_t kTblCap = 2048;               // block-table entries staged per segment
+constexpr uint32_t kSeqCap = 1024;               // sequences whose prefix sums fit
+constexpr uint32_t kMinChunk = 4;                // steps
+constexpr uint32_t kComputeUnits = 256;
+
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_t;
+
+template <typename T>
+__device__ __forceinline__ f32x16_t mfma32(const uint4 &a, const uint4 &b, f32x16_t c)
+{
+    if constexpr (T::kCode == XLITE_HIP_BF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+    }
+}
+
+struct StreamParams {
+    const uint16_t *q;
+    const uint16_t *k_cache;
+    const uint16_t *v_cache;
+    uint16_t *out;
+    const uint32_t *tree_mask;
+    const int32_t *query_start_loc;
+    const int32_t *lens;
+    const int32_t *cached_lens;
+    const int32_t *block_tables;
+    int4 *meta;            // [M tile id]: segments to merge (0: the results are final), first chunk, first-segment flag
+    float *acc;            // [head group][slot][kv head of the group][M rows of a tile][D], not normalised
+    float *ml;             // the same without D: reference maximum (log2 domain), normaliser
+    uint32_t q_tok_stride, n_heads, n_kv_heads, group;
+    uint32_t batch, block_size, block_magic, max_num_block, mask_words;
+    uint32_t slots;        // 2 x chunks a launch may have
+};
+
+// M tile ids of a sequence: floor(start * G / rows) + i on, at least as many as it has M tiles
+template <int NH>
+__device__ __forceinline__ uint32_t first_id(const StreamParams &p, uint32_t start, uint32_t seq)
+{
+    return static_cast<uint32_t>(static_cast<uint64_t>(start) * p.group / kRows<NH>) + seq;
+}
+__device__ __forceinline__ uint32_t uni(uint32_t x)
+{
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+}
+
+// NH: kv heads of a workgroup
+template <typename T, int NH>
+__global__ void __launch_bounds__(kThreads, 1)
+tree_stream_kernel(const StreamParams p)
+{
+    constexpr int KS = D / 16, DT = D / 32;
+    constexpr uint32_t ROWS = kRows<NH>;
+    constexpr uint32_t POSB = NH * 256;          // LDS bytes of a position
+    constexpr uint32_t SP = kHalf / POSB;        // positions of a step
+    constexpr uint32_t PPI = 1024 / POSB;        // positions of a copy
+    constexpr int CPW = 2;                       // copies per wave, step and tensor
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    uint32_t *tbl = reinterpret_cast<uint32_t *>(smem + kStages * kStage);
+    uint32_t *pref = tbl + kTblCap;              // batch + 1 words
+    const uint32_t smem_addr = stage::lds_address(smem);
+    const uint32_t lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const uint32_t G = p.group;
+    const uint32_t hsel = wave % NH, row_tile = wave / NH;
+    const uint32_t kvh = blockIdx.y * NH + hsel;
+
+    // ---- steps of every sequence, summed: thread t owns consecutive sequences
+    auto weight = [&](uint32_t i) {
+        const int32_t n = p.lens[i], c = p.cached_lens[i];
+        return n <= 0 ? 0u : ceil_div(static_cast<uint32_t>(c + n), SP) * ceil_div(static_cast<uint32_t>(n) * G, ROWS);
+    };
+    {
+        const uint32_t per = ceil_div(p.batch, static_cast<uint32_t>(kThreads));
+        const uint32_t i0 = min(p.batch, threadIdx.x * per), i1 = min(p.batch, i0 + per);
+        uint32_t mine = 0;
+        for (uint32_t i = i0; i < i1; i++) {
+            mine += weight(i);
+        }
+        uint32_t incl = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(incl, d);
+            incl += lane >= static_cast<uint32_t>(d) ? up : 0u;
+        }
+        if (lane == 63) {
+            tbl[wave] = incl;   // (the table's words are not in use yet)
+        }
+        __syncthreads();
+        uint32_t run = incl - mine;
+        for (uint32_t w = 0; w < wave; w++) {
+            run += tbl[w];
+        }
+        for (uint32_t i = i0; i < i1; i++) {
+            pref[i] = run;
+            run += weight(i);
+        }
+        if (threadIdx.x == kThreads - 1) {
+            pref[p.batch] = run;
+        }
+        __syncthreads();
+    }
+    const uint32_t total = uni(pref[p.batch]);
+    uint32_t chunk = max(ceil_div(total, gridDim.x), kMinChunk);
+    chunk = min(chunk, (kTblCap - 2) * p.block_size / SP);
+    const uint32_t n_chunks = ceil_div(total, chunk);
+
+    // ---- read roles (the pattern of position p + 32 is that of p)
+    const uint32_t k_off = col * POSB + hsel * 256;
+    const uint32_t kx = (half ^ stage::pattern<D>(col)) << 4;
+    uint32_t v_off;
+    {
+        const uint32_t g = lane >> 4, jp = (lane & 15) >> 2, q = lane & 3;
+        const uint32_t y = 2 * (g & 1) + (q >> 1), pos = 4 * (g >> 1) + jp;
+        v_off = kHalf + pos * POSB + hsel * 256 + ((y ^ stage::pattern<D>(pos)) << 4) + ((q & 1) << 3);
+    }
+    // ---- copy role: wave w fills copies 2 w and 2 w + 1 of the K and of the V half. Lane l of a copy: row l / 16 of its four
+    // (position, kv head) rows, chunk slot l % 16, which receives chunk slot ^ pattern(position)
+    const uint32_t row_bytes = p.n_kv_heads * 256;
+    for (uint32_t c = blockIdx.x; c < n_chunks; c += gridDim.x) {
+        const uint32_t c_begin = c * chunk, c_end = min(total, c_begin + chunk);
+        uint32_t at = c_begin;
+        uint32_t seq = 0;   // the last sequence whose first step is at or before `at`
+        {
+            uint32_t hi = p.batch;
+            while (hi - seq > 1) {
+                const uint32_t mid = (seq + hi) >> 1;
+                if (uni(pref[mid]) <= at) {
+                    seq = mid;
+                } else {
+                    hi = mid;
+                }
+            }
+        }
+        while (at < c_end) {
+            const uint32_t first = uni(pref[seq]), next = uni(pref[seq + 1]);
+            if (next == first) {   // no rows
+                seq++;
+                continue;
+            }
+            // ---- the segment: steps a .. b - 1 of M tile mt
+            const uint32_t nodes = uni(static_cast<uint32_t>(p.lens[seq])), cached = uni(static_cast<uint32_t>(p.cached_lens[seq]));
+            const uint32_t start = uni(static_cast<uint32_t>(p.query_start_loc[seq]));
+            const uint32_t range = cached + nodes, steps = ceil_div(range, SP);
+            const uint32_t mt = (at - first) / steps, a = (at - first) - mt * steps, b = min(steps, a + (c_end - at));
+            const uint32_t tile_first = first + mt * steps;      // of the M tile, in all steps
+            const bool whole = a == 0 && b == steps;
+            const bool first_seg = at == c_begin;
+            const uint32_t id = first_id<NH>(p, start, seq) + mt;
+            const uint32_t m_rows = nodes * G, m_first = mt * ROWS + row_tile * 32;   // (the wave's first)
+            const bool has_rows = m_first < m_rows;
+            const uint32_t m = min(m_first + col, m_rows - 1);       // (rows past the end repeat the last one, unstored)
+            const uint64_t tok = start + m / G;
+            const uint32_t head = kvh * G + m % G;
+            const uint32_t t0 = a * SP, t1 = min(range, b * SP);
+            const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
+            const uint32_t blk0 = t0 / p.block_size, blk1 = (t1 - 1) / p.block_size;
+
+            // ---- set-up: block-table entries, then the query rows, then the first two steps' copies
+            __syncthreads();   // (the table and the stages of the last segment have been read)
+            for (uint32_t i = threadIdx.x; i <= blk1 - blk0; i += kThreads) {
+                tbl[i] = static_cast<uint32_t>(table[blk0 + i]);
+            }
+            uint4 qreg[KS];
+            const uint16_t *src = p.q + tok * p.q_tok_stride + static_cast<uint64_t>(head) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                qreg[ks] = *reinterpret_cast<const uint4 *>(src + ks * 16 + half * 8);
+            }
+            if (a == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+                const uint32_t n = whole ? 0u : (tile_first + steps - 1) / chunk - c + 1;
+                p.meta[id] = make_int4(static_cast<int>(n), static_cast<int>(c), first_seg ? 1 : 0, 0);
+            }
+            f32x16_t O[DT];
+            float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    O[dt][k] = 0.f;
+                }
+            }
+            // complete these loads before any copy is issued: memory answers in order
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                asm volatile("" : "+v"(qreg[ks].x), "+v"(qreg[ks].y), "+v"(qreg[ks].z), "+v"(qreg[ks].w));
+            }
+            __syncthreads();
+            // copies of step `s` (from t0) into stage s % 4. Positions at or beyond t1 re-read the last one (their scores are
+            // masked). The positions of a copy share a block, and if blocks are multiples of all of a wave's, those do.
+            const bool one_block = p.block_size % (CPW * PPI) == 0;
+            auto issue = [&](uint32_t s) __attribute__((always_inline)) {
+                const uint32_t base_pos = t0 + s * SP + CPW * wave * PPI;
+                const uint32_t st = smem_addr + (s % kStages) * kStage + wave * (CPW * 1024);
+                const char *kc = reinterpret_cast<const char *>(p.k_cache) + blockIdx.y * (NH * 256);
+                const char *vc = reinterpret_cast<const char *>(p.v_cache) + blockIdx.y * (NH * 256);
+                // (worked out anew in every step, from a lane number that the compiler cannot carry along: a register spilled
+                // in this loop is reloaded by a memory load, whose wait is for every copy on its way)
+                uint32_t l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+                asm volatile("" : "+v"(l));
+                const uint32_t c_rel = (l >> 4) / NH, c_head = (l >> 4) % NH;
+                auto c_off = [&](int i) __attribute__((always_inline)) {
+                    const uint32_t pos = (CPW * wave + i) * PPI + c_rel;
+                    return c_head * 256 + (((l & 15u) ^ stage::pattern<D>(pos)) << 4);
+                };
+                if (one_block && base_pos + CPW * PPI <= t1) {
+                    const uint32_t blk = __umulhi(base_pos, p.block_magic);
+                    const uint32_t phys = uni(tbl[blk - blk0]);
+                    const uint64_t row0 = static_cast<uint64_t>(phys) * p.block_size + (base_pos - blk * p.block_size);
+                    const char *kb = kc + row0 * row_bytes, *vb = vc + row0 * row_bytes;
+#pragma unroll
+                    for (int i = 0; i < CPW; i++) {
+                        stage::copy_1k_once(st + i * 1024, c_off(i) + c_rel * row_bytes, kb + static_cast<uint32_t>(i * PPI) * row_bytes);
+                    }
+#pragma unroll
+                    for (int i = 0; i < CPW; i++) {
+                        stage::copy_1k_once(st + kHalf + i * 1024, c_off(i) + c_rel * row_bytes, vb + static_cast<uint32_t>(i * PPI) * row_bytes);
+                    }
+                    return;
+                }
+#pragma unroll
+                for (int i = 0; i < CPW; i++) {
+                    const uint32_t t_raw = base_pos + i * PPI;
+                    const uint32_t t = min(t_raw, t1 - 1) & ~(PPI - 1);
+                    const uint32_t rel = min(t_raw + c_rel, t1 - 1) - t;
+                    const uint32_t blk = __umulhi(t, p.block_magic);
+                    const uint32_t phys = uni(tbl[blk - blk0]);
+                    const uint64_t row0 = static_cast<uint64_t>(phys) * p.block_size + (t - blk * p.block_size);
+                    const char *kb = kc + row0 * row_bytes, *vb = vc + row0 * row_bytes;
+                    stage::copy_1k_once(st + i * 1024, c_off(i) + rel * row_bytes, kb);
+                    stage::copy_1k_once(st + kHalf + i * 1024, c_off(i) + rel * row_bytes, vb);
+                }
+            };
+
+            // 32 positions of a step: those from 32 h on. Register k of S holds position j0 + 8 (k / 4) + 4 half + k % 4.
+            auto compute = [&](uint32_t s, uint32_t h, auto mask_tag) __attribute__((always_inline)) {
+                constexpr bool MASK = decltype(mask_tag)::value;
+                const uint32_t j0 = t0 + s * SP + 32 * h;
+                const unsigned char *st = smem + (s % kStages) * kStage + h * 32 * POSB;
+                uint4 kop[KS];
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    kop[ks] = *reinterpret_cast<const uint4 *>(st + k_off + (((2 * ks) << 4) ^ kx));
+                }
+                f32x16_t S;
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    S[k] = 0.f;
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    S = mfma32<T>(kop[ks], qreg[ks], S);
+                }
+                // V^T operands: on their way during the softmax
+                typedef s16x4_t __attribute__((address_space(3))) * lds_tr_ptr;
+                unsigned char *vbase = const_cast<unsigned char *>(st);
+                uint4 vop[2][DT];
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+                        const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_tr_ptr)(vbase + kk * 16 * POSB + (v_off ^ (dt << 6)))));
+                        // 8 positions further: the pattern of position p + 8 is that of p XOR 2
+                        const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_tr_ptr)(vbase + (kk * 16 + 8) * POSB + (v_off ^ ((dt << 6) | (1 << 5))))));
+                        vop[kk][dt] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                [[maybe_unused]] uint32_t seen = 0;
+                if constexpr (MASK) {
+                    seen = tree_seen(p.tree_mask + tok * p.mask_words, p.mask_words, j0, cached, nodes) & ones(static_cast<int32_t>(t1 - j0));
+                    seen >>= 4 * half;
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        S[k] = (seen >> ((k / 4) * 8 + (k % 4))) & 1u ? S[k] : -INFINITY;
+                    }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    mx = fmaxf(mx, S[k]);
+                }
+                {
+                    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+                }
+                // (the reference moves only when exceeded by more than a factor of 4, as in the prefill kernel)
+                const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
+                const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+                const float alpha = fast_exp2((m_run - m_safe) * kLog2e);
+                const float neg_m = -m_safe * kLog2e;
+                m_run = m_new;
+                uint32_t w[8];
+                float psum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    const float e0 = fast_exp2(__builtin_fmaf(S[k], kLog2e, neg_m));
+                    const float e1 = fast_exp2(__builtin_fmaf(S[k + 1], kLog2e, neg_m));
+                    psum += e0 + e1;
+                    w[k / 2] = T::pack(e0, e1);   // rounded to the products' type: half a step of it, 2^-8 (2^-11) of each
+                }
+                const uint4 pb[2] = {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
+                l_run = l_run * alpha + psum;
+                if (__any(alpha != 1.0f)) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            // (in place: an opaque multiply keeps the accumulators in the same registers on both paths)
+                            asm volatile("v_mul_f32 %0, %1, %0" : "+v"(O[dt][k]) : "v"(alpha));
+                        }
+                    }
+                }
+                if constexpr (MASK) {
+                    // infinities and NaNs in V rows that some rows do not see (as in the prefill kernel)
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) {
+                            odd |= not_finite2<T>(vop[kk][dt].x) | not_finite2<T>(vop[kk][dt].y) | not_finite2<T>(vop[kk][dt].z) |
+                                   not_finite2<T>(vop[kk][dt].w);
+                        }
+                    }
+                    if (__any(odd)) {
+                        uint32_t sw[8];
+#pragma unroll
+                        for (int k = 0; k < 16; k += 2) {
+                            sw[k / 2] = T::pack((seen >> ((k / 4) * 8 + (k % 4))) & 1u ? 1.f : 0.f,
+                                                (seen >> (((k + 1) / 4) * 8 + ((k + 1) % 4))) & 1u ? 1.f : 0.f);
+                        }
+                        const uint4 sb[2] = {make_uint4(sw[0], sw[1], sw[2], sw[3]), make_uint4(sw[4], sw[5], sw[6], sw[7])};
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                            for (int what = 0; what < 3; what++) {
+                                f32x16_t hit;
+#pragma unroll
+                                for (int k = 0; k < 16; k++) {
+                                    hit[k] = 0.f;
+                                }
+#pragma unroll
+                                for (int kk = 0; kk < 2; kk++) {
+                                    hit = mfma32<T>(odd_values<T>(make_uint2(vop[kk][dt].x, vop[kk][dt].y), make_uint2(vop[kk][dt].z, vop[kk][dt].w), what),
+                                                    sb[kk], hit);
+                                }
+#pragma unroll
+                                for (int k = 0; k < 16; k++) {
+                                    O[dt][k] += hit[k] > 0.f ? (what == 0 ? INFINITY : what == 1 ? -INFINITY : NAN) : 0.f;
+                                }
+                            }
+#pragma unroll
+                            for (int kk = 0; kk < 2; kk++) {
+                                vop[kk][dt] = make_uint4(finite_only<T>(vop[kk][dt].x), finite_only<T>(vop[kk][dt].y),
+                                                         finite_only<T>(vop[kk][dt].z), finite_only<T>(vop[kk][dt].w));
+                            }
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+                        O[dt] = mfma32<T>(vop[kk][dt], pb[kk], O[dt]);
+                    }
+                }
+            };
+
+            const uint32_t n_steps = b - a, last = n_steps - 1;
+            // steps wholly below the cached length are seen by every row
+            const uint32_t plain = min(n_steps, cached > t0 ? (cached - t0) / SP : 0u);
+            issue(0);
+            if (last >= 1) {
+                issue(1);
+            }
+            if (last >= 2) {
+                issue(2);
+            }
+            auto turn = [&](uint32_t s, auto mask_tag) __attribute__((always_inline)) {
+                // this wave's share of step s has landed: only those of the next two are out
+                if (s + 2 <= last) {
+                    stage::wait<4 * CPW>();
+                } else if (s + 1 <= last) {
+                    stage::wait<2 * CPW>();
+                } else {
+                    stage::wait<0>();
+                }
+                __syncthreads();   // ... and everybody else's; the stage of step s - 1 is free
+                if (s + 3 <= last) {
+                    issue(s + 3);
+                }
+                if (has_rows) {    // (a wave without rows only copies)
+#pragma unroll 1
+                    for (uint32_t h = 0; h < SP / 32; h++) {
+                        compute(s, h, mask_tag);
+                    }
+                }
+            };
+            uint32_t s = 0;
+            for (; s < plain; s++) {
+                turn(s, std::integral_constant<bool, false>{});
+            }
+            for (; s < n_steps; s++) {
+                turn(s, std::integral_constant<bool, true>{});
+            }
+
+            // ---- results. O^T lane layout: column = M row, register k of tile dt = element 32 dt + 8 (k / 4) + 4 half + k % 4
+            const float l_tot = l_run + __shfl_xor(l_run, 32);
+            if (m_first + col < m_rows) {
+                if (whole) {
+                    const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;   // (NaN is not above 0 ...)
+                    const float scale = l_tot != l_tot ? l_tot : inv;     // (... and stays NaN)
+                    uint16_t *dst = p.out + (tok * p.n_heads + head) * D;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                        for (int kg = 0; kg < 4; kg++) {
+                            uint2 o;
+                            o.x = T::pack(O[dt][kg * 4] * scale, O[dt][kg * 4 + 1] * scale);
+                            o.y = T::pack(O[dt][kg * 4 + 2] * scale, O[dt][kg * 4 + 3] * scale);
+                            *reinterpret_cast<uint2 *>(dst + dt * 32 + kg * 8 + half * 4) = o;
+                        }
+                    }
+                } else {
+                    const uint64_t slot = static_cast<uint64_t>(blockIdx.y) * p.slots + 2 * c + (first_seg ? 0u : 1u);
+                    const uint64_t row = (slot * NH + hsel) * ROWS + row_tile * 32 + col;
+                    float *dst = p.acc + row * D;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                        for (int kg = 0; kg < 4; kg++) {
+                            *reinterpret_cast<float4 *>(dst + dt * 32 + kg * 8 + half * 4) =
+                                make_float4(O[dt][kg * 4], O[dt][kg * 4 + 1], O[dt][kg * 4 + 2], O[dt][kg * 4 + 3]);
+                        }
+                    }
+                    if (half == 0) {
+                        *reinterpret_cast<float2 *>(p.ml + row * 2) = make_float2(m_run * kLog2e, l_tot);
+                    }
+                }
+            }
+            at += b - a;
+            if (at >= next) {
+                seq++;
+            }
+        }
+    }
+}
+
+// Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), 16 threads of 8 columns per row.
+template <typename T, int NH>
+__global__ void __launch_bounds__(256)
+tree_merge_kernel(const StreamParams p)
+{
+    const uint32_t id = blockIdx.x, kvh = blockIdx.y, G = p.group;
+    uint32_t seq = 0;   // the last sequence whose ids start at or before `id`
+    {
+        uint32_t hi = p.batch;
+        while (hi - seq > 1) {
+            const uint32_t mid = (seq + hi) >> 1;
+            if (first_id<NH>(p, static_cast<uint32_t>(p.query_start_loc[mid]), mid) <= id) {
+                seq = mid;
+            } else {
+                hi = mid;
+            }
+        }
+    }
+    const int32_t n = p.lens[seq];
+    const uint32_t start = static_cast<uint32_t>(p.query_start_loc[seq]);
+    const uint32_t mt = id - first_id<NH>(p, start, seq);
+    const uint32_t in_tile = blockIdx.z * 16 + threadIdx.x / 16, m = mt * kRows<NH> + in_tile;
+    if (n <= 0 || m >= static_cast<uint32_t>(n) * G) {
+        return;
+    }
+    const int4 meta = p.meta[id];
+    const uint32_t segments = static_cast<uint32_t>(meta.x);
+    if (segments == 0) {
+        return;
+    }
+    const uint32_t c0 = static_cast<uint32_t>(meta.y), first = static_cast<uint32_t>(meta.z), col = (threadIdx.x % 16) * 8;
+    const uint64_t group0 = static_cast<uint64_t>(kvh / NH) * p.slots;
+    auto row_of = [&](uint32_t s) {
+        const uint64_t slot = group0 + (s == 0 ? 2 * c0 + (1 - first) : 2 * (c0 + s));
+        return (slot * NH + kvh % NH) * kRows<NH> + in_tile;
+    };
+    float m_all = -INFINITY, l = 0.f, o[8] = {};
+    for (uint32_t i0 = 0; i0 < segments; i0 += 4) {
+        float2 ml[4];
+        float4 x[4][2];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {   // (all loads on their way; past the end: the last one again, weighted zero)
+            const uint64_t row = row_of(min(i0 + u, segments - 1));
+            ml[u] = *reinterpret_cast<const float2 *>(p.ml + row * 2);
+            x[u][0] = *reinterpret_cast<const float4 *>(p.acc + row * D + col);
+            x[u][1] = *reinterpret_cast<const float4 *>(p.acc + row * D + col + 4);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const bool in = i0 + u < segments;
+            const float m_new = in ? fmaxf(m_all, ml[u].x) : m_all;
+            const float safe = m_new == -INFINITY ? 0.f : m_new;
+            const float wa = fast_exp2(m_all - safe), wb = fast_exp2(ml[u].x - safe);
+            if (in) {
+                const float *f = reinterpret_cast<const float *>(&x[u][0]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    o[e] = o[e] * wa + (wb != 0.f ? f[e] * wb : 0.f);   // (a part of weight zero that saw nothing holds zeros)
+                }
+                l = l * wa + ml[u].y * wb;
+                m_all = m_new;
+            }
+        }
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const float scale = l != l ? l : inv;
+    uint4 w;
+    w.x = T::pack(o[0] * scale, o[1] * scale);
+    w.y = T::pack(o[2] * scale, o[3] * scale);
+    w.z = T::pack(o[4] * scale, o[5] * scale);
+    w.w = T::pack(o[6] * scale, o[7] * scale);
+    *reinterpret_cast<uint4 *>(p.out + (static_cast<uint64_t>(start + m / G) * p.n_heads + kvh * G + m % G) * D + col) = w;
+}
+
+// The kv heads of a workgroup: as many as divide the model's and leave it the rows of a typical M tile (twice the average of
+// the batch, no more than the mask has nodes for).
+uint32_t heads_of(uint32_t total_tokens, uint32_t group, uint32_t n_kv_heads, uint32_t batch, uint32_t mask_words)
+{
+    const uint64_t rows = std::min<uint64_t>(2ull * total_tokens / batch, 32ull * mask_words) * group;
+    return n_kv_heads % 2 == 0 && rows < 2 * kRows<2> ? 2u : 1u;
+}
+
+struct StreamPlan {
+    uint32_t nh, groups, tiles, slots;
+    size_t bytes;
+};
+StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t batch, uint32_t block_size, uint32_t max_num_block,
+                   uint32_t nh)
+{
+    StreamPlan s;
+    const uint32_t G = n_heads / n_kv_heads, rows = 32 * kWaves / nh;
+    s.nh = nh;
+    s.groups = n_kv_heads / nh;
+    s.tiles = static_cast<uint32_t>(static_cast<uint64_t>(total_tokens) * G / rows) + batch;
+    // chunks: one per workgroup, more when a chunk's blocks would not fit the table
+    const uint64_t sp = kHalf / 256 / nh, per = std::max<uint64_t>(1, (kTblCap - 2) * static_cast<uint64_t>(block_size) / sp);
+    const uint64_t steps = s.tiles * ((static_cast<uint64_t>(max_num_block) * block_size + sp - 1) / sp);
+    s.slots = static_cast<uint32_t>(2 * std::max<uint64_t>(std::max(1u, kComputeUnits / s.groups), steps / per + 1));
+    s.bytes = s.tiles * sizeof(int4) + static_cast<size_t>(s.groups) * s.slots * nh * rows * (D + 2) * sizeof(float);
+    return s;
+}
+
+}  // namespace
+
+// head_dim 128, 16-bit caches; a copy's positions share a block; every block that a step can reach has its table entry in LDS
+bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
+                           uint32_t max_num_block, int kv_dtype)
+{
+    return head_dim == D && kv_dtype == XLITE_HIP_KV_SAME && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && block_size % 4 == 0 &&
+           batch <= kSeqCap && static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32);
+}
+
+size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t batch, uint32_t block_size,
+                                   uint32_t max_num_block)
+{
+    size_t need = 0;   // whatever heads_of will say
+    for (uint32_t nh : {1u, 2u}) {
+        if (n_kv_heads % nh == 0) {
+            need = std::max(need, plan_of(total_tokens, n_heads, n_kv_heads, batch, block_size, max_num_block, nh).bytes);
+        }
+    }
+    return need;
+}
+
+int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
+{
+    const StreamPlan plan = plan_of(a.total_tokens, a.n_heads, a.n_kv_heads, a.batch, a.block_size, a.max_num_block,
+                                    heads_of(a.total_tokens, a.n_heads / a.n_kv_heads, a.n_kv_heads, a.batch, a.mask_words));
+    if (a.workspace == nullptr || a.workspace_bytes < plan.bytes) {
+        return fail(XLITE_HIP_ENOSPC, __func__, "workspace too small: need " + std::to_string(plan.bytes) + " bytes, have " +
+                                                    std::to_string(a.workspace == nullptr ? 0 : a.workspace_bytes));
+    }
+    StreamParams p{};
+    p.q = static_cast<const uint16_t *>(a.qkv);
+    p.k_cache = static_cast<const uint16_t *>(a.k_cache);
+    p.v_cache = static_cast<const uint16_t *>(a.v_cache);
+    p.out = static_cast<uint16_t *>(a.output);
+    p.tree_mask = a.tree_mask;
+    p.query_start_loc = a.query_start_loc;
+    p.lens = a.lens;
+    p.cached_lens = a.cached_lens;
+    p.block_tables = a.block_tables;
+    p.q_tok_stride = (a.n_heads + 2 * a.n_kv_heads) * D;
+    p.n_heads = a.n_heads;
+    p.n_kv_heads = a.n_kv_heads;
+    p.group = a.n_heads / a.n_kv_heads;
+    p.batch = a.batch;
+    p.block_size = a.block_size;
+    p.block_magic = static_cast<uint32_t>((1ull << 32) / a.block_size) + 1;
+    p.max_num_block = a.max_num_block;
+    p.mask_words = a.mask_words;
+    p.slots = plan.slots;
+    p.meta = static_cast<int4 *>(a.workspace);
+    p.acc = reinterpret_cast<float *>(p.meta + plan.tiles);
+    p.ml = p.acc + static_cast<uint64_t>(plan.groups) * plan.slots * 32 * kWaves * D;
+    const size_t lds = kStages * kStage + (kTblCap + a.batch + 1) * sizeof(uint32_t);
+    const dim3 grid(std::max(1u, kComputeUnits / plan.groups), plan.groups), merge_grid(plan.tiles, a.n_kv_heads, 32 * kWaves / plan.nh / 16);
+    auto launch = [&](auto t, auto n) -> int {
+        using T = decltype(t);
+        constexpr int NH = decltype(n)::value;
+        auto kernel = tree_stream_kernel<T, NH>;
+        if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds)) {
+            return rc;
+        }
+        kernel<<<grid, kThreads, lds, stream>>>(p);
+        XL_LAUNCH_CHECK();
+        tree_merge_kernel<T, NH><<<merge_grid, 256, 0, stream>>>(p);
+        XL_LAUNCH_CHECK();
+        return XLITE_HIP_OK;
+    };
+    auto with_heads = [&](auto t) -> int {
+        return plan.nh == 2 ? launch(t, std::integral_constant<int, 2>{}) : launch(t, std::integral_constant<int, 1>{});
+    };
+    return a.dtype == XLITE_HIP_BF16 ? with_heads(BF16{}) : with_heads(FP16{});
+}
+
+}  // namespace xlite
