@@ -37,6 +37,7 @@ constexpr uint32_t kRows = 32 * kWaves / NH;     // M rows of a workgroup, per k
 constexpr uint32_t kStage = 2 * kHalf;
 constexpr uint32_t kTblCap = 2048;               // block-table entries staged per segment
 constexpr uint32_t kSeqCap = 1024;               // sequences whose prefix sums fit
+constexpr uint32_t kMaskCap = kThreads;          // mask words of an M tile kept in LDS: 128 rows of 4 heads and 512 nodes
 constexpr uint32_t kMinChunk = 4;                // steps
 constexpr uint32_t kComputeUnits = 256;
 
@@ -94,24 +95,42 @@ tree_stream_kernel(const StreamParams p)
     constexpr int CPW = 2;                       // copies per wave, step and tensor
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     uint32_t *tbl = reinterpret_cast<uint32_t *>(smem + kStages * kStage);
-    uint32_t *pref = tbl + kTblCap;              // batch + 1 words
+    uint32_t *mask_lds = tbl + kTblCap;
+    uint32_t *pref = mask_lds + kMaskCap;        // batch + 1 words
     const uint32_t smem_addr = stage::lds_address(smem);
     const uint32_t lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const uint32_t G = p.group;
     const uint32_t hsel = wave % NH, row_tile = wave / NH;
     const uint32_t kvh = blockIdx.y * NH + hsel;
 
-    // ---- steps of every sequence, summed: thread t owns consecutive sequences
-    auto weight = [&](uint32_t i) {
-        const int32_t n = p.lens[i], c = p.cached_lens[i];
+    // ---- steps of every sequence, summed. Up to 64 sequences: lane i of every wave holds what the batch says about sequence
+    // i (one round of loads, nothing through LDS); more: thread t owns consecutive sequences and the sums go to LDS.
+    auto weight = [&](int32_t n, int32_t c) {
         return n <= 0 ? 0u : ceil_div(static_cast<uint32_t>(c + n), SP) * ceil_div(static_cast<uint32_t>(n) * G, ROWS);
     };
-    {
+    const bool in_lanes = p.batch <= 64;
+    int32_t ln_len = 0, ln_cached = 0, ln_start = 0;
+    uint32_t ln_pref = 0, total;
+    if (in_lanes) {
+        const uint32_t i = min(lane, p.batch - 1);
+        ln_len = p.lens[i];
+        ln_cached = p.cached_lens[i];
+        ln_start = p.query_start_loc[i];
+        uint32_t incl = lane < p.batch ? weight(ln_len, ln_cached) : 0u;
+        const uint32_t mine = incl;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(incl, d);
+            incl += lane >= static_cast<uint32_t>(d) ? up : 0u;
+        }
+        ln_pref = incl - mine;   // (lanes past the batch: the sum of everything)
+        total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(incl), 63));
+    } else {
         const uint32_t per = ceil_div(p.batch, static_cast<uint32_t>(kThreads));
         const uint32_t i0 = min(p.batch, threadIdx.x * per), i1 = min(p.batch, i0 + per);
         uint32_t mine = 0;
         for (uint32_t i = i0; i < i1; i++) {
-            mine += weight(i);
+            mine += weight(p.lens[i], p.cached_lens[i]);
         }
         uint32_t incl = mine;
 #pragma unroll
@@ -129,14 +148,17 @@ tree_stream_kernel(const StreamParams p)
         }
         for (uint32_t i = i0; i < i1; i++) {
             pref[i] = run;
-            run += weight(i);
+            run += weight(p.lens[i], p.cached_lens[i]);
         }
         if (threadIdx.x == kThreads - 1) {
             pref[p.batch] = run;
         }
         __syncthreads();
+        total = uni(pref[p.batch]);
     }
-    const uint32_t total = uni(pref[p.batch]);
+    auto steps_before = [&](uint32_t i) {   // sequence i; i == batch: all of them
+        return in_lanes ? (i < 64 ? static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ln_pref), static_cast<int>(i))) : total) : uni(pref[i]);
+    };
     uint32_t chunk = max(ceil_div(total, gridDim.x), kMinChunk);
     chunk = min(chunk, (kTblCap - 2) * p.block_size / SP);
     const uint32_t n_chunks = ceil_div(total, chunk);
@@ -157,7 +179,9 @@ tree_stream_kernel(const StreamParams p)
         const uint32_t c_begin = c * chunk, c_end = min(total, c_begin + chunk);
         uint32_t at = c_begin;
         uint32_t seq = 0;   // the last sequence whose first step is at or before `at`
-        {
+        if (in_lanes) {
+            seq = static_cast<uint32_t>(__builtin_popcountll(__ballot(lane < p.batch && ln_pref <= at))) - 1;
+        } else {
             uint32_t hi = p.batch;
             while (hi - seq > 1) {
                 const uint32_t mid = (seq + hi) >> 1;
@@ -169,14 +193,17 @@ tree_stream_kernel(const StreamParams p)
             }
         }
         while (at < c_end) {
-            const uint32_t first = uni(pref[seq]), next = uni(pref[seq + 1]);
+            seq = uni(seq);
+            const uint32_t first = steps_before(seq), next = steps_before(seq + 1);
             if (next == first) {   // no rows
                 seq++;
                 continue;
             }
             // ---- the segment: steps a .. b - 1 of M tile mt
-            const uint32_t nodes = uni(static_cast<uint32_t>(p.lens[seq])), cached = uni(static_cast<uint32_t>(p.cached_lens[seq]));
-            const uint32_t start = uni(static_cast<uint32_t>(p.query_start_loc[seq]));
+            const int32_t at_lane = static_cast<int>(min(seq, 63u));
+            const uint32_t nodes = uni(static_cast<uint32_t>(in_lanes ? __builtin_amdgcn_readlane(ln_len, at_lane) : p.lens[seq]));
+            const uint32_t cached = uni(static_cast<uint32_t>(in_lanes ? __builtin_amdgcn_readlane(ln_cached, at_lane) : p.cached_lens[seq]));
+            const uint32_t start = uni(static_cast<uint32_t>(in_lanes ? __builtin_amdgcn_readlane(ln_start, at_lane) : p.query_start_loc[seq]));
             const uint32_t range = cached + nodes, steps = ceil_div(range, SP);
             const uint32_t mt = (at - first) / steps, a = (at - first) - mt * steps, b = min(steps, a + (c_end - at));
             const uint32_t tile_first = first + mt * steps;      // of the M tile, in all steps
@@ -194,14 +221,30 @@ tree_stream_kernel(const StreamParams p)
 
             // ---- set-up: block-table entries, then the query rows, then the first two steps' copies
             __syncthreads();   // (the table and the stages of the last segment have been read)
-            for (uint32_t i = threadIdx.x; i <= blk1 - blk0; i += kThreads) {
-                tbl[i] = static_cast<uint32_t>(table[blk0 + i]);
-            }
+            const uint32_t n_blk = blk1 - blk0 + 1;
+            // the mask's rows of the M tile, for a segment that reaches into the tree
+            const uint32_t tok_first = mt * ROWS / G;                   // (inside the sequence)
+            const uint32_t tok_count = (min(mt * ROWS + ROWS, m_rows) - 1) / G - tok_first + 1;
+            const uint32_t n_words = tok_count * p.mask_words;
+            const bool words_in_lds = n_words <= kMaskCap;
+            const uint32_t *words_src = p.tree_mask + static_cast<uint64_t>(start + tok_first) * p.mask_words;
+            const uint32_t word = words_src[words_in_lds ? min(threadIdx.x, n_words - 1) : 0u];
+            const uint32_t entry = static_cast<uint32_t>(table[blk0 + min(threadIdx.x, n_blk - 1)]);
             uint4 qreg[KS];
             const uint16_t *src = p.q + tok * p.q_tok_stride + static_cast<uint64_t>(head) * D;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 qreg[ks] = *reinterpret_cast<const uint4 *>(src + ks * 16 + half * 8);
+            }
+            // (this wait leaves the query rows on their way)
+            if (words_in_lds && threadIdx.x < n_words) {
+                mask_lds[threadIdx.x] = word;
+            }
+            if (threadIdx.x < n_blk) {
+                tbl[threadIdx.x] = entry;
+            }
+            for (uint32_t i = threadIdx.x + kThreads; i < n_blk; i += kThreads) {
+                tbl[i] = static_cast<uint32_t>(table[blk0 + i]);
             }
             if (a == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
                 const uint32_t n = whole ? 0u : (tile_first + steps - 1) / chunk - c + 1;
@@ -215,11 +258,6 @@ tree_stream_kernel(const StreamParams p)
                 for (int k = 0; k < 16; k++) {
                     O[dt][k] = 0.f;
                 }
-            }
-            // complete these loads before any copy is issued: memory answers in order
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                asm volatile("" : "+v"(qreg[ks].x), "+v"(qreg[ks].y), "+v"(qreg[ks].z), "+v"(qreg[ks].w));
             }
             __syncthreads();
             // copies of step `s` (from t0) into stage s % 4. Positions at or beyond t1 re-read the last one (their scores are
@@ -268,10 +306,16 @@ tree_stream_kernel(const StreamParams p)
                 }
             };
 
+            // which of the positions j0 .. j0 + 31 the lane's row sees, moved so that bit 8 (k / 4) + k % 4 is that of register k
+            auto seen_from = [&](uint32_t j0) __attribute__((always_inline)) {
+                const uint32_t *words = words_in_lds ? mask_lds + (m / G - tok_first) * p.mask_words : p.tree_mask + tok * p.mask_words;
+                return (tree_seen(words, p.mask_words, j0, cached, nodes) & ones(static_cast<int32_t>(t1 - j0))) >> (4 * half);
+            };
+            bool poisoned = false;
             // 32 positions of a step: those from 32 h on. Register k of S holds position j0 + 8 (k / 4) + 4 half + k % 4.
-            auto compute = [&](uint32_t s, uint32_t h, auto mask_tag) __attribute__((always_inline)) {
-                constexpr bool MASK = decltype(mask_tag)::value;
+            auto compute = [&](uint32_t s, uint32_t h) __attribute__((always_inline)) {
                 const uint32_t j0 = t0 + s * SP + 32 * h;
+                const bool masked = j0 + 32 > cached;   // (positions below the cached length are seen by every row)
                 const unsigned char *st = smem + (s % kStages) * kStage + h * 32 * POSB;
                 uint4 kop[KS];
 #pragma unroll
@@ -304,13 +348,34 @@ tree_stream_kernel(const StreamParams p)
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                [[maybe_unused]] uint32_t seen = 0;
-                if constexpr (MASK) {
-                    seen = tree_seen(p.tree_mask + tok * p.mask_words, p.mask_words, j0, cached, nodes) & ones(static_cast<int32_t>(t1 - j0));
-                    seen >>= 4 * half;
+                if (masked) {
+                    uint32_t seen = seen_from(j0);
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
                         S[k] = (seen >> ((k / 4) * 8 + (k % 4))) & 1u ? S[k] : -INFINITY;
+                    }
+                    // A row that does not see a position has probability zero there, and zero times an infinity or a NaN in
+                    // that position's V row would still poison it. Such values leave the operands; the rows that see them
+                    // get them back behind the loop.
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) {
+                            odd |= not_finite2<T>(vop[kk][dt].x) | not_finite2<T>(vop[kk][dt].y) | not_finite2<T>(vop[kk][dt].z) |
+                                   not_finite2<T>(vop[kk][dt].w);
+                        }
+                    }
+                    if (__any(odd)) {
+                        poisoned = true;
+#pragma unroll
+                        for (int kk = 0; kk < 2; kk++) {
+#pragma unroll
+                            for (int dt = 0; dt < DT; dt++) {
+                                vop[kk][dt] = make_uint4(finite_only<T>(vop[kk][dt].x), finite_only<T>(vop[kk][dt].y),
+                                                         finite_only<T>(vop[kk][dt].z), finite_only<T>(vop[kk][dt].w));
+                            }
+                        }
                     }
                 }
                 float mx = -INFINITY;
@@ -349,52 +414,6 @@ tree_stream_kernel(const StreamParams p)
                         }
                     }
                 }
-                if constexpr (MASK) {
-                    // infinities and NaNs in V rows that some rows do not see (as in the prefill kernel)
-                    uint32_t odd = 0;
-#pragma unroll
-                    for (int kk = 0; kk < 2; kk++) {
-#pragma unroll
-                        for (int dt = 0; dt < DT; dt++) {
-                            odd |= not_finite2<T>(vop[kk][dt].x) | not_finite2<T>(vop[kk][dt].y) | not_finite2<T>(vop[kk][dt].z) |
-                                   not_finite2<T>(vop[kk][dt].w);
-                        }
-                    }
-                    if (__any(odd)) {
-                        uint32_t sw[8];
-#pragma unroll
-                        for (int k = 0; k < 16; k += 2) {
-                            sw[k / 2] = T::pack((seen >> ((k / 4) * 8 + (k % 4))) & 1u ? 1.f : 0.f,
-                                                (seen >> (((k + 1) / 4) * 8 + ((k + 1) % 4))) & 1u ? 1.f : 0.f);
-                        }
-                        const uint4 sb[2] = {make_uint4(sw[0], sw[1], sw[2], sw[3]), make_uint4(sw[4], sw[5], sw[6], sw[7])};
-#pragma unroll
-                        for (int dt = 0; dt < DT; dt++) {
-#pragma unroll
-                            for (int what = 0; what < 3; what++) {
-                                f32x16_t hit;
-#pragma unroll
-                                for (int k = 0; k < 16; k++) {
-                                    hit[k] = 0.f;
-                                }
-#pragma unroll
-                                for (int kk = 0; kk < 2; kk++) {
-                                    hit = mfma32<T>(odd_values<T>(make_uint2(vop[kk][dt].x, vop[kk][dt].y), make_uint2(vop[kk][dt].z, vop[kk][dt].w), what),
-                                                    sb[kk], hit);
-                                }
-#pragma unroll
-                                for (int k = 0; k < 16; k++) {
-                                    O[dt][k] += hit[k] > 0.f ? (what == 0 ? INFINITY : what == 1 ? -INFINITY : NAN) : 0.f;
-                                }
-                            }
-#pragma unroll
-                            for (int kk = 0; kk < 2; kk++) {
-                                vop[kk][dt] = make_uint4(finite_only<T>(vop[kk][dt].x), finite_only<T>(vop[kk][dt].y),
-                                                         finite_only<T>(vop[kk][dt].z), finite_only<T>(vop[kk][dt].w));
-                            }
-                        }
-                    }
-                }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int kk = 0; kk < 2; kk++) {
@@ -406,8 +425,6 @@ tree_stream_kernel(const StreamParams p)
             };
 
             const uint32_t n_steps = b - a, last = n_steps - 1;
-            // steps wholly below the cached length are seen by every row
-            const uint32_t plain = min(n_steps, cached > t0 ? (cached - t0) / SP : 0u);
             issue(0);
             if (last >= 1) {
                 issue(1);
@@ -415,7 +432,12 @@ tree_stream_kernel(const StreamParams p)
             if (last >= 2) {
                 issue(2);
             }
-            auto turn = [&](uint32_t s, auto mask_tag) __attribute__((always_inline)) {
+            // (the query rows were requested before the copies; their wait is for both)
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                asm volatile("" : "+v"(qreg[ks].x), "+v"(qreg[ks].y), "+v"(qreg[ks].z), "+v"(qreg[ks].w));
+            }
+            for (uint32_t s = 0; s < n_steps; s++) {
                 // this wave's share of step s has landed: only those of the next two are out
                 if (s + 2 <= last) {
                     stage::wait<4 * CPW>();
@@ -431,18 +453,27 @@ tree_stream_kernel(const StreamParams p)
                 if (has_rows) {    // (a wave without rows only copies)
 #pragma unroll 1
                     for (uint32_t h = 0; h < SP / 32; h++) {
-                        compute(s, h, mask_tag);
+                        compute(s, h);
                     }
                 }
-            };
-            uint32_t s = 0;
-            for (; s < plain; s++) {
-                turn(s, std::integral_constant<bool, false>{});
             }
-            for (; s < n_steps; s++) {
-                turn(s, std::integral_constant<bool, true>{});
+            if (poisoned) {   // (rare, and not fast: the tree's V rows are read again, value by value)
+                for (uint32_t j = max(t0, cached); j < t1; j++) {
+                    const uint32_t blk = j / p.block_size;
+                    const uint64_t row = static_cast<uint64_t>(static_cast<uint32_t>(table[blk])) * p.block_size + (j - blk * p.block_size);
+                    const uint16_t *v = p.v_cache + (row * p.n_kv_heads + kvh) * D + 4 * half;
+                    const bool see = tree_seen(p.tree_mask + tok * p.mask_words, p.mask_words, j, cached, nodes) & 1u;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            const uint32_t bits = v[dt * 32 + (k / 4) * 8 + (k % 4)];
+                            const float x = T::to_f32(static_cast<uint16_t>(bits));
+                            O[dt][k] += see && not_finite2<T>(bits) ? x : 0.f;
+                        }
+                    }
+                }
             }
-
             // ---- results. O^T lane layout: column = M row, register k of tile dt = element 32 dt + 8 (k / 4) + 4 half + k % 4
             const float l_tot = l_run + __shfl_xor(l_run, 32);
             if (m_first + col < m_rows) {
@@ -462,18 +493,18 @@ tree_stream_kernel(const StreamParams p)
                     }
                 } else {
                     const uint64_t slot = static_cast<uint64_t>(blockIdx.y) * p.slots + 2 * c + (first_seg ? 0u : 1u);
-                    const uint64_t row = (slot * NH + hsel) * ROWS + row_tile * 32 + col;
-                    float *dst = p.acc + row * D;
+                    // as the registers lie: 16 pieces of 1 KiB per 32 rows, piece 4 dt + kg lane by lane
+                    const uint64_t tile = (slot * NH + hsel) * (ROWS / 32) + row_tile;
+                    float4 *dst = reinterpret_cast<float4 *>(p.acc + tile * 32 * D) + lane;
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
                         for (int kg = 0; kg < 4; kg++) {
-                            *reinterpret_cast<float4 *>(dst + dt * 32 + kg * 8 + half * 4) =
-                                make_float4(O[dt][kg * 4], O[dt][kg * 4 + 1], O[dt][kg * 4 + 2], O[dt][kg * 4 + 3]);
+                            dst[(dt * 4 + kg) * 64] = make_float4(O[dt][kg * 4], O[dt][kg * 4 + 1], O[dt][kg * 4 + 2], O[dt][kg * 4 + 3]);
                         }
                     }
                     if (half == 0) {
-                        *reinterpret_cast<float2 *>(p.ml + row * 2) = make_float2(m_run * kLog2e, l_tot);
+                        *reinterpret_cast<float2 *>(p.ml + (tile * 32 + col) * 2) = make_float2(m_run * kLog2e, l_tot);
                     }
                 }
             }
@@ -485,14 +516,24 @@ tree_stream_kernel(const StreamParams p)
     }
 }
 
-// Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), 16 threads of 8 columns per row.
+// Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), 16 threads of 8 columns (a piece of the stored layout) per row.
 template <typename T, int NH>
 __global__ void __launch_bounds__(256)
 tree_merge_kernel(const StreamParams p)
 {
     const uint32_t id = blockIdx.x, kvh = blockIdx.y, G = p.group;
     uint32_t seq = 0;   // the last sequence whose ids start at or before `id`
-    {
+    int32_t n;
+    uint32_t start;
+    const int4 meta = p.meta[id];
+    if (p.batch <= 64) {   // one round of loads
+        const uint32_t lane = threadIdx.x & 63, i = min(lane, p.batch - 1);
+        const int32_t ln_start = p.query_start_loc[i], ln_len = p.lens[i];
+        const uint64_t started = __ballot(lane < p.batch && first_id<NH>(p, static_cast<uint32_t>(ln_start), lane) <= id);
+        seq = static_cast<uint32_t>(max(__builtin_popcountll(started) - 1, 0));
+        n = __shfl(ln_len, static_cast<int>(seq));
+        start = static_cast<uint32_t>(__shfl(ln_start, static_cast<int>(seq)));
+    } else {
         uint32_t hi = p.batch;
         while (hi - seq > 1) {
             const uint32_t mid = (seq + hi) >> 1;
@@ -502,20 +543,19 @@ tree_merge_kernel(const StreamParams p)
                 hi = mid;
             }
         }
+        n = p.lens[seq];
+        start = static_cast<uint32_t>(p.query_start_loc[seq]);
     }
-    const int32_t n = p.lens[seq];
-    const uint32_t start = static_cast<uint32_t>(p.query_start_loc[seq]);
     const uint32_t mt = id - first_id<NH>(p, start, seq);
-    const uint32_t in_tile = blockIdx.z * 16 + threadIdx.x / 16, m = mt * kRows<NH> + in_tile;
+    const uint32_t in_tile = blockIdx.z * 16 + threadIdx.x % 16, m = mt * kRows<NH> + in_tile;
     if (n <= 0 || m >= static_cast<uint32_t>(n) * G) {
         return;
     }
-    const int4 meta = p.meta[id];
     const uint32_t segments = static_cast<uint32_t>(meta.x);
     if (segments == 0) {
         return;
     }
-    const uint32_t c0 = static_cast<uint32_t>(meta.y), first = static_cast<uint32_t>(meta.z), col = (threadIdx.x % 16) * 8;
+    const uint32_t c0 = static_cast<uint32_t>(meta.y), first = static_cast<uint32_t>(meta.z), piece = threadIdx.x / 16;
     const uint64_t group0 = static_cast<uint64_t>(kvh / NH) * p.slots;
     auto row_of = [&](uint32_t s) {
         const uint64_t slot = group0 + (s == 0 ? 2 * c0 + (1 - first) : 2 * (c0 + s));
@@ -529,8 +569,9 @@ tree_merge_kernel(const StreamParams p)
         for (int u = 0; u < 4; u++) {   // (all loads on their way; past the end: the last one again, weighted zero)
             const uint64_t row = row_of(min(i0 + u, segments - 1));
             ml[u] = *reinterpret_cast<const float2 *>(p.ml + row * 2);
-            x[u][0] = *reinterpret_cast<const float4 *>(p.acc + row * D + col);
-            x[u][1] = *reinterpret_cast<const float4 *>(p.acc + row * D + col + 4);
+            const float4 *src = reinterpret_cast<const float4 *>(p.acc + (row & ~31ull) * D) + piece * 64 + (row & 31);
+            x[u][0] = src[0];    // columns 8 piece .. + 3
+            x[u][1] = src[32];   // columns 8 piece + 4 .. + 7
         }
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -556,7 +597,7 @@ tree_merge_kernel(const StreamParams p)
     w.y = T::pack(o[2] * scale, o[3] * scale);
     w.z = T::pack(o[4] * scale, o[5] * scale);
     w.w = T::pack(o[6] * scale, o[7] * scale);
-    *reinterpret_cast<uint4 *>(p.out + (static_cast<uint64_t>(start + m / G) * p.n_heads + kvh * G + m % G) * D + col) = w;
+    *reinterpret_cast<uint4 *>(p.out + (static_cast<uint64_t>(start + m / G) * p.n_heads + kvh * G + m % G) * D + piece * 8) = w;
 }
 
 // The kv heads of a workgroup: as many as divide the model's and leave it the rows of a typical M tile (twice the average of
@@ -640,7 +681,7 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     p.meta = static_cast<int4 *>(a.workspace);
     p.acc = reinterpret_cast<float *>(p.meta + plan.tiles);
     p.ml = p.acc + static_cast<uint64_t>(plan.groups) * plan.slots * 32 * kWaves * D;
-    const size_t lds = kStages * kStage + (kTblCap + a.batch + 1) * sizeof(uint32_t);
+    const size_t lds = kStages * kStage + (kTblCap + kMaskCap + a.batch + 1) * sizeof(uint32_t);
     const dim3 grid(std::max(1u, kComputeUnits / plan.groups), plan.groups), merge_grid(plan.tiles, a.n_kv_heads, 32 * kWaves / plan.nh / 16);
     auto launch = [&](auto t, auto n) -> int {
         using T = decltype(t);
