@@ -16,9 +16,12 @@ namespace {
 // does not depend on any order. One workgroup per (sequence, kv head); the keys are read once, into registers.
 // A weight's neighbours in memory belong to the other kv heads: the heads of a sequence run on one XCD, at the same time, so
 // that its lines come from memory once and from that XCD's L2 for the other heads.
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / 64;
+// Measured, 64 sequences x 8 heads, an eighth kept: 15 us over 4000 positions, 34 over 16000, 61 over 32000, 118 over 64000;
+// one sequence of 32000 37 us. The weights of 64 x 32768 positions are 67 MB, 13 us at the rate of a copy: what bounds it is the
+// chain of a workgroup's steps (loads through the block table 12 us, three histograms 10, ballots 3, output 4) and that only
+// two workgroups' keys fit a compute unit, so that little of one list's chain hides behind another's.
 constexpr uint32_t kXcds = 8;
+constexpr int kAhead = 16;   // loads a thread has under way
 
 // weights in the order of a descending sort: NaN first, -0 and +0 alike; never 0, which stands for "no weight"
 __device__ __forceinline__ uint32_t weight_key(float w)
@@ -44,13 +47,14 @@ struct SelectParams {
 // exponent and two bits of the mantissa, so that few lanes of a wave meet in one bin (with 8 bits a dozen did, and the
 // first pass took longer than the rest of the kernel together).
 constexpr int kHistCopies = 4;
+template <int T>
 struct SelectScratch {
     uint32_t hist[kHistCopies][2048];
-    uint32_t wave_sum[kSelWaves];
+    uint32_t wave_sum[T / 64];
     uint32_t found[2];   // the digit, and how many keys lie in the bins above it
 };
-template <typename EACH>
-__device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScratch &s, uint32_t *threshold, uint32_t *equal)
+template <int T, typename EACH>
+__device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScratch<T> &s, uint32_t *threshold, uint32_t *equal)
 {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t *mine = s.hist[wave % kHistCopies];
@@ -60,8 +64,8 @@ __device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScrat
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t bits = pass == 2 ? 10u : 11u;
 #pragma unroll
-        for (int i = 0; i < kHistCopies * 2048 / kSelThreads; i++) {
-            (&s.hist[0][0])[threadIdx.x + i * kSelThreads] = 0;
+        for (int i = 0; i < kHistCopies * 2048 / T; i++) {
+            (&s.hist[0][0])[threadIdx.x + i * T] = 0;
         }
         __syncthreads();
         each([&](uint32_t k) {
@@ -70,14 +74,21 @@ __device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScrat
             }
         });
         __syncthreads();
-        // thread t: bins 2047 - 2 t and 2046 - 2 t, in descending order
-        uint32_t c[2] = {0, 0};
+        // thread t: bins 2047 - P t, 2046 - P t, ..., in descending order
+        constexpr int P = 2048 / T;
+        uint32_t c[P] = {}, sum = 0;
 #pragma unroll
         for (int h = 0; h < kHistCopies; h++) {
-            c[0] += s.hist[h][2047 - 2 * threadIdx.x];
-            c[1] += s.hist[h][2046 - 2 * threadIdx.x];
+#pragma unroll
+            for (int e = 0; e < P; e++) {
+                c[e] += s.hist[h][2047 - P * threadIdx.x - e];
+            }
         }
-        uint32_t incl = c[0] + c[1];
+#pragma unroll
+        for (int e = 0; e < P; e++) {
+            sum += c[e];
+        }
+        uint32_t incl = sum;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(incl, d);
@@ -87,15 +98,15 @@ __device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScrat
             s.wave_sum[wave] = incl;
         }
         __syncthreads();
-        uint32_t above = incl - c[0] - c[1];
+        uint32_t above = incl - sum;
 #pragma unroll
-        for (uint32_t w = 0; w < kSelWaves; w++) {
+        for (uint32_t w = 0; w < (T / 64); w++) {
             above += w < wave ? s.wave_sum[w] : 0u;
         }
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < P; e++) {
             if (above < left && left <= above + c[e]) {   // exactly one bin of one thread
-                s.found[0] = 2047 - 2 * threadIdx.x - e;
+                s.found[0] = 2047 - P * threadIdx.x - e;
                 s.found[1] = above;
             }
             above += c[e];
@@ -108,14 +119,14 @@ __device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScrat
     *equal = left;
 }
 
-// KPT: keys a thread holds in registers (the context fits KPT * 1024 positions); 0: any length, the keys are read again in
-// every pass
-template <int KPT>
-__global__ void __launch_bounds__(kSelThreads)
+// T threads. KPT: keys a thread holds in registers (the judged positions fit KPT * T); 0: any length, the keys are read again
+// in every pass
+template <int KPT, int T>
+__global__ void __launch_bounds__(T, KPT == 64 ? 4 : 1)
 select_kept_kernel(const SelectParams p)
 {
-    __shared__ SelectScratch scratch;
-    __shared__ uint2 counts[(KPT > 0 ? KPT : 1) * kSelWaves];   // (above, equal) of a wave's 64 positions, then the sums before them
+    __shared__ SelectScratch<T> scratch;
+    __shared__ uint2 counts[(KPT > 0 ? KPT : kAhead) * (T / 64)];   // (above, equal) of a wave's 64 positions, then the sums before them
     const uint32_t xcd = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
     const uint32_t seq = place / p.n_kv_heads * kXcds + xcd, kvh = place % p.n_kv_heads;
     if (seq >= p.batch) {
@@ -128,11 +139,11 @@ select_kept_kernel(const SelectParams p)
     if (kvh == 0 && threadIdx.x == 0) {
         p.kept_lens[seq] = static_cast<int32_t>(count);
     }
-    for (uint32_t i = count + threadIdx.x; i < p.budget; i += kSelThreads) {
+    for (uint32_t i = count + threadIdx.x; i < p.budget; i += T) {
         out[i] = -1;
     }
     if (length <= p.budget) {
-        for (uint32_t i = threadIdx.x; i < length; i += kSelThreads) {
+        for (uint32_t i = threadIdx.x; i < length; i += T) {
             out[i] = static_cast<int32_t>(i);
         }
         return;
@@ -145,10 +156,10 @@ select_kept_kernel(const SelectParams p)
     };
     const uint32_t lo = p.sink, hi = length - p.recent;   // the judged positions
     const uint32_t n = p.budget - p.sink - p.recent;      // fewer than hi - lo: length > budget
-    for (uint32_t i = threadIdx.x; i < p.sink; i += kSelThreads) {
+    for (uint32_t i = threadIdx.x; i < p.sink; i += T) {
         out[i] = static_cast<int32_t>(i);
     }
-    for (uint32_t i = threadIdx.x; i < p.recent; i += kSelThreads) {
+    for (uint32_t i = threadIdx.x; i < p.recent; i += T) {
         out[p.sink + n + i] = static_cast<int32_t>(hi + i);
     }
     if (n == 0) {
@@ -160,11 +171,15 @@ select_kept_kernel(const SelectParams p)
         uint32_t key[KPT];
 #pragma unroll
         for (int j = 0; j < KPT; j++) {
-            const uint32_t i = lo + j * kSelThreads + threadIdx.x;
+            const uint32_t i = lo + j * T + threadIdx.x;
             key[j] = key_at(min(i, hi - 1));
             key[j] = i < hi ? key[j] : 0u;
+            if (j % kAhead == kAhead - 1) {   // with all of them under way their addresses would take the keys' registers
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("" ::: "memory");
+            }
         }
-        nth_largest([&](auto &&f) {
+        nth_largest<T>([&](auto &&f) {
 #pragma unroll
             for (int j = 0; j < KPT; j++) {
                 f(key[j]);
@@ -174,12 +189,12 @@ select_kept_kernel(const SelectParams p)
         for (int j = 0; j < KPT; j++) {
             const uint64_t a = __ballot(key[j] > threshold), e = __ballot(key[j] == threshold);
             if (lane == 0) {
-                counts[j * kSelWaves + wave] = make_uint2(__builtin_popcountll(a), __builtin_popcountll(e));
+                counts[j * (T / 64) + wave] = make_uint2(__builtin_popcountll(a), __builtin_popcountll(e));
             }
         }
         __syncthreads();
         if (wave == 0) {   // exclusive sums in position order: lane l owns KPT / 4 consecutive entries
-            constexpr int PER = (KPT * kSelWaves + 63) / 64;
+            constexpr int PER = (KPT * (T / 64) + 63) / 64;
             uint2 sum = make_uint2(0, 0);
 #pragma unroll
             for (int i = 0; i < PER; i++) {
@@ -204,46 +219,69 @@ select_kept_kernel(const SelectParams p)
             }
         }
         __syncthreads();
+        // compared and counted anew below: kept over the barrier the ballots and positions take more registers than the keys
+        uint32_t first = lo + threadIdx.x;
+        asm volatile("" : "+v"(threshold), "+v"(first));
 #pragma unroll
         for (int j = 0; j < KPT; j++) {
             const bool is_above = key[j] > threshold, is_equal = key[j] == threshold;
             const uint64_t am = __ballot(is_above), em = __ballot(is_equal);
-            const uint2 before = counts[j * kSelWaves + wave];
+            const uint2 before = counts[j * (T / 64) + wave];
             const uint32_t a = before.x + __builtin_popcountll(am & below), e = before.y + __builtin_popcountll(em & below);
             if (is_above || (is_equal && e < equal)) {
-                out[p.sink + a + min(e, equal)] = static_cast<int32_t>(lo + j * kSelThreads + threadIdx.x);
+                out[p.sink + a + min(e, equal)] = static_cast<int32_t>(first + j * T);
             }
         }
     } else {
-        nth_largest([&](auto &&f) {
-            for (uint32_t i = lo + threadIdx.x; i < hi; i += kSelThreads) {
-                f(key_at(i));
+        nth_largest<T>([&](auto &&f) {
+            for (uint32_t i0 = lo + threadIdx.x; i0 < hi; i0 += kAhead * T) {
+                uint32_t key[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) {
+                    key[j] = key_at(min(i0 + j * T, hi - 1));
+                }
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) {
+                    if (i0 + j * T < hi) {
+                        f(key[j]);
+                    }
+                }
             }
         }, n, scratch, &threshold, &equal);
         uint32_t above_before = 0, equal_before = 0;
-        for (uint32_t i0 = lo; i0 < hi; i0 += kSelThreads) {
-            const uint32_t i = i0 + threadIdx.x;
-            const uint32_t k = key_at(min(i, hi - 1));
-            const bool is_above = i < hi && k > threshold, is_equal = i < hi && k == threshold;
-            const uint64_t above_mask = __ballot(is_above), equal_mask = __ballot(is_equal);
-            __syncthreads();
-            if (lane == 0) {
-                counts[wave] = make_uint2(__builtin_popcountll(above_mask), __builtin_popcountll(equal_mask));
-            }
-            __syncthreads();
-            uint32_t a = above_before, e = equal_before;
+        for (uint32_t i0 = lo; i0 < hi; i0 += kAhead * T) {
+            uint32_t key[kAhead];
 #pragma unroll
-            for (uint32_t w = 0; w < kSelWaves; w++) {
-                const uint2 c = counts[w];
-                a += w < wave ? c.x : 0u;
-                e += w < wave ? c.y : 0u;
-                above_before += c.x;
-                equal_before += c.y;
+            for (int j = 0; j < kAhead; j++) {
+                const uint32_t i = i0 + j * T + threadIdx.x;
+                key[j] = key_at(min(i, hi - 1));
+                key[j] = i < hi ? key[j] : 0u;
             }
-            a += __builtin_popcountll(above_mask & below);
-            e += __builtin_popcountll(equal_mask & below);
-            if (is_above || (is_equal && e < equal)) {
-                out[p.sink + a + min(e, equal)] = static_cast<int32_t>(i);
+            __syncthreads();   // the counts of the round before have been read
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const uint64_t above_mask = __ballot(key[j] > threshold), equal_mask = __ballot(key[j] == threshold);
+                if (lane == 0) {
+                    counts[j * (T / 64) + wave] = make_uint2(__builtin_popcountll(above_mask), __builtin_popcountll(equal_mask));
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const bool is_above = key[j] > threshold, is_equal = key[j] == threshold;
+                uint32_t a = above_before + __builtin_popcountll(__ballot(is_above) & below);
+                uint32_t e = equal_before + __builtin_popcountll(__ballot(is_equal) & below);
+#pragma unroll
+                for (uint32_t w = 0; w < T / 64; w++) {
+                    const uint2 c = counts[j * (T / 64) + w];
+                    a += w < wave ? c.x : 0u;
+                    e += w < wave ? c.y : 0u;
+                    above_before += c.x;
+                    equal_before += c.y;
+                }
+                if (is_above || (is_equal && e < equal)) {
+                    out[p.sink + a + min(e, equal)] = static_cast<int32_t>(i0 + j * T + threadIdx.x);
+                }
             }
         }
     }
@@ -399,14 +437,20 @@ extern "C" int xlite_hip_select_kept(void *stream, const float *weights, int32_t
     const uint32_t judged = max_num_block * block_size - std::min(max_num_block * block_size, sink + recent);   // at most
     hipStream_t s = as_stream(stream);
     const dim3 g(static_cast<uint32_t>(grid));
-    if (judged <= 4 * kSelThreads) {
-        select_kept_kernel<4><<<g, kSelThreads, 0, s>>>(p);
-    } else if (judged <= 16 * kSelThreads) {
-        select_kept_kernel<16><<<g, kSelThreads, 0, s>>>(p);
-    } else if (judged <= 40 * kSelThreads) {
-        select_kept_kernel<40><<<g, kSelThreads, 0, s>>>(p);
+    // The fewest keys a thread that hold the longest list: keys beyond a list's end cost their step all the same. 512 threads
+    // up to 32768, where two workgroups share a compute unit (64 lists of 8 heads x 32768: 58 us; 1024 threads with 40 keys
+    // and one workgroup 70); 1024 beyond (64000: 118 us); reading the keys again in every pass costs 413 there with a load at
+    // a time and remains for what no workgroup can hold (100000: 496 with 16 under way).
+    if (judged <= 4 * 1024) {
+        select_kept_kernel<4, 1024><<<g, 1024, 0, s>>>(p);
+    } else if (judged <= 16 * 1024) {
+        select_kept_kernel<16, 1024><<<g, 1024, 0, s>>>(p);
+    } else if (judged <= 64 * 512) {
+        select_kept_kernel<64, 512><<<g, 512, 0, s>>>(p);
+    } else if (judged <= 64 * 1024) {
+        select_kept_kernel<64, 1024><<<g, 1024, 0, s>>>(p);
     } else {
-        select_kept_kernel<0><<<g, kSelThreads, 0, s>>>(p);
+        select_kept_kernel<0, 1024><<<g, 1024, 0, s>>>(p);
     }
     XL_LAUNCH_CHECK();
     return XLITE_HIP_OK;

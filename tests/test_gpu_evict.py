@@ -178,6 +178,25 @@ def test_select(rt, KV, bs, lens, budget, recent, sink, kind):
             assert kept[i, h].tolist() == want + [-1] * (budget - len(want)), (i, h)
 
 
+@pytest.mark.parametrize("kind", ["random", "ties"])
+@pytest.mark.parametrize("lens", [[32769, 4000], [33100], [65536, 2], [65601], [65700, 66], [100003]])
+def test_select_long(rt, lens, kind):
+    """Around the lengths at which a list's keys stop fitting a workgroup's registers."""
+    from gvirt_amd._C import select_kept
+    KV, bs, budget, recent, sink = 1, 48, 1000, 60, 4
+    tables, mb, NB, g = paged(len(lens), lens, bs)
+    w = torch.rand(NB, bs, KV, generator=g)
+    if kind == "ties":
+        w = (w * 4).floor()
+    kept, kept_lens = i32([[[9] * budget] * KV] * len(lens)), i32([9] * len(lens))
+    select_kept(rt, w.to(DEV), kept, kept_lens, i32(lens), tables.to(DEV), KV, bs, len(lens), mb, budget, recent, sink)
+    kept = kept.cpu()
+    assert kept_lens.tolist() == [min(n, budget) for n in lens]
+    for i, n in enumerate(lens):
+        want = plain_select(w.view(-1, KV)[slots(tables[i], n, bs), 0].tolist(), n, budget, recent, sink)
+        assert kept[i, 0].tolist() == want + [-1] * (budget - len(want)), i
+
+
 # ---- compact_kv_cache ------------------------------------------------------------------------------------------------------
 
 def compact_case(rt, seed, totals, starts, KV, D, bs, dtype, per_head, counts, width, weights=True, lists=None):
