@@ -267,7 +267,7 @@ row_stats_kernel(const WeightsParams p)
     }
 }
 
-// The same for 16-bit caches of head_dim 64 and 128, K tiles of 64 positions copied straight into LDS (a ring of four) and
+// The same for 16-bit caches of head_dim 64 and 128, K tiles of 64 positions copied straight into LDS (a ring of three) and
 // shared by the four waves. Read from memory by every wave, as above, a K chunk of 32 positions touches 32 lines per
 // instruction and every line four times: the vector cache's look-ups took longer than the products and the exponentials.
 template <typename T, int D>
@@ -822,17 +822,20 @@ __device__ __forceinline__ uint32_t stored_base(const WeightsParams &p, uint32_t
     return (p.window != 0 ? seq * p.window : s.start) * p.group;
 }
 
-// A wave takes the positions of one kv head, 64 at a time, of the workgroup's chunk [chunk * split_len, + split_len): K rows
+// A wave takes the positions of one kv head, 32 at a time, of the workgroup's chunk [chunk * split_len, + split_len): K rows
 // straight from memory as the A operand (a lane reads its row's chunk of 16 bytes, four lanes a row's 64 consecutive bytes),
-// the next 64 in flight; 16 M rows as the columns. It leaves the scores and every row's maximum and sum over the chunk.
+// the next 32 in flight; 16 M rows as the columns. It leaves the scores and every row's maximum and sum over the chunk.
 // Waves of a workgroup: the kv heads side by side, so that they read a position's whole row together, and where there are
 // fewer than eight heads, neighbouring chunks.
+// Measured, 64 decode rows of 8 kv heads over up to 4096 positions of 128 elements (335 MB of K): 89 us, 3.8 TB/s, with 32
+// positions an iteration and four waves a SIMD; 64 positions and two waves took 101. What bounds it: pieces of 64 bytes, four
+// requests for a row, each its own look-up (whole KiB through LDS reach 5.6 TB/s in attention over trees).
 template <typename T, int D, int KVF>
 __global__ void __launch_bounds__(512)
 store_scores_kernel(const WeightsParams p)
 {
     constexpr int KS = D / 32;
-    constexpr int NT = D == 256 ? 2 : 4;      // tiles of 16 positions of an iteration
+    constexpr int NT = 2;                     // tiles of 16 positions of an iteration
     constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
     constexpr uint32_t ROWB = D * (KV8 ? 1 : 2);
     typedef typename std::conditional<KV8, uint2, uint4>::type raw_t;
