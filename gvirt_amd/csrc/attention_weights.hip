@@ -822,42 +822,100 @@ __device__ __forceinline__ uint32_t stored_base(const WeightsParams &p, uint32_t
     return (p.window != 0 ? seq * p.window : s.start) * p.group;
 }
 
-// A wave takes the positions of one kv head, 32 at a time, of the workgroup's chunk [chunk * split_len, + split_len): K rows
-// straight from memory as the A operand (a lane reads its row's chunk of 16 bytes, four lanes a row's 64 consecutive bytes),
-// the next 32 in flight; 16 M rows as the columns. It leaves the scores and every row's maximum and sum over the chunk.
-// Waves of a workgroup: the kv heads side by side, so that they read a position's whole row together, and where there are
-// fewer than eight heads, neighbouring chunks.
-// Measured, 64 decode rows of 8 kv heads over up to 4096 positions of 128 elements (335 MB of K): 89 us, 3.8 TB/s, with 32
-// positions an iteration and four waves a SIMD; 64 positions and two waves took 101. What bounds it: pieces of 64 bytes, four
-// requests for a row, each its own look-up (whole KiB through LDS reach 5.6 TB/s in attention over trees).
+// A wave takes the positions of one kv head, of a chunk [chunk * split_len, + split_len): K rows are copied as they stand into
+// the wave's own ring of stages in LDS (no barriers), a whole row by neighbouring lanes, 16 rows are the A operand of a
+// product with 16 M rows as columns. It leaves the scores and every row's maximum and sum over the chunk. Waves of a
+// workgroup: kv heads side by side, and where there are fewer than four, neighbouring chunks.
+// Bound by memory. Measured, 64 decode rows of 8 kv heads over up to 4096 positions of 128 elements (340 MB of K): 73 us, 4.7
+// TB/s; 79 without the hint that nobody reads the bytes again, 89 with the operand read straight from memory (a row in four
+// requests of 64 bytes). A ring of four stages (two workgroups a compute unit instead of three) is no faster.
+template <int D, bool KV8>
+struct StoredTile {
+    static constexpr uint32_t ROWB = D * (KV8 ? 1 : 2);
+    static constexpr uint32_t C = ROWB / 16;                                    // 16-byte chunks of a row
+    static constexpr uint32_t BN = ROWB * 16 > 4096 ? 16 : 4096 / ROWB;         // positions of a stage: 16 .. 64
+    static constexpr uint32_t BYTES = BN * ROWB, COPIES = BYTES / 1024;
+    static constexpr uint32_t SCALES = KV8 ? 256 : 0;                           // a stage's K scales, behind its rows
+    static constexpr int STAGES = D == 256 ? 2 : 3;
+    static constexpr uint32_t RING = STAGES * (BYTES + SCALES);
+    // 16-byte chunk i of a stage, exchanged within its 256 bytes: 16 rows' chunks of one column lie in different banks
+    static __device__ __forceinline__ uint32_t exchanged(uint32_t i)
+    {
+        return i ^ ((C == 32 ? i >> 5 : i >> 4) & 15u);
+    }
+};
+constexpr uint32_t kStoredWaves = 4;
+
+__host__ __device__ __forceinline__ uint32_t stored_table(uint32_t split_len, uint32_t block_size)   // entries, in whole 16 bytes
+{
+    return (split_len / block_size + 2 + 3) / 4 * 4;
+}
+
 template <typename T, int D, int KVF>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(64 * kStoredWaves)
 store_scores_kernel(const WeightsParams p)
 {
-    constexpr int KS = D / 32;
-    constexpr int NT = 2;                     // tiles of 16 positions of an iteration
     constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
-    constexpr uint32_t ROWB = D * (KV8 ? 1 : 2);
-    typedef typename std::conditional<KV8, uint2, uint4>::type raw_t;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, jq = lane >> 4;
-    const uint32_t heads = min(p.n_kv_heads, 8u), per_wg = 8u / heads;       // kv heads and chunks of a workgroup
-    if (wave >= heads * per_wg) {
-        return;
-    }
-    const uint32_t kvh = blockIdx.z * heads + wave % heads, chunk = blockIdx.x * per_wg + wave / heads, seq = blockIdx.y, G = p.group;
+    typedef StoredTile<D, KV8> Tile;
+    constexpr int KS = D / 32, NT = Tile::BN / 16, S = Tile::STAGES, C = Tile::C;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, jq = lane >> 4;
+    const uint32_t heads = min(p.n_kv_heads, kStoredWaves), per_wg = kStoredWaves / heads;   // kv heads and chunks of a workgroup
+    const uint32_t parts = ceil_div(p.n_kv_heads, heads);
+    const uint32_t kvh = blockIdx.x % parts * heads + wave % heads, chunk = blockIdx.x / parts * per_wg + wave / heads;
+    const uint32_t seq = blockIdx.y, G = p.group;
     const Sequence s = sequence_of(p, seq);
     const uint32_t total = s.cached + s.nodes;
     const uint32_t begin = chunk * p.split_len, end = min(total, begin + p.split_len);
-    if (kvh >= p.n_kv_heads || s.nodes == 0 || chunk >= p.splits) {
+    if (wave >= heads * per_wg || kvh >= p.n_kv_heads || s.nodes == 0 || chunk >= p.splits) {
         return;
     }
+    const uint32_t entries = stored_table(p.split_len, p.block_size);
+    unsigned char *ring = smem + wave * (Tile::RING + entries * 4);
+    uint32_t *tbl = reinterpret_cast<uint32_t *>(ring + Tile::RING);
+    const uint32_t ring_addr = stage::lds_address(smem) + wave * (Tile::RING + entries * 4);
     const uint32_t base = stored_base(p, seq, s);
     const uint64_t rows0 = static_cast<uint64_t>(kvh) * p.m_total + base;
-    const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
+    auto block_of = [&](uint32_t pos) __attribute__((always_inline)) { return p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size; };
+    const uint32_t blk0 = block_of(begin);
+    if (begin < end) {
+        const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block + blk0;
+        const uint32_t blocks = block_of(end - 1) - blk0 + 1;
+        for (uint32_t i = lane; i < blocks; i += 64) {
+            tbl[i] = static_cast<uint32_t>(table[i]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    // row of K, of a scale
+    auto row_at = [&](uint32_t pos) __attribute__((always_inline)) {
+        const uint32_t t = min(pos, end - 1), b = block_of(t);
+        return (static_cast<uint64_t>(tbl[b - blk0]) * p.block_size + (t - b * p.block_size)) * p.n_kv_heads + kvh;
+    };
+    // copies of the chunk's tile `it` into stage `slot` (positions past the end repeat the last one: their scores are masked, and
+    // every tile is the same number of copies)
+    auto issue = [&](uint32_t it, uint32_t slot, bool once) __attribute__((always_inline)) {
+        const uint32_t t0 = begin + it * Tile::BN, st = ring_addr + slot * (Tile::BYTES + Tile::SCALES);
+#pragma unroll
+        for (uint32_t i = 0; i < Tile::COPIES; i++) {
+            const uint32_t x = Tile::exchanged(64 * i + lane);
+            const unsigned char *src = p.k_cache + row_at(t0 + x / C) * Tile::ROWB + x % C * 16;
+            if (once) {
+                stage::copy_lanes_16_once(st + i * 1024, src);
+            } else {
+                stage::copy_lanes_16(st + i * 1024, src);
+            }
+        }
+        if constexpr (KV8) {
+            stage::copy_lanes_4(st + Tile::BYTES, p.k_scale + row_at(t0 + min(lane, Tile::BN - 1)));
+        }
+    };
     for (uint32_t m0 = 0; m0 < s.m_rows; m0 += 16) {
         const uint32_t m = min(m0 + col, s.m_rows - 1);
         const uint32_t r = s.first + m / G;
         const uint32_t lim = s.cached + r + 1;
+        const bool once = m0 + 16 >= s.m_rows;   // no further rows read the chunk again
         float m_run = -INFINITY, l_run = 0.f;
         if (begin < end) {
             const uint16_t *src = p.q + static_cast<uint64_t>(s.start + r) * p.q_tok_stride + static_cast<uint64_t>(kvh * G + m % G) * D;
@@ -866,65 +924,50 @@ store_scores_kernel(const WeightsParams p)
             for (int ks = 0; ks < KS; ks++) {
                 qreg[ks] = *reinterpret_cast<const uint4 *>(src + ks * 32 + jq * 8);
             }
-            raw_t next[NT][KS];
-            float scale_next[NT];
-            auto request = [&](uint32_t t0) __attribute__((always_inline)) {
+            // complete these loads before any copy is issued
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const uint64_t at = slot_of(p, table, min(t0 + nt * 16 + col, end - 1)) * p.n_kv_heads + kvh;
-                    const unsigned char *row = p.k_cache + at * ROWB;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        next[nt][ks] = *reinterpret_cast<const raw_t *>(row + (4 * ks + jq) * sizeof(raw_t));
-                    }
-                    if constexpr (KV8) {
-                        scale_next[nt] = p.k_scale[at];
-                    }
-                }
-            };
+            for (int ks = 0; ks < KS; ks++) {
+                asm volatile("" : "+v"(qreg[ks].x), "+v"(qreg[ks].y), "+v"(qreg[ks].z), "+v"(qreg[ks].w));
+            }
             float *out = p.scores + (rows0 + m0 + col) * p.pitch;
-            request(begin);
-            for (uint32_t t0 = begin; t0 < end; t0 += 16 * NT) {
-                raw_t now[NT][KS];
-                float scale[NT];
+            const uint32_t n_it = ceil_div(end - begin, Tile::BN);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        now[nt][ks] = next[nt][ks];
-                    }
-                    if constexpr (KV8) {
-                        scale[nt] = scale_next[nt];
-                    }
-                }
-                if (t0 + 16 * NT < end) {
-                    request(t0 + 16 * NT);
-                }
-                f32x4v_t S[NT];
+            for (int i = 0; i < S - 1; i++) {
+                issue(i, i, once);
+            }
+            uint32_t slot = 0;
+            for (uint32_t it = 0; it < n_it; it++) {
+                stage::wait<(S - 2) * (Tile::COPIES + (KV8 ? 1 : 0))>();   // this tile has landed (the scores' stores make it wait for a little more)
+                issue(it + S - 1, slot == 0 ? S - 1 : slot - 1, once);    // into the stage that the last iteration has read
+                const unsigned char *st = ring + slot * (Tile::BYTES + Tile::SCALES);
+                slot = slot == S - 1 ? 0u : slot + 1;
+                const uint32_t t0 = begin + it * Tile::BN;
+                f32x4v_t sc[NT];
                 float mx = m_run;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    S[nt] = f32x4v_t{0.f, 0.f, 0.f, 0.f};
+                    sc[nt] = f32x4v_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++) {
                         if constexpr (KV8) {
-                            S[nt] = mfma16<T>(dequant8<T, KVF>(now[nt][ks], 1.0f), qreg[ks], S[nt]);
+                            const uint32_t at = Tile::exchanged((nt * 16 + col) * C + 2 * ks + (jq >> 1)) * 16 + (jq & 1u) * 8;
+                            sc[nt] = mfma16<T>(dequant8<T, KVF>(*reinterpret_cast<const uint2 *>(st + at), 1.0f), qreg[ks], sc[nt]);
                         } else {
-                            S[nt] = mfma16<T>(now[nt][ks], qreg[ks], S[nt]);
+                            const uint32_t at = Tile::exchanged((nt * 16 + col) * C + 4 * ks + jq) * 16;
+                            sc[nt] = mfma16<T>(*reinterpret_cast<const uint4 *>(st + at), qreg[ks], sc[nt]);
                         }
+                    }
+                    f32x4v_t mul = {kLog2e, kLog2e, kLog2e, kLog2e};
+                    if constexpr (KV8) {
+                        mul *= *reinterpret_cast<const f32x4v_t *>(st + Tile::BYTES + (nt * 16 + 4 * jq) * 4);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const uint32_t o = nt * 16 + 4 * jq + e;
-                        float x = S[nt][e] * kLog2e;
-                        if constexpr (KV8) {   // the scale of position t0 + 16 nt + col; register e holds another one
-                            x *= __shfl(scale[nt], static_cast<int>(4 * jq + e));
-                        }
-                        S[nt][e] = x;
-                        mx = fmaxf(mx, t0 + o < lim ? x : -INFINITY);
+                        sc[nt][e] *= mul[e];
+                        mx = fmaxf(mx, t0 + nt * 16 + 4 * jq + e < lim ? sc[nt][e] : -INFINITY);
                     }
                     if (m0 + col < s.m_rows) {   // (positions past the end: inside the row's pitch, nobody reads them)
-                        *reinterpret_cast<float4 *>(out + t0 + nt * 16 + 4 * jq) = make_float4(S[nt][0], S[nt][1], S[nt][2], S[nt][3]);
+                        *reinterpret_cast<float4 *>(out + t0 + nt * 16 + 4 * jq) = make_float4(sc[nt][0], sc[nt][1], sc[nt][2], sc[nt][3]);
                     }
                 }
                 const float m_safe = mx == -INFINITY ? 0.f : mx;
@@ -933,13 +976,14 @@ store_scores_kernel(const WeightsParams p)
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float x = fast_exp2(S[nt][e] - m_safe);
+                        const float x = fast_exp2(sc[nt][e] - m_safe);
                         sum += t0 + nt * 16 + 4 * jq + e < lim ? x : 0.f;
                     }
                 }
                 l_run = l_run * fast_exp2(m_run - m_safe) + sum;
                 m_run = mx;
             }
+            stage::wait<0>();   // (nothing is left on its way into LDS)
         }
         // the row's four lanes
 #pragma unroll
@@ -1017,9 +1061,9 @@ Plan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint3
     if (plan.stored) {
         plan.rows = static_cast<uint32_t>(bounded) * G;
         plan.pitch = ceil_div(max_ctx, 64u) * 64u;
-        // chunks of 64 to 256 positions: as long as there are four workgroups (of eight waves) per compute unit
+        // chunks of 64 to 512 positions: the longest that leave 4096 waves (16 per compute unit; 12 fit)
         const uint64_t waves64 = static_cast<uint64_t>(batch) * ceil_div(max_ctx, 64u) * n_kv_heads;
-        plan.split_len = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(4, waves64 / 8192))) * 64u;
+        plan.split_len = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(8, waves64 / 4096))) * 64u;
         plan.splits = ceil_div(max_ctx, plan.split_len);
         const size_t rows = static_cast<size_t>(plan.rows) * n_kv_heads;
         plan.bytes = ((rows + 3) / 4 * 4 + rows * plan.pitch + 2 * rows * plan.splits) * sizeof(float);
@@ -1124,8 +1168,13 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
         using T = decltype(t);
         constexpr int D = decltype(d)::value, KVF = decltype(kvf)::value;
         if (plan.stored) {
-            const uint32_t heads = std::min(n_kv_heads, 8u);
-            store_scores_kernel<T, D, KVF><<<dim3(ceil_div(plan.splits, 8u / heads), batch, ceil_div(n_kv_heads, heads)), 512, 0, s>>>(p);
+            const uint32_t heads = std::min(n_kv_heads, kStoredWaves);
+            const size_t lds = kStoredWaves * (StoredTile<D, KVF != XLITE_HIP_KV_SAME>::RING + stored_table(plan.split_len, block_size) * sizeof(uint32_t));
+            if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(store_scores_kernel<T, D, KVF>), lds)) {
+                return rc;
+            }
+            store_scores_kernel<T, D, KVF><<<dim3(ceil_div(plan.splits, kStoredWaves / heads) * ceil_div(n_kv_heads, heads), batch),
+                                             64 * kStoredWaves, lds, s>>>(p);
         } else {
             // K through LDS: 16-bit caches whose copies (four positions of 128 elements, eight of 64) lie in one block, and a
             // split's block-table entries behind the stages

@@ -27,6 +27,10 @@ __device__ __forceinline__ void copy_lanes_16(uint32_t lds_addr, const void *src
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t" :: "s"(lds_addr), "v"(src) : "memory", "m0");
 }
+__device__ __forceinline__ void copy_lanes_16_once(uint32_t lds_addr, const void *src)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt\n\t" :: "s"(lds_addr), "v"(src) : "memory", "m0");
+}
 __device__ __forceinline__ void copy_lanes_4(uint32_t lds_addr, const void *src)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\t" :: "s"(lds_addr), "v"(src) : "memory", "m0");
