@@ -2,6 +2,8 @@
 // prefill kernel that reads quantised caches itself (prefill_mfma.hip): the same code, so the two give the same bits.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace xlite {
@@ -37,6 +39,20 @@ __device__ __forceinline__ uint4 dequant8(const uint2 &raw, float scale)
         x[j] = clamp_f16(x[j]);
     }
     return make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
+}
+
+// eight 16-bit values of storage type FROM as type TO
+template <typename FROM, typename TO>
+__device__ __forceinline__ uint4 convert8(const uint4 &x)
+{
+    if constexpr (std::is_same<FROM, TO>::value) {
+        return x;
+    } else {
+        auto one = [](uint32_t w) {
+            return TO::pack(fminf(fmaxf(FROM::lo(w), -65504.f), 65504.f), fminf(fmaxf(FROM::hi(w), -65504.f), 65504.f));
+        };
+        return make_uint4(one(x.x), one(x.y), one(x.z), one(x.w));
+    }
 }
 
 }  // namespace xlite

@@ -124,20 +124,6 @@ __device__ __forceinline__ void dma_wait()
     asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
 }
 
-// eight 16-bit values of storage type FROM as type TO
-template <typename FROM, typename TO>
-__device__ __forceinline__ uint4 convert8(const uint4 &x)
-{
-    if constexpr (std::is_same<FROM, TO>::value) {
-        return x;
-    } else {
-        auto one = [](uint32_t w) {
-            return TO::pack(fminf(fmaxf(FROM::lo(w), -65504.f), 65504.f), fminf(fmaxf(FROM::hi(w), -65504.f), 65504.f));
-        };
-        return make_uint4(one(x.x), one(x.y), one(x.z), one(x.w));
-    }
-}
-
 // T: the type of the caches and of the products; TIO: the type of the query rows and of the output (the same, or
 // bf16 over fp16 caches: a bf16 model over the fp16 copy of a quantised cache)
 // KVF: the cache is 16-bit (copied straight into LDS), or int8 / fp8 bytes with one fp32 scale per (position, kv head):

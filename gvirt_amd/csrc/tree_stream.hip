@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "attention_common.h"
+#include "kv8.h"
 #include "stage.h"
 
 namespace xlite {
@@ -35,6 +36,10 @@ constexpr uint32_t kStages = 4;
 template <int NH>
 constexpr uint32_t kRows = 32 * kWaves / NH;     // M rows of a workgroup, per kv head
 constexpr uint32_t kStage = 2 * kHalf;
+constexpr uint32_t kWaveRaw = 2 * 1024 + 256;    // caches of bytes: what a wave copies in a step, 8 rows of K and of V and their scales
+constexpr uint32_t kRawStage = kWaves * kWaveRaw;
+template <bool KV8>
+constexpr uint32_t kStageBytes = KV8 ? 2 * kStage + kStages * kRawStage : kStages * kStage;
 constexpr uint32_t kTblCap = 2048;               // block-table entries staged per segment
 constexpr uint32_t kSeqCap = 1024;               // sequences whose prefix sums fit
 constexpr uint32_t kMaskCap = kThreads;          // mask words of an M tile kept in LDS: 128 rows of 4 heads and 512 nodes
@@ -55,8 +60,10 @@ __device__ __forceinline__ f32x16_t mfma32(const uint4 &a, const uint4 &b, f32x1
 
 struct StreamParams {
     const uint16_t *q;
-    const uint16_t *k_cache;
-    const uint16_t *v_cache;
+    const unsigned char *k_cache;
+    const unsigned char *v_cache;
+    const float *k_scale;  // caches of bytes: [slot][kv head]
+    const float *v_scale;
     uint16_t *out;
     const uint32_t *tree_mask;
     const int32_t *query_start_loc;
@@ -82,11 +89,13 @@ __device__ __forceinline__ uint32_t uni(uint32_t x)
     return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
 }
 
-// NH: kv heads of a workgroup
-template <typename T, int NH>
+// NH: kv heads of a workgroup. T: the type of the products; TIO: of the query rows and the output (the same, or bf16 with fp16
+// products over caches of bytes, KVF).
+template <typename T, int NH, int KVF, typename TIO>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_stream_kernel(const StreamParams p)
 {
+    constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
     constexpr int KS = D / 16, DT = D / 32;
     constexpr uint32_t ROWS = kRows<NH>;
     constexpr uint32_t POSB = NH * 256;          // LDS bytes of a position
@@ -94,7 +103,7 @@ tree_stream_kernel(const StreamParams p)
     constexpr uint32_t PPI = 1024 / POSB;        // positions of a copy
     constexpr int CPW = 2;                       // copies per wave, step and tensor
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    uint32_t *tbl = reinterpret_cast<uint32_t *>(smem + kStages * kStage);
+    uint32_t *tbl = reinterpret_cast<uint32_t *>(smem + kStageBytes<KV8>);
     uint32_t *mask_lds = tbl + kTblCap;
     uint32_t *pref = mask_lds + kMaskCap;        // batch + 1 words
     const uint32_t smem_addr = stage::lds_address(smem);
@@ -306,6 +315,34 @@ tree_stream_kernel(const StreamParams p)
                 }
             };
 
+            // Caches of bytes: a wave copies the bytes of 8 (position, kv head) rows and their scales of K and of V per step, four
+            // steps ahead, and turns what it copied itself into fp16 rows of one of two stages: no barrier in between.
+            constexpr uint32_t RP = 8 / NH;   // positions of a wave
+            auto row8 = [&](uint32_t s, uint32_t r) __attribute__((always_inline)) {
+                const uint32_t pos = min(t0 + s * SP + wave * RP + r / NH, t1 - 1), blk = __umulhi(pos, p.block_magic);
+                return (static_cast<uint64_t>(tbl[blk - blk0]) * p.block_size + (pos - blk * p.block_size)) * p.n_kv_heads + blockIdx.y * NH + r % NH;
+            };
+            auto issue8 = [&](uint32_t s) __attribute__((always_inline)) {
+                const uint32_t st = smem_addr + 2 * kStage + (s % kStages) * kRawStage + wave * kWaveRaw;
+                const uint64_t off = row8(s, lane >> 3) * D + (lane & 7u) * 16;
+                stage::copy_lanes_16_once(st, p.k_cache + off);
+                stage::copy_lanes_16_once(st + 1024, p.v_cache + off);
+                stage::copy_lanes_4(st + 2048, ((lane & 8u) != 0 ? p.v_scale : p.k_scale) + row8(s, lane & 7u));   // K: words 0 .. 7, V: 8 .. 15
+            };
+            auto widen = [&](uint32_t s) __attribute__((always_inline)) {
+                const unsigned char *raw = smem + 2 * kStage + (s % kStages) * kRawStage + wave * kWaveRaw;
+                const uint32_t r = lane >> 3, pos = wave * RP + r / NH, x = stage::pattern<D>(pos);
+                unsigned char *dst = smem + (s % 2) * kStage + pos * POSB + (r % NH) * 256;
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const uint4 bytes = *reinterpret_cast<const uint4 *>(raw + v * 1024 + lane * 16);
+                    const float scale = *reinterpret_cast<const float *>(raw + 2048 + v * 32 + r * 4);
+                    const uint32_t c = 2 * (lane & 7u);
+                    *reinterpret_cast<uint4 *>(dst + v * kHalf + ((c ^ x) << 4)) = dequant8<T, KVF>(make_uint2(bytes.x, bytes.y), scale);
+                    *reinterpret_cast<uint4 *>(dst + v * kHalf + (((c + 1) ^ x) << 4)) = dequant8<T, KVF>(make_uint2(bytes.z, bytes.w), scale);
+                }
+            };
+
             // which of the positions j0 .. j0 + 31 the lane's row sees, moved so that bit 8 (k / 4) + k % 4 is that of register k
             auto seen_from = [&](uint32_t j0) __attribute__((always_inline)) {
                 const uint32_t *words = words_in_lds ? mask_lds + (m / G - tok_first) * p.mask_words : p.tree_mask + tok * p.mask_words;
@@ -316,7 +353,7 @@ tree_stream_kernel(const StreamParams p)
             auto compute = [&](uint32_t s, uint32_t h) __attribute__((always_inline)) {
                 const uint32_t j0 = t0 + s * SP + 32 * h;
                 const bool masked = j0 + 32 > cached;   // (positions below the cached length are seen by every row)
-                const unsigned char *st = smem + (s % kStages) * kStage + h * 32 * POSB;
+                const unsigned char *st = smem + (s % (KV8 ? 2 : kStages)) * kStage + h * 32 * POSB;
                 uint4 kop[KS];
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
@@ -356,17 +393,17 @@ tree_stream_kernel(const StreamParams p)
                     }
                     // A row that does not see a position has probability zero there, and zero times an infinity or a NaN in
                     // that position's V row would still poison it. Such values leave the operands; the rows that see them
-                    // get them back behind the loop.
+                    // get them back behind the loop. (Values widened from bytes are finite.)
                     uint32_t odd = 0;
 #pragma unroll
-                    for (int kk = 0; kk < 2; kk++) {
+                    for (int kk = 0; kk < (KV8 ? 0 : 2); kk++) {
 #pragma unroll
                         for (int dt = 0; dt < DT; dt++) {
                             odd |= not_finite2<T>(vop[kk][dt].x) | not_finite2<T>(vop[kk][dt].y) | not_finite2<T>(vop[kk][dt].z) |
                                    not_finite2<T>(vop[kk][dt].w);
                         }
                     }
-                    if (__any(odd)) {
+                    if (!KV8 && __any(odd)) {
                         poisoned = true;
 #pragma unroll
                         for (int kk = 0; kk < 2; kk++) {
@@ -425,19 +462,50 @@ tree_stream_kernel(const StreamParams p)
             };
 
             const uint32_t n_steps = b - a, last = n_steps - 1;
-            issue(0);
-            if (last >= 1) {
-                issue(1);
-            }
-            if (last >= 2) {
-                issue(2);
+            if constexpr (KV8) {
+                for (uint32_t s = 0; s < min(n_steps, kStages); s++) {
+                    issue8(s);
+                }
+            } else {
+                issue(0);
+                if (last >= 1) {
+                    issue(1);
+                }
+                if (last >= 2) {
+                    issue(2);
+                }
             }
             // (the query rows were requested before the copies; their wait is for both)
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 asm volatile("" : "+v"(qreg[ks].x), "+v"(qreg[ks].y), "+v"(qreg[ks].z), "+v"(qreg[ks].w));
+                qreg[ks] = convert8<TIO, T>(qreg[ks]);
             }
             for (uint32_t s = 0; s < n_steps; s++) {
+                if constexpr (KV8) {
+                    // this wave's share of step s has landed: three copies of each of the next three steps are out
+                    if (s + 3 <= last) {
+                        stage::wait<9>();
+                    } else if (s + 2 <= last) {
+                        stage::wait<6>();
+                    } else if (s + 1 <= last) {
+                        stage::wait<3>();
+                    } else {
+                        stage::wait<0>();
+                    }
+                    widen(s);          // (the stage of step s - 2: everybody was past it at the barrier of step s - 1)
+                    __syncthreads();
+                    if (s + 4 <= last) {
+                        issue8(s + 4);
+                    }
+                    if (has_rows) {
+#pragma unroll 1
+                        for (uint32_t h = 0; h < SP / 32; h++) {
+                            compute(s, h);
+                        }
+                    }
+                    continue;
+                }
                 // this wave's share of step s has landed: only those of the next two are out
                 if (s + 2 <= last) {
                     stage::wait<4 * CPW>();
@@ -457,11 +525,11 @@ tree_stream_kernel(const StreamParams p)
                     }
                 }
             }
-            if (poisoned) {   // (rare, and not fast: the tree's V rows are read again, value by value)
+            if (!KV8 && poisoned) {   // (rare, and not fast: the tree's V rows are read again, value by value)
                 for (uint32_t j = max(t0, cached); j < t1; j++) {
                     const uint32_t blk = j / p.block_size;
                     const uint64_t row = static_cast<uint64_t>(static_cast<uint32_t>(table[blk])) * p.block_size + (j - blk * p.block_size);
-                    const uint16_t *v = p.v_cache + (row * p.n_kv_heads + kvh) * D + 4 * half;
+                    const uint16_t *v = reinterpret_cast<const uint16_t *>(p.v_cache) + (row * p.n_kv_heads + kvh) * D + 4 * half;
                     const bool see = tree_seen(p.tree_mask + tok * p.mask_words, p.mask_words, j, cached, nodes) & 1u;
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
@@ -486,8 +554,8 @@ tree_stream_kernel(const StreamParams p)
 #pragma unroll
                         for (int kg = 0; kg < 4; kg++) {
                             uint2 o;
-                            o.x = T::pack(O[dt][kg * 4] * scale, O[dt][kg * 4 + 1] * scale);
-                            o.y = T::pack(O[dt][kg * 4 + 2] * scale, O[dt][kg * 4 + 3] * scale);
+                            o.x = TIO::pack(O[dt][kg * 4] * scale, O[dt][kg * 4 + 1] * scale);
+                            o.y = TIO::pack(O[dt][kg * 4 + 2] * scale, O[dt][kg * 4 + 3] * scale);
                             *reinterpret_cast<uint2 *>(dst + dt * 32 + kg * 8 + half * 4) = o;
                         }
                     }
@@ -630,11 +698,12 @@ StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
 
 }  // namespace
 
-// head_dim 128, 16-bit caches; a copy's positions share a block; every block that a step can reach has its table entry in LDS
+// head_dim 128; a copy's positions share a block (16-bit caches: four of them; bytes are copied from an address per lane); every
+// block that a step can reach has its table entry in LDS
 bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
                            uint32_t max_num_block, int kv_dtype)
 {
-    return head_dim == D && kv_dtype == XLITE_HIP_KV_SAME && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && block_size % 4 == 0 &&
+    return head_dim == D && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && (block_size % 4 == 0 || kv_dtype != XLITE_HIP_KV_SAME) &&
            batch <= kSeqCap && static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32);
 }
 
@@ -660,8 +729,10 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     }
     StreamParams p{};
     p.q = static_cast<const uint16_t *>(a.qkv);
-    p.k_cache = static_cast<const uint16_t *>(a.k_cache);
-    p.v_cache = static_cast<const uint16_t *>(a.v_cache);
+    p.k_cache = static_cast<const unsigned char *>(a.k_cache);
+    p.v_cache = static_cast<const unsigned char *>(a.v_cache);
+    p.k_scale = a.k_scale;
+    p.v_scale = a.v_scale;
     p.out = static_cast<uint16_t *>(a.output);
     p.tree_mask = a.tree_mask;
     p.query_start_loc = a.query_start_loc;
@@ -681,25 +752,35 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     p.meta = static_cast<int4 *>(a.workspace);
     p.acc = reinterpret_cast<float *>(p.meta + plan.tiles);
     p.ml = p.acc + static_cast<uint64_t>(plan.groups) * plan.slots * 32 * kWaves * D;
-    const size_t lds = kStages * kStage + (kTblCap + kMaskCap + a.batch + 1) * sizeof(uint32_t);
     const dim3 grid(std::max(1u, kComputeUnits / plan.groups), plan.groups), merge_grid(plan.tiles, a.n_kv_heads, 32 * kWaves / plan.nh / 16);
-    auto launch = [&](auto t, auto n) -> int {
+    auto launch = [&](auto t, auto n, auto kvf, auto io) -> int {
         using T = decltype(t);
-        constexpr int NH = decltype(n)::value;
-        auto kernel = tree_stream_kernel<T, NH>;
+        using TIO = decltype(io);
+        constexpr int NH = decltype(n)::value, KVF = decltype(kvf)::value;
+        auto kernel = tree_stream_kernel<T, NH, KVF, TIO>;
+        const size_t lds = kStageBytes<KVF != XLITE_HIP_KV_SAME> + (kTblCap + kMaskCap + a.batch + 1) * sizeof(uint32_t);
         if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds)) {
             return rc;
         }
         kernel<<<grid, kThreads, lds, stream>>>(p);
         XL_LAUNCH_CHECK();
-        tree_merge_kernel<T, NH><<<merge_grid, 256, 0, stream>>>(p);
+        tree_merge_kernel<TIO, NH><<<merge_grid, 256, 0, stream>>>(p);
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;
     };
-    auto with_heads = [&](auto t) -> int {
-        return plan.nh == 2 ? launch(t, std::integral_constant<int, 2>{}) : launch(t, std::integral_constant<int, 1>{});
+    auto with_heads = [&](auto t, auto kvf, auto io) -> int {
+        return plan.nh == 2 ? launch(t, std::integral_constant<int, 2>{}, kvf, io) : launch(t, std::integral_constant<int, 1>{}, kvf, io);
     };
-    return a.dtype == XLITE_HIP_BF16 ? with_heads(BF16{}) : with_heads(FP16{});
+    auto with_bytes = [&](auto kvf) -> int {
+        return a.dtype == XLITE_HIP_BF16 ? with_heads(FP16{}, kvf, BF16{}) : with_heads(FP16{}, kvf, FP16{});
+    };
+    switch (a.kv_dtype) {
+    case XLITE_HIP_KV_INT8: return with_bytes(std::integral_constant<int, XLITE_HIP_KV_INT8>{});
+    case XLITE_HIP_KV_FP8: return with_bytes(std::integral_constant<int, XLITE_HIP_KV_FP8>{});
+    default: break;
+    }
+    using Same = std::integral_constant<int, XLITE_HIP_KV_SAME>;
+    return a.dtype == XLITE_HIP_BF16 ? with_heads(BF16{}, Same{}, BF16{}) : with_heads(FP16{}, Same{}, FP16{});
 }
 
 }  // namespace xlite
