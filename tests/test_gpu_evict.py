@@ -257,6 +257,45 @@ def test_compact_ignores_entries_that_break_the_rules(rt):
     compact_case(rt, 4, [64], None, 2, 64, 16, BF, True, [8], 8, lists=[[[7] * 8, [9, 9, 9, 9, 8, 8, 8, 7]]])   # a source twice
 
 
+def test_select_and_compact_captured():
+    """Both captured together, replayed on weights and rows that change, the lists written by the one and read by the other."""
+    from gvirt_amd._C import Runtime, compact_kv_cache, select_kept
+    r2 = Runtime(0, 8)
+    r2.blocking = False
+    KV, D, bs, lens, budget, recent, sink = 2, 64, 16, [100, 30, 0, 333], 48, 8, 2
+    tables, mb, NB, g = paged(17, lens, bs)
+    k, v, w = (torch.zeros(NB, bs, KV, x, dtype=t, device=DEV) for x, t in ((D, BF), (D, BF), (1, torch.float32)))
+    w = w.view(NB, bs, KV)
+    kept, kept_lens, td, ld = i32([[[0] * budget] * KV] * 4), i32([0] * 4), tables.to(DEV), i32(lens)
+
+    def both():
+        select_kept(r2, w, kept, kept_lens, ld, td, KV, bs, 4, mb, budget, recent, sink)
+        compact_kv_cache(r2, k, v, kept, kept_lens, td, KV, D, bs, 4, mb, weights=w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for _ in range(3):
+        w0, k0, v0 = torch.rand(NB, bs, KV, generator=g), torch.randn(NB, bs, KV, D, generator=g).to(BF), torch.randn(NB, bs, KV, D, generator=g).to(BF)
+        for dst, src in ((w, w0), (k, k0), (v, v0)):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, n in enumerate(lens):
+            at = slots(tables[i], n, bs)
+            for h in range(KV):
+                want = plain_select(w0.view(-1, KV)[at, h].tolist(), n, budget, recent, sink)
+                assert kept[i, h].tolist() == want + [-1] * (budget - len(want))
+                for new, old in ((w, w0), (k, k0), (v, v0)):
+                    assert torch.equal(new.cpu().view(NB * bs, KV, -1)[at[:len(want)], h], old.view(NB * bs, KV, -1)[at[want], h])
+        torch.ones(1000, device=DEV).sum().item()
+
+
 def test_evicting_keeps_what_attention_sees(rt):
     """The operators as they are used: weights accumulate over decode steps, the cache is cut per kv head, and attention
     over the cut cache is attention over the kept rows."""

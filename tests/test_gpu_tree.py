@@ -130,6 +130,40 @@ def test_long_contexts_split_over_workgroups(rt, batch, nodes, context):
     check(run(rt, w), w)
 
 
+@pytest.mark.parametrize("cache", ["same", "int8"])
+@pytest.mark.parametrize("H,KV,lens,clens", [
+    (4, 2, [1, 3, 0, 5, 2] * 14, [37 * i % 200 for i in range(70)]),     # more sequences than a wave has lanes
+    (8, 2, [100] + [1] * 7, [70, 0, 33, 5, 64, 1, 127, 300]),            # one tree of many times the others' rows
+    (8, 2, [200, 0, 2], [40, 3, 500]), (9, 3, [90], [65]),
+    (2, 2, [300], [11])])                                                # rows of mask words that do not fit next to each other
+def test_many_sequences_and_many_rows(rt, H, KV, lens, clens, cache):
+    w = make(6, lens, clens, H, KV, 128, 16, torch.bfloat16, cache)
+    check(run(rt, w), w)
+
+
+@pytest.mark.parametrize("cache", ["same", "int8"])
+def test_less_workspace_gives_the_same_attention_or_an_error(rt, cache):
+    """With less scratch than a shape asks for, another kernel serves it or nothing is launched."""
+    w = make(8, [9, 1, 40], [300, 64, 0], 8, 2, 128, 16, torch.bfloat16, cache)
+    d = W.to_device({k: v for k, v in w.items() if isinstance(v, torch.Tensor)}, DEV)
+    p = lambda n: d[n].data_ptr() if d.get(n) is not None else None  # noqa: E731
+    lib, T, kv = rt._lib, w["qkv"].shape[0], 0 if cache == "same" else 1
+    need = lib.xlite_hip_tree_attention_workspace_bytes(T, 8, 2, 128, 16, 3, w["mb"], kv)
+    served = []
+    for size in (need, need // 2, need // 4, need // 16, 64):
+        ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+        out = torch.full((T, 8 * 128), 7.0, dtype=torch.bfloat16, device=DEV)
+        rc = lib.xlite_hip_tree_attention(rt.stream(), p("qkv"), p("k"), p("v"), out.data_ptr(), p("mask"), w["mask"].shape[1], p("qsl"), p("lens"),
+                                          p("clens"), p("tables"), T, 8, 2, 128, 16, 3, w["mb"], 1, kv, p("ks"), p("vs"), ws.data_ptr(), size)
+        torch.cuda.synchronize()
+        served.append(rc)
+        if rc == 0:
+            check(out.cpu(), w)
+        else:
+            assert b"workspace" in lib.xlite_hip_last_error() and (out == 7.0).all()
+    assert served[0] == 0   # (the prefill kernels run without partials: 64 bytes may be enough)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_any_mask_and_rows_that_see_nothing(rt, D):
     for clens in ([0, 0, 31], [0, 70, 0]):
@@ -278,6 +312,40 @@ def test_verify_paths(rt, dtype, vocab, lens, max_path):
     cnt, nxt = i32([9] * len(lens)), i32([9] * len(lens))
     verify_tree(rt, logits.to(DEV), i32(tokens), i32(parents), acc, cnt, nxt, i32(starts), i32(lens), len(lens))
     assert (acc.cpu().tolist(), cnt.cpu().tolist(), nxt.cpu().tolist()) == want
+
+
+def test_verify_on_another_stream_and_captured():
+    """A captured call on inputs that change between its replays."""
+    from gvirt_amd._C import Runtime, verify_tree
+    r2 = Runtime(0, 8)
+    r2.blocking = False
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    lens, starts, parents = [3, 0, 4], [0, 3, 3], [-1, 0, 0, -1, 0, 1, 1]
+    cases = []
+    for seed in (1, 2, 3):
+        g = torch.Generator().manual_seed(seed)
+        logits, tokens = torch.randn(7, 300, generator=g), torch.randint(0, 300, (7,), generator=g)
+        tokens[1 + seed % 2], tokens[4] = logits[0].argmax(), logits[3].argmax()
+        cases.append((logits, tokens, plain_verify(logits.double(), tokens.tolist(), parents, starts, lens, 3)))
+    logits, tokens = cases[0][0].to(DEV), cases[0][1].int().to(DEV)
+    acc, cnt, nxt, par, s0, n = i32([[9] * 3] * 3), i32([9] * 3), i32([9] * 3), i32(parents), i32(starts), i32(lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        verify_tree(r2, logits, tokens, par, acc, cnt, nxt, s0, n, 3)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert (acc.tolist(), cnt.tolist(), nxt.tolist()) == cases[0][2]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        verify_tree(r2, logits, tokens, par, acc, cnt, nxt, s0, n, 3)
+    for x, t, want in cases[::-1]:
+        logits.copy_(x)
+        tokens.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (acc.tolist(), cnt.tolist(), nxt.tolist()) == want
+        torch.ones(1000, device=DEV).sum().item()
 
 
 def test_verify_ignores_parents_that_do_not_stand_before_their_child(rt):
