@@ -785,8 +785,8 @@ def select_kept(rt: Runtime, weights: torch.Tensor, kept: torch.Tensor, kept_len
                 recent: int, sink: int = 0) -> None:
     """Which positions a cache keeps (not part of the reference API): per sequence and kv head the first `sink`, the last
     `recent` and the largest `weights` of the rest, `budget` in all (everything, if it fits; equal weights: the lower
-    position). `kept` [batch, n_kv_heads, budget] gets ascending positions, then -1, `kept_lens` [batch] their number:
-    the lists of `compact_kv_cache`."""
+    position). `kept` [batch, n_kv_heads, budget] gets ascending positions, then -1, `kept_lens` [batch] (not the tensor
+    of `context_lens`) their number: the lists of `compact_kv_cache`."""
     name = "select_kept"
     _req(n_kv_heads > 0 and block_size > 0, "select_kept: n_kv_heads and block_size must be positive")
     _on(rt, name, "weights", weights, torch.float32)

@@ -33,6 +33,8 @@ struct AttentionArgs {
 };
 enum { kAllRows = 0, kOnlySingle = 1, kSkipSingle = 2 };
 
+inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 // the low n bits (none below 0, all from 32 on)
 __device__ __forceinline__ uint32_t ones(int32_t n)
 {

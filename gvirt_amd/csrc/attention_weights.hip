@@ -1127,6 +1127,7 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
     XL_REQUIRE(kv_dtype == XLITE_HIP_KV_SAME || head_dim != 256, "quantised KV caches: head_dim must be 64 or 128");
     XL_REQUIRE(static_cast<uint64_t>(total_tokens) * n_heads < (1ull << 31) && batch <= 65535 && n_kv_heads <= 65535,
                "more rows than one launch takes");
+    XL_REQUIRE(aligned16(qkv) && aligned16(k_cache) && aligned16(workspace), "qkv, k_cache and workspace must be aligned to 16 bytes");
     const Plan plan = plan_of(total_tokens, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, window);
     if (workspace == nullptr || workspace_bytes < plan.bytes) {
         return fail(XLITE_HIP_ENOSPC, __func__, "workspace too small: need " + std::to_string(plan.bytes) + " bytes, have " +

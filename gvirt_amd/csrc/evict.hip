@@ -431,6 +431,8 @@ extern "C" int xlite_hip_select_kept(void *stream, const float *weights, int32_t
     XL_REQUIRE(budget > 0 && budget < (1u << 31), "budget must be positive");
     XL_REQUIRE(static_cast<uint64_t>(recent) + sink <= budget, "recent + sink must not exceed budget");
     XL_REQUIRE((static_cast<uint64_t>(batch) + kXcds) * n_kv_heads < (1ull << 31), "more lists than one launch takes");
+    // (the list of one head is written while the others still read the lengths)
+    XL_REQUIRE(kept_lens != context_lens, "kept_lens must not be context_lens");
     SelectParams p{weights, kept, kept_lens, context_lens, block_tables, n_kv_heads, block_size, max_num_block,
                    budget, recent, sink, batch, magic_of(block_size, max_num_block)};
     const uint64_t grid = (static_cast<uint64_t>(batch) + kXcds - 1) / kXcds * kXcds * n_kv_heads;
@@ -473,8 +475,7 @@ extern "C" int xlite_hip_compact_kv_cache(void *stream, void *k_cache, void *v_c
     XL_REQUIRE(static_cast<uint64_t>(max_num_block) * block_size < (1ull << 31), "block tables reach beyond 2^31 positions");
     const uint64_t head_bytes = static_cast<uint64_t>(head_dim) * (kv_dtype == XLITE_HIP_KV_SAME ? 2 : 1);
     XL_REQUIRE(head_bytes % 16 == 0, "a kv head's row must be a multiple of 16 bytes");
-    XL_REQUIRE((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) % 16 == 0,
-               "caches must be aligned to 16 bytes");
+    XL_REQUIRE(aligned16(k_cache) && aligned16(v_cache), "caches must be aligned to 16 bytes");
     CompactParams p{};
     p.k_cache = static_cast<unsigned char *>(k_cache);
     p.v_cache = static_cast<unsigned char *>(v_cache);

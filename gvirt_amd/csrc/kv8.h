@@ -1,5 +1,5 @@
 // Dequantisation of 8-bit cache values, shared by the copy that serves the 16-bit kernels (kv_dequant.hip) and by the
-// prefill kernel that reads quantised caches itself (prefill_mfma.hip): the same code, so the two give the same bits.
+// kernels that read quantised caches themselves (prefill_mfma.hip, tree_stream.hip): the same code, so they give the same bits.
 #pragma once
 
 #include <type_traits>

@@ -66,13 +66,15 @@ extern "C" int xlite_hip_tree_attention(void *stream, const void *qkv, const voi
                "n_heads must be a positive multiple of n_kv_heads");
     XL_REQUIRE(block_size > 0 && max_num_block > 0, "block_size and max_num_block must be positive");
     XL_REQUIRE(static_cast<uint64_t>(max_num_block) * block_size < (1ull << 31), "block tables reach beyond 2^31 positions");
-    XL_REQUIRE(mask_words > 0 && mask_words <= (1u << 26), "mask_words must be positive");
+    XL_REQUIRE(mask_words > 0 && mask_words <= (1u << 22), "mask_words must be positive, at most 2^22");
     XL_REQUIRE(mfma_gqa_supported(head_dim), "head_dim must be 64, 128 or 256");
     XL_REQUIRE(static_cast<uint64_t>(total_tokens) * n_heads < (1ull << 31) &&
                    ceil_div(total_tokens * (n_heads / n_kv_heads), 128u) + batch <= 65535 && n_kv_heads <= 65535,
                "more rows than one launch takes");
     XL_REQUIRE(kv_dtype == XLITE_HIP_KV_SAME || (k_scale && v_scale), "a quantised KV cache needs k_scale and v_scale");
     XL_REQUIRE(kv_dtype == XLITE_HIP_KV_SAME || head_dim != 256, "quantised KV caches: head_dim must be 64 or 128");
+    XL_REQUIRE(aligned16(qkv) && aligned16(k_cache) && aligned16(v_cache) && aligned16(output) && aligned16(workspace),
+               "qkv, caches, output and workspace must be aligned to 16 bytes");
     AttentionArgs a{qkv, k_cache, v_cache, output, query_start_loc, lens, cached_lens, block_tables,
                     total_tokens, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block,
                     dtype, kv_dtype, k_scale, v_scale, workspace, workspace_bytes};

@@ -456,10 +456,11 @@ int xlite_hip_prepare_tree(const uint32_t *lens, const uint32_t *cached_lens, co
  * 0 .. cached_lens[i] - 1 and, of the step's own positions cached_lens[i] + n (n < lens[i]), those
  * whose bit n is set in its row of tree_mask [total_tokens, mask_words] (any mask: not only
  * ancestors; bits from lens[i] on are ignored, nodes from 32 * mask_words on are seen by nobody).
- * A row that sees nothing gets zeros. Infinities and NaNs in rows that a row does not see do not
+ * mask_words <= 2^22. A row that sees nothing gets zeros. Infinities and NaNs in rows that a row does not see do not
  * reach it. Everything else as in xlite_hip_attention (quantised caches: head_dim 64 or 128).
- * workspace: xlite_hip_tree_attention_workspace_bytes(); with less the KV axis is not split
- * (a batch over a quantised cache that needs a 16-bit copy fails with XLITE_HIP_ENOSPC).
+ * workspace: xlite_hip_tree_attention_workspace_bytes(); with less another kernel serves the
+ * batch, in the end without splitting the KV axis (one over a quantised cache that needs a 16-bit
+ * copy fails with XLITE_HIP_ENOSPC). qkv, caches, output and workspace: aligned to 16 bytes.
  * ---------------------------------------------------------------------- */
 size_t xlite_hip_tree_attention_workspace_bytes(uint32_t total_tokens, uint32_t n_heads,
                                                 uint32_t n_kv_heads, uint32_t head_dim,
@@ -503,6 +504,7 @@ int xlite_hip_verify_tree(void *stream, const void *logits, const int32_t *token
  * Sums are fp32, in the same order in every run. A block may stand in one sequence's table only.
  * Sequences without rows are left as they are. 16-bit caches, or quantised ones (K bytes and
  * k_scale, head_dim 64 or 128). workspace: xlite_hip_attention_weights_workspace_bytes() (required).
+ * qkv, k_cache and workspace: aligned to 16 bytes.
  * ---------------------------------------------------------------------- */
 size_t xlite_hip_attention_weights_workspace_bytes(uint32_t total_tokens, uint32_t n_heads,
                                                    uint32_t n_kv_heads, uint32_t head_dim,
@@ -522,7 +524,7 @@ int xlite_hip_attention_weights(void *stream, const void *qkv, const void *k_cac
  * `recent` and, of those between, the budget - sink - recent with the largest weights (NaN counts as
  * the largest; equal weights: the lower position). recent + sink <= budget.
  * kept      [batch, n_kv_heads, budget]: positions in ascending order, then -1
- * kept_lens [batch] = min(context_lens, budget)
+ * kept_lens [batch] = min(context_lens, budget); not the tensor of context_lens
  * ---------------------------------------------------------------------- */
 int xlite_hip_select_kept(void *stream, const float *weights, int32_t *kept, int32_t *kept_lens,
                           const int32_t *context_lens, const int32_t *block_tables, uint32_t n_kv_heads,

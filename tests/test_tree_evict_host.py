@@ -96,6 +96,19 @@ BAD = [
 ]
 
 
+def test_c_entry_points_refuse_what_they_could_not_read():
+    """Tensors off their alignment, a mask longer than any tree, lengths that the call itself would overwrite."""
+    lib = _lib.load()
+    off = ctypes.c_void_p((1 << 20) + 8)
+    for name, good, bads, why in (("tree_attention", TREE, [dict(qkv=off), dict(k=off), dict(v=off), dict(out=off), dict(ws=off, ws_bytes=64)], b"aligned"),
+                                  ("tree_attention", TREE, [dict(words=(1 << 22) + 1)], b"mask_words"),
+                                  ("attention_weights", WEIGHTS, [dict(qkv=off), dict(k=off), dict(ws=off)], b"aligned"),
+                                  ("select_kept", SELECT, [dict()], b"context_lens")):
+        for bad in bads:
+            assert getattr(lib, "xlite_hip_" + name)(*dict(good, **bad).values()) < 0, bad
+            assert why in lib.xlite_hip_last_error(), (bad, lib.xlite_hip_last_error())
+
+
 @pytest.mark.parametrize("name,good,bads", BAD, ids=[b[0] for b in BAD])
 def test_c_entry_points_refuse(name, good, bads):
     lib = _lib.load()
