@@ -21,6 +21,7 @@ namespace {
 // chain of a workgroup's steps (loads through the block table 12 us, three histograms 10, ballots 3, output 4) and that only
 // two workgroups' keys fit a compute unit, so that little of one list's chain hides behind another's.
 constexpr uint32_t kXcds = 8;
+constexpr uint32_t kSelTable = 4096;   // block-table entries in LDS
 constexpr int kAhead = 16;   // loads a thread has under way
 
 // weights in the order of a descending sort: NaN first, -0 and +0 alike; never 0, which stands for "no weight"
@@ -119,13 +120,14 @@ __device__ __forceinline__ void nth_largest(EACH &&each, uint32_t n, SelectScrat
     *equal = left;
 }
 
-// T threads. KPT: keys a thread holds in registers (the judged positions fit KPT * T); 0: any length, the keys are read again
-// in every pass
+// T threads. KPT: keys a thread holds in registers (the judged positions fit KPT * T, the block table kSelTable; block_magic
+// is there); 0: any length, the keys are read again in every pass
 template <int KPT, int T>
 __global__ void __launch_bounds__(T, KPT == 64 ? 4 : 1)
 select_kept_kernel(const SelectParams p)
 {
     __shared__ SelectScratch<T> scratch;
+    __shared__ uint32_t table_lds[KPT > 0 ? kSelTable : 1];
     __shared__ uint2 counts[(KPT > 0 ? KPT : kAhead) * (T / 64)];   // (above, equal) of a wave's 64 positions, then the sums before them
     const uint32_t xcd = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
     const uint32_t seq = place / p.n_kv_heads * kXcds + xcd, kvh = place % p.n_kv_heads;
@@ -149,9 +151,16 @@ select_kept_kernel(const SelectParams p)
         return;
     }
     const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
+    if constexpr (KPT > 0) {
+        for (uint32_t i = threadIdx.x; i < ceil_div(length, p.block_size); i += T) {
+            table_lds[i] = static_cast<uint32_t>(table[i]);
+        }
+        __syncthreads();
+    }
     auto key_at = [&](uint32_t pos) {
-        const uint32_t b = p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size;
-        const uint64_t slot = static_cast<uint64_t>(static_cast<uint32_t>(table[b])) * p.block_size + (pos - b * p.block_size);
+        const uint32_t b = KPT > 0 || p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size;
+        const uint32_t entry = KPT > 0 ? table_lds[b] : static_cast<uint32_t>(table[b]);
+        const uint64_t slot = static_cast<uint64_t>(entry) * p.block_size + (pos - b * p.block_size);
         return weight_key(p.weights[slot * p.n_kv_heads + kvh]);
     };
     const uint32_t lo = p.sink, hi = length - p.recent;   // the judged positions
@@ -168,30 +177,45 @@ select_kept_kernel(const SelectParams p)
     const uint64_t below = (1ull << lane) - 1;
     uint32_t threshold, equal;
     if constexpr (KPT > 0) {
+        // A quarter of the keys at a time, as far as the list reaches: f(j) for the keys of the quarters it has, rest(j) for the others.
+        constexpr int QUARTER = KPT / 4;
+        auto quarters = [&](auto &&f, auto &&rest) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                if (lo + g * QUARTER * T < hi) {
+#pragma unroll
+                    for (int j = g * QUARTER; j < (g + 1) * QUARTER; j++) {
+                        f(j);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = g * QUARTER; j < (g + 1) * QUARTER; j++) {
+                        rest(j);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);   // (all of a thread's loads under way: their addresses would take the keys' registers)
+            }
+        };
+        auto nothing = [](int) {};
         uint32_t key[KPT];
-#pragma unroll
-        for (int j = 0; j < KPT; j++) {
+        quarters([&](int j) {
             const uint32_t i = lo + j * T + threadIdx.x;
-            key[j] = key_at(min(i, hi - 1));
-            key[j] = i < hi ? key[j] : 0u;
-            if (j % kAhead == kAhead - 1) {   // with all of them under way their addresses would take the keys' registers
-                __builtin_amdgcn_sched_barrier(0);
-                asm volatile("" ::: "memory");
-            }
-        }
+            const uint32_t k = key_at(min(i, hi - 1));
+            key[j] = i < hi ? k : 0u;
+        }, [&](int j) { key[j] = 0; });
         nth_largest<T>([&](auto &&f) {
-#pragma unroll
-            for (int j = 0; j < KPT; j++) {
-                f(key[j]);
-            }
+            quarters([&](int j) { f(key[j]); }, nothing);
         }, n, scratch, &threshold, &equal);
-#pragma unroll
-        for (int j = 0; j < KPT; j++) {
+        quarters([&](int j) {
             const uint64_t a = __ballot(key[j] > threshold), e = __ballot(key[j] == threshold);
             if (lane == 0) {
                 counts[j * (T / 64) + wave] = make_uint2(__builtin_popcountll(a), __builtin_popcountll(e));
             }
-        }
+        }, [&](int j) {
+            if (lane == 0) {
+                counts[j * (T / 64) + wave] = make_uint2(0, 0);
+            }
+        });
         __syncthreads();
         if (wave == 0) {   // exclusive sums in position order: lane l owns KPT / 4 consecutive entries
             constexpr int PER = (KPT * (T / 64) + 63) / 64;
@@ -222,8 +246,7 @@ select_kept_kernel(const SelectParams p)
         // compared and counted anew below: kept over the barrier the ballots and positions take more registers than the keys
         uint32_t first = lo + threadIdx.x;
         asm volatile("" : "+v"(threshold), "+v"(first));
-#pragma unroll
-        for (int j = 0; j < KPT; j++) {
+        quarters([&](int j) {
             const bool is_above = key[j] > threshold, is_equal = key[j] == threshold;
             const uint64_t am = __ballot(is_above), em = __ballot(is_equal);
             const uint2 before = counts[j * (T / 64) + wave];
@@ -231,7 +254,7 @@ select_kept_kernel(const SelectParams p)
             if (is_above || (is_equal && e < equal)) {
                 out[p.sink + a + min(e, equal)] = static_cast<int32_t>(first + j * T);
             }
-        }
+        }, nothing);
     } else {
         nth_largest<T>([&](auto &&f) {
             for (uint32_t i0 = lo + threadIdx.x; i0 < hi; i0 += kAhead * T) {
@@ -443,7 +466,10 @@ extern "C" int xlite_hip_select_kept(void *stream, const float *weights, int32_t
     // up to 32768, where two workgroups share a compute unit (64 lists of 8 heads x 32768: 58 us; 1024 threads with 40 keys
     // and one workgroup 70); 1024 beyond (64000: 118 us); reading the keys again in every pass costs 413 there with a load at
     // a time and remains for what no workgroup can hold (100000: 496 with 16 under way).
-    if (judged <= 4 * 1024) {
+    const bool registers = max_num_block <= kSelTable && p.block_magic != 0;
+    if (!registers) {
+        select_kept_kernel<0, 1024><<<g, 1024, 0, s>>>(p);
+    } else if (judged <= 4 * 1024) {
         select_kept_kernel<4, 1024><<<g, 1024, 0, s>>>(p);
     } else if (judged <= 16 * 1024) {
         select_kept_kernel<16, 1024><<<g, 1024, 0, s>>>(p);
