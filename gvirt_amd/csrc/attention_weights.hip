@@ -6,11 +6,14 @@
 // A batch of few rows per sequence (decode steps, short windows) is bound by reading K: the scores are formed once, stored in
 // fp32 (a few per cent of the bytes of K) with every row's maximum and sum per chunk of positions, and summed up in a second
 // pass over them. A batch of many rows is bound by the exponentials and forms the scores twice instead of storing them (a
-// chunk of 2048 rows behind 6144 positions has 0.9 G of them, 3.7 GB in fp32):
+// chunk of 2048 rows behind 6144 positions has 0.4 G of them for 28 heads, 1.6 GB in fp32):
 //   row statistics: log2 of every row's normaliser. A wave owns 64 M rows (an M row: a counted row and one query head of the
 //     kv head) as the columns of S^T = K Q^T, so a row's running maximum and sum live in one lane pair.
 //   column sums: a wave owns 64 positions as the columns of S = Q K^T and walks the M rows, so a position's sum lives in one
 //     lane pair: no atomics, one owner per weight, the same order of additions in every run.
+// Measured, 2 chunks of 2048 rows behind 6144 positions, 28 heads over 4 of 128 elements (210 GFLOP of scores, formed twice): row
+// statistics 245 us, column sums 300, together 0.77 PFLOP/s (a large bf16 product reaches 1.28): the matrix instructions share
+// the SIMDs with 0.8 G exponentials a pass.
 #include <algorithm>
 #include <type_traits>
 

@@ -16,10 +16,11 @@ namespace {
 // does not depend on any order. One workgroup per (sequence, kv head); the keys are read once, into registers.
 // A weight's neighbours in memory belong to the other kv heads: the heads of a sequence run on one XCD, at the same time, so
 // that its lines come from memory once and from that XCD's L2 for the other heads.
-// Measured, 64 sequences x 8 heads, an eighth kept: 15 us over 4000 positions, 34 over 16000, 61 over 32000, 118 over 64000;
-// one sequence of 32000 37 us. The weights of 64 x 32768 positions are 67 MB, 13 us at the rate of a copy: what bounds it is the
-// chain of a workgroup's steps (loads through the block table 12 us, three histograms 10, ballots 3, output 4) and that only
-// two workgroups' keys fit a compute unit, so that little of one list's chain hides behind another's.
+// Measured, 64 sequences x 8 heads, an eighth kept: 16 us over 4000 positions, 32 over 16000, 58 over 32000, 114 over 64000;
+// one sequence of 32000 34 us. The weights of 64 x 32768 positions are 67 MB, 13 us at the rate of a copy. What bounds it: a wave's
+// keys lie 32 bytes apart, so that a list takes eight times its bytes out of L2 (27 us of the 58 with two lists a compute unit);
+// the histograms take 11, the ballots 3, the output 5, and only two lists' keys fit a compute unit's registers. Two heads a
+// workgroup in neighbouring lanes fetch half the lines: 57 us, but 47 instead of 34 for one sequence.
 constexpr uint32_t kXcds = 8;
 constexpr uint32_t kSelTable = 4096;   // block-table entries in LDS
 constexpr int kAhead = 16;   // loads a thread has under way
@@ -315,7 +316,9 @@ select_kept_kernel(const SelectParams p)
 // row are independent, so a workgroup owns a slice of the rows' bytes (or one fp32 per row: scales, weights) and walks the
 // list in order, a batch of entries at a time: all of a batch is read before any of it is written (a barrier), and what later
 // batches read lies above everything written so far (kept[i] >= i), so the next batch is read ahead of that barrier. Bound
-// by memory: every moved row is read and written once.
+// by memory: every moved row is read and written once. Measured: 16 sequences of 8192 positions cut to 2048 per head of 8 (128
+// elements of 16 bits, and the weights), 135 MB moved: 61 us, 4.4 TB/s read and written; 64 paths of 6 rows 6 us. Rows of 256
+// bytes of one head are scattered over pages: a plain copy of as many bytes takes 52 us.
 constexpr int kMoveUnroll = 4;
 constexpr uint32_t kMoveTable = 4096;   // block-table entries kept in LDS (longer tables are read from memory)
 
@@ -463,9 +466,9 @@ extern "C" int xlite_hip_select_kept(void *stream, const float *weights, int32_t
     hipStream_t s = as_stream(stream);
     const dim3 g(static_cast<uint32_t>(grid));
     // The fewest keys a thread that hold the longest list: keys beyond a list's end cost their step all the same. 512 threads
-    // up to 32768, where two workgroups share a compute unit (64 lists of 8 heads x 32768: 58 us; 1024 threads with 40 keys
-    // and one workgroup 70); 1024 beyond (64000: 118 us); reading the keys again in every pass costs 413 there with a load at
-    // a time and remains for what no workgroup can hold (100000: 496 with 16 under way).
+    // up to 32768, where two workgroups share a compute unit (64 x 8 lists of 32000: 58 us; 1024 threads with 40 keys
+    // and one workgroup 70); 1024 beyond (64000: 114 us). Reading the keys again in every pass costs 413 there with a load at a
+    // time; it remains for what no workgroup can hold (100000: 490 with 16 under way) and for tables that do not fit LDS.
     const bool registers = max_num_block <= kSelTable && p.block_magic != 0;
     if (!registers) {
         select_kept_kernel<0, 1024><<<g, 1024, 0, s>>>(p);

@@ -1,4 +1,4 @@
-// Attention over drafted trees for head_dim 128 and 16-bit caches: the cache streamed once, past all rows of a tree.
+// Attention over drafted trees for head_dim 128: the cache streamed once, past all rows of a tree.
 //
 // A tree has few rows (nodes x query heads of a kv head: an M row each), so its attention is bound by reading K and V. The
 // prefill kernel gives a workgroup one kv head: its copies are 256-byte rows up to two kilobytes apart, which memory serves
@@ -8,7 +8,15 @@
 //     S^T[pos][m]  = K[pos][:] . Q[m][:]           v_mfma_f32_32x32x16 (A = K rows, ds_read_b128; B = Q)
 //     O^T[d][m]   += V^T[d][pos] . P^T[pos][m]     v_mfma_f32_32x32x16 (A = V^T, ds_read_b64_tr_b16; B = P)
 // Four stages of 32 KiB: one is consumed while three are on their way (with two of 64 KiB half of what memory delivers in a
-// round trip was not asked for: 447 against XXX us for 64 trees of 32 over 8192 positions).
+// round trip was not asked for: 447 against 385 us for 64 trees of 32 over 8192 positions).
+// Caches of bytes: raw bytes are copied four steps ahead (18 KiB each with their scales) and widened to fp16 x scale into one of
+// two stages; from there on the kernel is the same.
+//
+// Bound by memory where trees are small next to their contexts. Measured: 64 trees of 32 nodes over 8192 positions, 8 kv heads of
+// 4, 2.19 GB: 385 us, 5.7 TB/s (the prefill kernel 514); 16 ragged trees of up to 27 over up to 4096, 170 MB: 42 us and 11 of
+// merging. 8 trees of up to 16 over up to 16384 int8 positions, 97 MB: 57 us and 10 of merging (the prefill kernel 80); there the
+// widening (120 vector instructions per 16 KiB and wave) next to scores, softmax and products fills the vector units. With the
+// products of one half of the waves beside the widening of the other half the time was the same.
 //
 // Work split: a sequence owns ceil(len G / rows) M tiles of ceil((cached + len) / step) steps each; the steps of all M tiles laid
 // end to end are cut into equal chunks, one per workgroup, whatever the sequences' lengths (they live in device memory: every
@@ -228,7 +236,7 @@ tree_stream_kernel(const StreamParams p)
             const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
             const uint32_t blk0 = t0 / p.block_size, blk1 = (t1 - 1) / p.block_size;
 
-            // ---- set-up: block-table entries, then the query rows, then the first two steps' copies
+            // ---- set-up: block-table entries, then the query rows, then the first steps' copies
             __syncthreads();   // (the table and the stages of the last segment have been read)
             const uint32_t n_blk = blk1 - blk0 + 1;
             // the mask's rows of the M tile, for a segment that reaches into the tree

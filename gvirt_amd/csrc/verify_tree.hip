@@ -1,5 +1,10 @@
 // Which path of a drafted tree the model itself takes (greedy): from node 0 on, the token of the largest logit of the node's
 // row; if a child carries that token the path goes on there, otherwise the token is the sequence's next one.
+// The path is not known before its logits are read, one row after the other. A few rows are all read at once by as many
+// workgroups as there is room for and the walk only compares what they found (a tree of 8 over 32000 logits: 3.3 us and 3.2 us
+// of walking, launch-bound); many rows would be mostly rows off the path, so that a workgroup per sequence reads those of
+// its path (64 trees of up to 32 over 131072 16-bit logits, paths of up to 4, 64 MB: 23 us, 2.8 TB/s; 64 of the 256 compute units
+// are at work, each in dependent trips to memory; reading all 1047 rows, 274 MB, would take 43).
 #include <algorithm>
 
 #include "attention_common.h"
@@ -263,7 +268,7 @@ walk_rows_kernel(const VerifyParams p)
 }
 
 // Up to so many rows all of them are read, by as many workgroups as there is room for; beyond, each sequence's workgroup
-// reads the rows of its path one after the other.
+// reads the rows of its path one after the other (384 rows of 131072 logits are 100 MB, 16 us, as long as a path of three).
 constexpr uint32_t kAllRows = 384;
 uint32_t parts_per_row(uint32_t rows)
 {
