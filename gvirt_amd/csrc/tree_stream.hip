@@ -8,13 +8,13 @@
 //     S^T[pos][m]  = K[pos][:] . Q[m][:]           v_mfma_f32_32x32x16 (A = K rows, ds_read_b128; B = Q)
 //     O^T[d][m]   += V^T[d][pos] . P^T[pos][m]     v_mfma_f32_32x32x16 (A = V^T, ds_read_b64_tr_b16; B = P)
 // Four stages of 32 KiB: one is consumed while three are on their way (with two of 64 KiB half of what memory delivers in a
-// round trip was not asked for: 447 against 385 us for 64 trees of 32 over 8192 positions).
+// round trip was not asked for: 447 against 385-405 us for 64 trees of 32 over 8192 positions).
 // Caches of bytes: raw bytes are copied four steps ahead (18 KiB each with their scales) and widened to fp16 x scale into one of
 // two stages; from there on the kernel is the same.
 //
 // Bound by memory where trees are small next to their contexts. Measured: 64 trees of 32 nodes over 8192 positions, 8 kv heads of
-// 4, 2.19 GB: 385 us, 5.7 TB/s (the prefill kernel 514); 16 ragged trees of up to 27 over up to 4096, 170 MB: 42 us and 11 of
-// merging. 8 trees of up to 16 over up to 16384 int8 positions, 97 MB: 57 us and 10 of merging (the prefill kernel 80); there the
+// 4, 2.19 GB: 385-405 us, 5.4-5.7 TB/s (the prefill kernel 514); 16 ragged trees of up to 27 over up to 4096, 170 MB: 49 us and
+// 8 of merging. 8 trees of up to 16 over up to 16384 int8 positions, 97 MB: 57 us and 10 of merging (the prefill kernel 80); there the
 // widening (120 vector instructions per 16 KiB and wave) next to scores, softmax and products fills the vector units. With the
 // products of one half of the waves beside the widening of the other half the time was the same.
 //
