@@ -194,8 +194,8 @@ size_t prefill_mfma_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uin
 // tree_stream.hip
 bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
                            uint32_t max_num_block, int kv_dtype);
-size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t batch, uint32_t block_size,
-                                   uint32_t max_num_block);
+size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t batch,
+                                   uint32_t block_size, uint32_t max_num_block);
 int launch_tree_stream(hipStream_t stream, const AttentionArgs &a);
 
 // kv_dequant.hip: the 16-bit copy of a quantised cache's visible blocks, at the front of the workspace

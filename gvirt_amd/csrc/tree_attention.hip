@@ -2,7 +2,8 @@
 // nodes of one drafted tree per sequence, already written to the cache behind the cached positions; a row sees every
 // cached position and those nodes whose bit its mask has:
 //     out_r = sum_j [seen(r, j)] exp(q_r . k_j) v_j / sum_j [seen(r, j)] exp(q_r . k_j),   0 where nothing is seen.
-// head_dim 128: a kernel of its own that streams the cache past all rows of a tree (tree_stream.hip).
+// head_dim 128, and 64 over caches of bytes: a kernel of its own that streams the cache past all rows of a tree
+// (tree_stream.hip).
 // Other shapes: the walk is that of a prefill chunk with another mask, and only tiles that reach into the tree look at it, so
 // the prefill kernels serve them with a mask of their own (prefill_mfma.hip, mfma_attention.hip: TREE).
 #include <algorithm>
@@ -38,7 +39,7 @@ extern "C" size_t xlite_hip_tree_attention_workspace_bytes(uint32_t total_tokens
     }
     size_t need = tree_bytes_16(total_tokens, n_heads, n_kv_heads, head_dim, batch, max_num_block * block_size);
     if (tree_stream_supported(n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, kv_dtype)) {
-        need = std::max(need, tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, batch, block_size, max_num_block));
+        need = std::max(need, tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, head_dim, batch, block_size, max_num_block));
     }
     if (kv_dtype != XLITE_HIP_KV_SAME) {
         need += kv_dequant_bytes(n_kv_heads, head_dim, block_size, batch, max_num_block);
@@ -82,7 +83,7 @@ extern "C" int xlite_hip_tree_attention(void *stream, const void *qkv, const voi
     a.mask_words = mask_words;
     hipStream_t s = as_stream(stream);
     if (tree_stream_supported(n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, kv_dtype) && workspace != nullptr &&
-        workspace_bytes >= tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, batch, block_size, max_num_block)) {
+        workspace_bytes >= tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, head_dim, batch, block_size, max_num_block)) {
         return launch_tree_stream(s, a);
     }
     if (kv_dtype == XLITE_HIP_KV_SAME) {

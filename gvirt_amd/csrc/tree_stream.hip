@@ -9,14 +9,15 @@
 //     O^T[d][m]   += V^T[d][pos] . P^T[pos][m]     v_mfma_f32_32x32x16 (A = V^T, ds_read_b64_tr_b16; B = P)
 // Four stages of 32 KiB: one is consumed while three are on their way (with two of 64 KiB half of what memory delivers in a
 // round trip was not asked for: 447 against 385-405 us for 64 trees of 32 over 8192 positions).
-// Caches of bytes: raw bytes are copied four steps ahead (18 KiB each with their scales) and widened to fp16 x scale into one of
-// two stages; from there on the kernel is the same.
+// Caches of bytes: raw bytes are copied four steps ahead (18 KiB each with their scales) and widened to fp16 into one of two
+// stages; the scales join the scores. With the scales multiplied into fp16 rows an fp16 result was off by 5.5-8 e-4 of its size
+// instead of 2.1 e-4 (its own rounding).
 //
 // Bound by memory where trees are small next to their contexts. Measured: 64 trees of 32 nodes over 8192 positions, 8 kv heads of
 // 4, 2.19 GB: 385-405 us, 5.4-5.7 TB/s (the prefill kernel 514); 16 ragged trees of up to 27 over up to 4096, 170 MB: 49 us and
-// 8 of merging. 8 trees of up to 16 over up to 16384 int8 positions, 97 MB: 57 us and 10 of merging (the prefill kernel 80); there the
-// widening (120 vector instructions per 16 KiB and wave) next to scores, softmax and products fills the vector units. With the
-// products of one half of the waves beside the widening of the other half the time was the same.
+// 8 of merging. 8 trees of up to 16 over up to 16384 int8 positions, 97 MB: 57 us and 10 of merging (the prefill kernel 80): 2 us a
+// step of 16 KiB, the chain of widening, barrier, operands, scores, softmax and products of two waves a SIMD. Half the vector
+// instructions for widening, or the products of one half of the waves beside the widening of the other: the same time.
 //
 // Work split: a sequence owns ceil(len G / rows) M tiles of ceil((cached + len) / step) steps each; the steps of all M tiles laid
 // end to end are cut into equal chunks, one per workgroup, whatever the sequences' lengths (they live in device memory: every
@@ -36,7 +37,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 2.0f / kLog2e;   // the reference maximum moves when a score exceeds it by a factor of 4
-constexpr int D = 128;
+constexpr int kRow = 128;                        // elements of a row in LDS
 constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * 64;
 constexpr uint32_t kHalf = 16 * 1024;            // K or V of a stage: 32 positions of two kv heads, 64 of one
@@ -46,8 +47,10 @@ constexpr uint32_t kRows = 32 * kWaves / NH;     // M rows of a workgroup, per k
 constexpr uint32_t kStage = 2 * kHalf;
 constexpr uint32_t kWaveRaw = 2 * 1024 + 256;    // caches of bytes: what a wave copies in a step, 8 rows of K and of V and their scales
 constexpr uint32_t kRawStage = kWaves * kWaveRaw;
+constexpr uint32_t kScales = 3 * 64 * 4;         // of a widened stage: three numbers per (kv head, position)
 template <bool KV8>
-constexpr uint32_t kStageBytes = KV8 ? 2 * kStage + kStages * kRawStage : kStages * kStage;
+constexpr uint32_t kStageBytes = KV8 ? 2 * (kStage + kScales) + kStages * kRawStage : kStages * kStage;
+constexpr float kLeastScale = 0x1p-100f;         // of a V row, in the arithmetic of its logarithm and reciprocal
 constexpr uint32_t kTblCap = 2048;               // block-table entries staged per segment
 constexpr uint32_t kSeqCap = 1024;               // sequences whose prefix sums fit
 constexpr uint32_t kMaskCap = kThreads;          // mask words of an M tile kept in LDS: 128 rows of 4 heads and 512 nodes
@@ -98,12 +101,13 @@ __device__ __forceinline__ uint32_t uni(uint32_t x)
 }
 
 // NH: kv heads of a workgroup. T: the type of the products; TIO: of the query rows and the output (the same, or bf16 with fp16
-// products over caches of bytes, KVF).
-template <typename T, int NH, int KVF, typename TIO>
+// products over caches of bytes, KVF). D: 128, or 64 over caches of bytes (half of a row in LDS is not used then).
+template <typename T, int NH, int KVF, typename TIO, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_stream_kernel(const StreamParams p)
 {
     constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
+    static_assert(D == 128 || (D == 64 && KV8), "head_dim 128, or 64 over caches of bytes");
     constexpr int KS = D / 16, DT = D / 32;
     constexpr uint32_t ROWS = kRows<NH>;
     constexpr uint32_t POSB = NH * 256;          // LDS bytes of a position
@@ -182,12 +186,12 @@ tree_stream_kernel(const StreamParams p)
 
     // ---- read roles (the pattern of position p + 32 is that of p)
     const uint32_t k_off = col * POSB + hsel * 256;
-    const uint32_t kx = (half ^ stage::pattern<D>(col)) << 4;
+    const uint32_t kx = (half ^ stage::pattern<kRow>(col)) << 4;
     uint32_t v_off;
     {
         const uint32_t g = lane >> 4, jp = (lane & 15) >> 2, q = lane & 3;
         const uint32_t y = 2 * (g & 1) + (q >> 1), pos = 4 * (g >> 1) + jp;
-        v_off = kHalf + pos * POSB + hsel * 256 + ((y ^ stage::pattern<D>(pos)) << 4) + ((q & 1) << 3);
+        v_off = kHalf + pos * POSB + hsel * 256 + ((y ^ stage::pattern<kRow>(pos)) << 4) + ((q & 1) << 3);
     }
     // ---- copy role: wave w fills copies 2 w and 2 w + 1 of the K and of the V half. Lane l of a copy: row l / 16 of its four
     // (position, kv head) rows, chunk slot l % 16, which receives chunk slot ^ pattern(position)
@@ -292,7 +296,7 @@ tree_stream_kernel(const StreamParams p)
                 const uint32_t c_rel = (l >> 4) / NH, c_head = (l >> 4) % NH;
                 auto c_off = [&](int i) __attribute__((always_inline)) {
                     const uint32_t pos = (CPW * wave + i) * PPI + c_rel;
-                    return c_head * 256 + (((l & 15u) ^ stage::pattern<D>(pos)) << 4);
+                    return c_head * 256 + (((l & 15u) ^ stage::pattern<kRow>(pos)) << 4);
                 };
                 if (one_block && base_pos + CPW * PPI <= t1) {
                     const uint32_t blk = __umulhi(base_pos, p.block_magic);
@@ -324,30 +328,50 @@ tree_stream_kernel(const StreamParams p)
             };
 
             // Caches of bytes: a wave copies the bytes of 8 (position, kv head) rows and their scales of K and of V per step, four
-            // steps ahead, and turns what it copied itself into fp16 rows of one of two stages: no barrier in between.
-            constexpr uint32_t RP = 8 / NH;   // positions of a wave
+            // steps ahead, and widens what it copied itself into fp16 rows of one of two stages: no barrier in between. The
+            // bytes' values are exact in fp16 and the scales stay in fp32: K's multiplies the scores, V's goes into the
+            // exponents (p vs = 2^(x + log2 vs), rounded once, in range whatever the scales) and out of the normaliser.
+            constexpr uint32_t RP = 8 / NH;                 // positions of a wave
+            constexpr uint32_t COPIES = D / 64;             // of 1 KiB: K and V, or both in one
             auto row8 = [&](uint32_t s, uint32_t r) __attribute__((always_inline)) {
                 const uint32_t pos = min(t0 + s * SP + wave * RP + r / NH, t1 - 1), blk = __umulhi(pos, p.block_magic);
                 return (static_cast<uint64_t>(tbl[blk - blk0]) * p.block_size + (pos - blk * p.block_size)) * p.n_kv_heads + blockIdx.y * NH + r % NH;
             };
+            constexpr uint32_t RAW = 2 * (kStage + kScales);
             auto issue8 = [&](uint32_t s) __attribute__((always_inline)) {
-                const uint32_t st = smem_addr + 2 * kStage + (s % kStages) * kRawStage + wave * kWaveRaw;
-                const uint64_t off = row8(s, lane >> 3) * D + (lane & 7u) * 16;
-                stage::copy_lanes_16_once(st, p.k_cache + off);
-                stage::copy_lanes_16_once(st + 1024, p.v_cache + off);
+                const uint32_t st = smem_addr + RAW + (s % kStages) * kRawStage + wave * kWaveRaw;
+                if constexpr (D == 128) {
+                    const uint64_t off = row8(s, lane >> 3) * D + (lane & 7u) * 16;
+                    stage::copy_lanes_16_once(st, p.k_cache + off);
+                    stage::copy_lanes_16_once(st + 1024, p.v_cache + off);
+                } else {
+                    stage::copy_lanes_16_once(st, (half != 0 ? p.v_cache : p.k_cache) + row8(s, (lane >> 2) & 7u) * D + (lane & 3u) * 16);
+                }
                 stage::copy_lanes_4(st + 2048, ((lane & 8u) != 0 ? p.v_scale : p.k_scale) + row8(s, lane & 7u));   // K: words 0 .. 7, V: 8 .. 15
             };
             auto widen = [&](uint32_t s) __attribute__((always_inline)) {
-                const unsigned char *raw = smem + 2 * kStage + (s % kStages) * kRawStage + wave * kWaveRaw;
-                const uint32_t r = lane >> 3, pos = wave * RP + r / NH, x = stage::pattern<D>(pos);
-                unsigned char *dst = smem + (s % 2) * kStage + pos * POSB + (r % NH) * 256;
+                const unsigned char *raw = smem + RAW + (s % kStages) * kRawStage + wave * kWaveRaw;
+                unsigned char *st = smem + (s % 2) * kStage;
+                const uint32_t r = D == 128 ? lane >> 3 : (lane >> 2) & 7u, c = 2 * (D == 128 ? lane & 7u : lane & 3u);
+                const uint32_t pos = wave * RP + r / NH, x = stage::pattern<kRow>(pos);
+                unsigned char *dst = st + pos * POSB + (r % NH) * 256 + (D == 128 ? 0u : half * kHalf);
 #pragma unroll
-                for (int v = 0; v < 2; v++) {
+                for (uint32_t v = 0; v < COPIES; v++) {
                     const uint4 bytes = *reinterpret_cast<const uint4 *>(raw + v * 1024 + lane * 16);
-                    const float scale = *reinterpret_cast<const float *>(raw + 2048 + v * 32 + r * 4);
-                    const uint32_t c = 2 * (lane & 7u);
-                    *reinterpret_cast<uint4 *>(dst + v * kHalf + ((c ^ x) << 4)) = dequant8<T, KVF>(make_uint2(bytes.x, bytes.y), scale);
-                    *reinterpret_cast<uint4 *>(dst + v * kHalf + (((c + 1) ^ x) << 4)) = dequant8<T, KVF>(make_uint2(bytes.z, bytes.w), scale);
+                    *reinterpret_cast<uint4 *>(dst + v * kHalf + ((c ^ x) << 4)) = widen8<KVF>(make_uint2(bytes.x, bytes.y));
+                    *reinterpret_cast<uint4 *>(dst + v * kHalf + (((c + 1) ^ x) << 4)) = widen8<KVF>(make_uint2(bytes.z, bytes.w));
+                }
+                if (lane < 16) {
+                    const float scale = *reinterpret_cast<const float *>(raw + 2048 + lane * 4);
+                    const uint32_t rs = lane & 7u;
+                    float *to = reinterpret_cast<float *>(smem + 2 * kStage + (s % 2) * kScales) + (rs % NH) * SP + wave * RP + rs / NH;
+                    if (lane < 8) {
+                        to[0] = scale * kLog2e;
+                    } else {
+                        const float vs = fminf(fmaxf(scale, kLeastScale), 1.0f / kLeastScale);
+                        to[64] = __log2f(vs);
+                        to[128] = 1.0f / vs;
+                    }
                 }
             };
 
@@ -393,6 +417,17 @@ tree_stream_kernel(const StreamParams p)
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
+                [[maybe_unused]] const float *scales = reinterpret_cast<const float *>(smem + 2 * kStage + (s % 2) * kScales) + hsel * SP + 32 * h + 4 * half;
+                if constexpr (KV8) {   // in units of log2, with V's scale
+#pragma unroll
+                    for (int kg = 0; kg < 4; kg++) {
+                        const float4 ks = *reinterpret_cast<const float4 *>(scales + 8 * kg), lv = *reinterpret_cast<const float4 *>(scales + 64 + 8 * kg);
+                        S[4 * kg] = __builtin_fmaf(S[4 * kg], ks.x, lv.x);
+                        S[4 * kg + 1] = __builtin_fmaf(S[4 * kg + 1], ks.y, lv.y);
+                        S[4 * kg + 2] = __builtin_fmaf(S[4 * kg + 2], ks.z, lv.z);
+                        S[4 * kg + 3] = __builtin_fmaf(S[4 * kg + 3], ks.w, lv.w);
+                    }
+                }
                 if (masked) {
                     uint32_t seen = seen_from(j0);
 #pragma unroll
@@ -433,18 +468,27 @@ tree_stream_kernel(const StreamParams p)
                     mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
                 }
                 // (the reference moves only when exceeded by more than a factor of 4, as in the prefill kernel)
-                const float m_new = mx > m_run + kRescaleSlack ? mx : m_run;
+                const float m_new = mx > m_run + (KV8 ? 2.0f : kRescaleSlack) ? mx : m_run;
                 const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-                const float alpha = fast_exp2((m_run - m_safe) * kLog2e);
+                const float alpha = fast_exp2((m_run - m_safe) * (KV8 ? 1.0f : kLog2e));
                 const float neg_m = -m_safe * kLog2e;
                 m_run = m_new;
                 uint32_t w[8];
                 float psum = 0.f;
 #pragma unroll
                 for (int k = 0; k < 16; k += 2) {
-                    const float e0 = fast_exp2(__builtin_fmaf(S[k], kLog2e, neg_m));
-                    const float e1 = fast_exp2(__builtin_fmaf(S[k + 1], kLog2e, neg_m));
-                    psum += e0 + e1;
+                    float e0, e1;
+                    if constexpr (KV8) {
+                        e0 = fast_exp2(S[k] - m_safe);
+                        e1 = fast_exp2(S[k + 1] - m_safe);
+                        const float2 inv = *reinterpret_cast<const float2 *>(scales + 128 + (k / 4) * 8 + k % 4);
+                        psum = __builtin_fmaf(e0, inv.x, psum);
+                        psum = __builtin_fmaf(e1, inv.y, psum);
+                    } else {
+                        e0 = fast_exp2(__builtin_fmaf(S[k], kLog2e, neg_m));
+                        e1 = fast_exp2(__builtin_fmaf(S[k + 1], kLog2e, neg_m));
+                        psum += e0 + e1;
+                    }
                     w[k / 2] = T::pack(e0, e1);   // rounded to the products' type: half a step of it, 2^-8 (2^-11) of each
                 }
                 const uint4 pb[2] = {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
@@ -491,13 +535,13 @@ tree_stream_kernel(const StreamParams p)
             }
             for (uint32_t s = 0; s < n_steps; s++) {
                 if constexpr (KV8) {
-                    // this wave's share of step s has landed: three copies of each of the next three steps are out
+                    // this wave's share of step s has landed: COPIES + 1 of each of the next three steps are out
                     if (s + 3 <= last) {
-                        stage::wait<9>();
+                        stage::wait<3 * (COPIES + 1)>();
                     } else if (s + 2 <= last) {
-                        stage::wait<6>();
+                        stage::wait<2 * (COPIES + 1)>();
                     } else if (s + 1 <= last) {
-                        stage::wait<3>();
+                        stage::wait<COPIES + 1>();
                     } else {
                         stage::wait<0>();
                     }
@@ -580,7 +624,7 @@ tree_stream_kernel(const StreamParams p)
                         }
                     }
                     if (half == 0) {
-                        *reinterpret_cast<float2 *>(p.ml + (tile * 32 + col) * 2) = make_float2(m_run * kLog2e, l_tot);
+                        *reinterpret_cast<float2 *>(p.ml + (tile * 32 + col) * 2) = make_float2(KV8 ? m_run : m_run * kLog2e, l_tot);
                     }
                 }
             }
@@ -592,9 +636,9 @@ tree_stream_kernel(const StreamParams p)
     }
 }
 
-// Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), 16 threads of 8 columns (a piece of the stored layout) per row.
-template <typename T, int NH>
-__global__ void __launch_bounds__(256)
+// Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), D / 8 threads of 8 columns (a piece of the stored layout) per row.
+template <typename T, int NH, int D>
+__global__ void __launch_bounds__(2 * D)
 tree_merge_kernel(const StreamParams p)
 {
     const uint32_t id = blockIdx.x, kvh = blockIdx.y, G = p.group;
@@ -688,8 +732,8 @@ struct StreamPlan {
     uint32_t nh, groups, tiles, slots;
     size_t bytes;
 };
-StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t batch, uint32_t block_size, uint32_t max_num_block,
-                   uint32_t nh)
+StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t batch, uint32_t block_size,
+                   uint32_t max_num_block, uint32_t nh)
 {
     StreamPlan s;
     const uint32_t G = n_heads / n_kv_heads, rows = 32 * kWaves / nh;
@@ -700,28 +744,28 @@ StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
     const uint64_t sp = kHalf / 256 / nh, per = std::max<uint64_t>(1, (kTblCap - 2) * static_cast<uint64_t>(block_size) / sp);
     const uint64_t steps = s.tiles * ((static_cast<uint64_t>(max_num_block) * block_size + sp - 1) / sp);
     s.slots = static_cast<uint32_t>(2 * std::max<uint64_t>(std::max(1u, kComputeUnits / s.groups), steps / per + 1));
-    s.bytes = s.tiles * sizeof(int4) + static_cast<size_t>(s.groups) * s.slots * nh * rows * (D + 2) * sizeof(float);
+    s.bytes = s.tiles * sizeof(int4) + static_cast<size_t>(s.groups) * s.slots * nh * rows * (head_dim + 2) * sizeof(float);
     return s;
 }
 
 }  // namespace
 
-// head_dim 128; a copy's positions share a block (16-bit caches: four of them; bytes are copied from an address per lane); every
+// head_dim 128, or 64 over caches of bytes; a copy's positions share a block (16-bit caches: four of them; bytes are copied from an address per lane); every
 // block that a step can reach has its table entry in LDS
 bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
                            uint32_t max_num_block, int kv_dtype)
 {
-    return head_dim == D && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && (block_size % 4 == 0 || kv_dtype != XLITE_HIP_KV_SAME) &&
+    return (head_dim == 128 || (head_dim == 64 && kv_dtype != XLITE_HIP_KV_SAME)) && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && (block_size % 4 == 0 || kv_dtype != XLITE_HIP_KV_SAME) &&
            batch <= kSeqCap && static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32);
 }
 
-size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t batch, uint32_t block_size,
-                                   uint32_t max_num_block)
+size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t batch,
+                                   uint32_t block_size, uint32_t max_num_block)
 {
     size_t need = 0;   // whatever heads_of will say
     for (uint32_t nh : {1u, 2u}) {
         if (n_kv_heads % nh == 0) {
-            need = std::max(need, plan_of(total_tokens, n_heads, n_kv_heads, batch, block_size, max_num_block, nh).bytes);
+            need = std::max(need, plan_of(total_tokens, n_heads, n_kv_heads, head_dim, batch, block_size, max_num_block, nh).bytes);
         }
     }
     return need;
@@ -729,7 +773,7 @@ size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint
 
 int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
 {
-    const StreamPlan plan = plan_of(a.total_tokens, a.n_heads, a.n_kv_heads, a.batch, a.block_size, a.max_num_block,
+    const StreamPlan plan = plan_of(a.total_tokens, a.n_heads, a.n_kv_heads, a.head_dim, a.batch, a.block_size, a.max_num_block,
                                     heads_of(a.total_tokens, a.n_heads / a.n_kv_heads, a.n_kv_heads, a.batch, a.mask_words));
     if (a.workspace == nullptr || a.workspace_bytes < plan.bytes) {
         return fail(XLITE_HIP_ENOSPC, __func__, "workspace too small: need " + std::to_string(plan.bytes) + " bytes, have " +
@@ -747,7 +791,7 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     p.lens = a.lens;
     p.cached_lens = a.cached_lens;
     p.block_tables = a.block_tables;
-    p.q_tok_stride = (a.n_heads + 2 * a.n_kv_heads) * D;
+    p.q_tok_stride = (a.n_heads + 2 * a.n_kv_heads) * a.head_dim;
     p.n_heads = a.n_heads;
     p.n_kv_heads = a.n_kv_heads;
     p.group = a.n_heads / a.n_kv_heads;
@@ -759,36 +803,39 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     p.slots = plan.slots;
     p.meta = static_cast<int4 *>(a.workspace);
     p.acc = reinterpret_cast<float *>(p.meta + plan.tiles);
-    p.ml = p.acc + static_cast<uint64_t>(plan.groups) * plan.slots * 32 * kWaves * D;
+    p.ml = p.acc + static_cast<uint64_t>(plan.groups) * plan.slots * 32 * kWaves * a.head_dim;
     const dim3 grid(std::max(1u, kComputeUnits / plan.groups), plan.groups), merge_grid(plan.tiles, a.n_kv_heads, 32 * kWaves / plan.nh / 16);
-    auto launch = [&](auto t, auto n, auto kvf, auto io) -> int {
+    auto launch = [&](auto t, auto n, auto kvf, auto io, auto d) -> int {
         using T = decltype(t);
         using TIO = decltype(io);
-        constexpr int NH = decltype(n)::value, KVF = decltype(kvf)::value;
-        auto kernel = tree_stream_kernel<T, NH, KVF, TIO>;
+        constexpr int NH = decltype(n)::value, KVF = decltype(kvf)::value, D = decltype(d)::value;
+        auto kernel = tree_stream_kernel<T, NH, KVF, TIO, D>;
         const size_t lds = kStageBytes<KVF != XLITE_HIP_KV_SAME> + (kTblCap + kMaskCap + a.batch + 1) * sizeof(uint32_t);
         if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds)) {
             return rc;
         }
         kernel<<<grid, kThreads, lds, stream>>>(p);
         XL_LAUNCH_CHECK();
-        tree_merge_kernel<TIO, NH><<<merge_grid, 256, 0, stream>>>(p);
+        tree_merge_kernel<TIO, NH, D><<<merge_grid, 2 * D, 0, stream>>>(p);
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;
     };
-    auto with_heads = [&](auto t, auto kvf, auto io) -> int {
-        return plan.nh == 2 ? launch(t, std::integral_constant<int, 2>{}, kvf, io) : launch(t, std::integral_constant<int, 1>{}, kvf, io);
+    auto with_heads = [&](auto t, auto kvf, auto io, auto d) -> int {
+        return plan.nh == 2 ? launch(t, std::integral_constant<int, 2>{}, kvf, io, d) : launch(t, std::integral_constant<int, 1>{}, kvf, io, d);
     };
-    auto with_bytes = [&](auto kvf) -> int {
-        return a.dtype == XLITE_HIP_BF16 ? with_heads(FP16{}, kvf, BF16{}) : with_heads(FP16{}, kvf, FP16{});
+    using D64 = std::integral_constant<int, 64>;
+    using D128 = std::integral_constant<int, 128>;
+    auto with_dim = [&](auto kvf, auto io) -> int {
+        return a.head_dim == 128 ? with_heads(FP16{}, kvf, io, D128{}) : with_heads(FP16{}, kvf, io, D64{});
     };
+    auto with_bytes = [&](auto kvf) -> int { return a.dtype == XLITE_HIP_BF16 ? with_dim(kvf, BF16{}) : with_dim(kvf, FP16{}); };
     switch (a.kv_dtype) {
     case XLITE_HIP_KV_INT8: return with_bytes(std::integral_constant<int, XLITE_HIP_KV_INT8>{});
     case XLITE_HIP_KV_FP8: return with_bytes(std::integral_constant<int, XLITE_HIP_KV_FP8>{});
     default: break;
     }
     using Same = std::integral_constant<int, XLITE_HIP_KV_SAME>;
-    return a.dtype == XLITE_HIP_BF16 ? with_heads(BF16{}, Same{}, BF16{}) : with_heads(FP16{}, Same{}, FP16{});
+    return a.dtype == XLITE_HIP_BF16 ? with_heads(BF16{}, Same{}, BF16{}, D128{}) : with_heads(FP16{}, Same{}, FP16{}, D128{});
 }
 
 }  // namespace xlite

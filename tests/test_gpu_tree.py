@@ -141,6 +141,38 @@ def test_many_sequences_and_many_rows(rt, H, KV, lens, clens, cache):
     check(run(rt, w), w)
 
 
+@pytest.mark.parametrize("cache", ["int8", "fp8"])
+@pytest.mark.parametrize("H,KV,D,bs", [(14, 2, 64, 16), (28, 4, 128, 24), (3, 3, 64, 7), (8, 2, 128, 64)])
+def test_bytes_are_widened_exactly(rt, H, KV, D, bs, cache):
+    """The values of a cache of bytes are exact in fp16 and its scales stay in fp32, whatever their sizes: an fp16 model loses
+    what the probabilities (times V's scale) and the result are rounded, u each. Scores are off by (D + 8) half units of the
+    sum of their products' sizes in fp32, and their sum with log2 of a scale (up to 64) by 2^-18 of a factor of two."""
+    w = make(14, [9, 1, 30], [300, 64, 5], H, KV, D, bs, torch.float16, cache)
+    g = torch.Generator().manual_seed(1)
+    w["vs"] = w["vs"] * torch.exp2(torch.randint(-20, 4, w["vs"].shape, generator=g).float())
+    w["vs"][torch.rand(w["vs"].shape, generator=g) < 0.1] = 0.0
+    want, tol = reference(w)
+    got = run(rt, w).view(want.shape).double()
+    u = 2.0 ** -11
+    for i in range(3):
+        n, c, s0 = int(w["lens"][i]), int(w["clens"][i]), int(w["qsl"][i])
+        pos = torch.arange(c + n)
+        blk = w["tables"][i * w["mb"] + pos // bs].long()
+        k = w["k"][blk, pos % bs].double() * w["ks"][blk, pos % bs].double().unsqueeze(-1)
+        v = w["v"][blk, pos % bs].double() * w["vs"][blk, pos % bs].double().unsqueeze(-1)
+        for r in range(n):
+            seen = list(range(c)) + [c + j for j in range(n) if int(w["mask"][s0 + r, j // 32]) >> (j % 32) & 1]
+            q = w["qkv"][s0 + r].view(-1, D)[:H].double()
+            for h in range(H):
+                kk, vv = k[seen, h // (H // KV)], v[seen, h // (H // KV)]
+                p = torch.softmax(kk @ q[h], 0)
+                off = (D + 8) * 2.0 ** -24 * float((kk.abs() @ q[h].abs()).max()) + 2.0 ** -18
+                # (a product below fp16's normal numbers, 2^-14 of the largest one's power of two, is off by 2^-25 of that)
+                least = 2.0 ** -25 * 2 * float((p * vv.abs().amax(-1)).max()) * len(seen)
+                bound = (u + 2 * off + 2.0 ** -16) * (p @ vv.abs()) + u * want[s0 + r, h].abs() + least + 2.0 ** -25
+                assert ((got[s0 + r, h] - want[s0 + r, h]).abs() <= bound).all(), (i, r, h)
+
+
 @pytest.mark.parametrize("cache", ["same", "int8"])
 def test_less_workspace_gives_the_same_attention_or_an_error(rt, cache):
     """With less scratch than a shape asks for, another kernel serves it or nothing is launched."""
