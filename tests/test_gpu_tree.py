@@ -173,6 +173,14 @@ def test_bytes_are_widened_exactly(rt, H, KV, D, bs, cache):
                 assert ((got[s0 + r, h] - want[s0 + r, h]).abs() <= bound).all(), (i, r, h)
 
 
+@pytest.mark.parametrize("cache", ["same", "fp8"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_more_sequences_than_prefix_sums_fit(rt, D, cache):
+    lens = [[1, 2, 0, 1, 3][i % 5] for i in range(1030)]
+    w = make(15, lens, [i % 37 for i in range(1030)], 2, 1, D, 16, torch.float16, cache)
+    check(run(rt, w), w)
+
+
 @pytest.mark.parametrize("cache", ["same", "int8"])
 def test_less_workspace_gives_the_same_attention_or_an_error(rt, cache):
     """With less scratch than a shape asks for, another kernel serves it or nothing is launched."""
