@@ -97,26 +97,18 @@ __device__ __forceinline__ uint4 cache_chunk(const unsigned char *row, uint32_t 
     }
 }
 
-// M row m of a sequence, walked in steps of 32: token and head without a division per step
-struct RowCursor {
-    uint32_t r, h, dr, dh, group;
-    __device__ __forceinline__ RowCursor(uint32_t m, uint32_t g) : r(m / g), h(m - m / g * g), dr(32u / g), dh(32u - 32u / g * g), group(g) {}
-    __device__ __forceinline__ void step()
-    {
-        h += dh;
-        r += dr;
-        const bool over = h >= group;
-        h -= over ? group : 0u;
-        r += over ? 1u : 0u;
-    }
-};
+// tiles of 32 rows of a wave (head_dim 256: the registers hold one), positions of a staged tile
+template <int D>
+constexpr int kRowTiles = D == 256 ? 1 : 2;
+template <int D>
+constexpr int kStagedPositions = D == 256 ? 32 : 64;
 
 template <typename T, int D, int KVF>
 __global__ void __launch_bounds__(kThreads)
 row_stats_kernel(const WeightsParams p)
 {
     constexpr int KS = D / 16;
-    constexpr int RT = D == 256 ? 1 : 2;      // tiles of 32 rows of a wave (head_dim 256: the registers hold one)
+    constexpr int RT = kRowTiles<D>;
     constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
     constexpr uint32_t ROWB = D * (KV8 ? 1 : 2);
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
@@ -270,14 +262,14 @@ row_stats_kernel(const WeightsParams p)
     }
 }
 
-// The same for 16-bit caches of head_dim 64 and 128, K tiles of 64 positions copied straight into LDS (a ring of three) and
+// The same for 16-bit caches, K tiles of 64 positions (32 of head_dim 256) copied straight into LDS (a ring of three) and
 // shared by the four waves. Read from memory by every wave, as above, a K chunk of 32 positions touches 32 lines per
 // instruction and every line four times: the vector cache's look-ups took longer than the products and the exponentials.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
 row_stats_staged_kernel(const WeightsParams p)
 {
-    constexpr int KS = D / 16, RT = 2, BN = 64, STAGES = 3;
+    constexpr int KS = D / 16, RT = kRowTiles<D>, BN = kStagedPositions<D>, STAGES = 3;
     constexpr uint32_t ROWB = D * 2, STAGE = BN * ROWB, TILE = 4 * 32 * RT;
     constexpr int PPC = 1024 / ROWB;           // positions per copy
     constexpr int CPW = BN / PPC / 4;          // copies per wave and tile
@@ -371,8 +363,7 @@ row_stats_staged_kernel(const WeightsParams p)
             }
         };
         const uint32_t n_tiles = ceil_div(end - begin, static_cast<uint32_t>(BN));
-        const uint32_t row_off = D == 128 ? col * 256 : (col >> 1) * 256;
-        const uint32_t x = D == 128 ? (half ^ stage::pattern<D>(col)) << 4 : ((((col & 1) << 3) | half) ^ stage::pattern<D>(col >> 1)) << 4;
+        const uint32_t row_off = stage::row_offset<D>(col), x = stage::row_swizzle<D>(col, half);
         issue(0);
         issue(1);
         for (uint32_t tile = 0; tile < n_tiles; tile++) {
@@ -380,13 +371,13 @@ row_stats_staged_kernel(const WeightsParams p)
             __syncthreads();      // ... and everybody else's; stage (tile - 1) % 3 is free
             issue(tile + 2);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < BN / 32; h++) {
                 const uint32_t t0 = begin + tile * BN + h * 32;
                 const unsigned char *base = smem + (tile % STAGES) * STAGE + h * 32 * ROWB + row_off;
                 uint4 kop[KS];
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
-                    kop[ks] = *reinterpret_cast<const uint4 *>(base + (((2 * ks) << 4) ^ x));
+                    kop[ks] = *reinterpret_cast<const uint4 *>(base + stage::chunk_offset(ks, x));
                 }
                 f32x16_t S[RT];
 #pragma unroll
@@ -489,159 +480,19 @@ join_stats_kernel(const float *__restrict__ stats, float *__restrict__ norm, uin
     }
 }
 
-template <typename T, int D, int KVF>
-__global__ void __launch_bounds__(2 * kThreads)
-column_sums_kernel(const WeightsParams p)
-{
-    constexpr int KS = D / 16;
-    constexpr int PT = 1;                     // tiles of 32 positions of a wave (the registers hold one)
-    constexpr uint32_t WG = 4 * 32 * PT;      // positions of the workgroup: two waves for each 32 PT of them
-    constexpr uint32_t ROWB = D * (KVF == XLITE_HIP_KV_SAME ? 2 : 1);
-    __shared__ float other[4][32 * PT];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, half = lane >> 5;
-    const uint32_t kvh = blockIdx.z, seq = blockIdx.y, G = p.group;
-    const uint32_t mine = wave & 3u, turn = wave >> 2;   // which 64 positions, and which of the M tiles: even or odd ones
-    const Sequence s = sequence_of(p, seq);
-    const uint32_t total = s.cached + s.nodes;
-    if (s.nodes == 0 || blockIdx.x * WG >= total) {
-        return;
-    }
-    const uint32_t p0 = blockIdx.x * WG + mine * 32 * PT;   // the wave's first position
-    const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
-    uint64_t at[PT];
-    uint4 kreg[PT][KS];
-    float mul[PT], acc[PT];
-#pragma unroll
-    for (int pt = 0; pt < PT; pt++) {
-        at[pt] = slot_of(p, table, min(p0 + pt * 32 + col, total - 1)) * p.n_kv_heads + kvh;
-        const unsigned char *row = p.k_cache + at[pt] * ROWB;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            kreg[pt][ks] = cache_chunk<T, KVF>(row, 2 * ks + half);
-        }
-        mul[pt] = kLog2e;
-        acc[pt] = 0.f;
-        if constexpr (KVF != XLITE_HIP_KV_SAME) {
-            mul[pt] *= p.k_scale[at[pt]];
-        }
-    }
-    // the first row that sees the wave's first position (rows before it see none of its positions)
-    const uint32_t first_seen = p0 > s.cached + s.first ? (p0 - s.cached - s.first) * G : 0u;
-    const uint64_t tok0 = s.start + s.first;
-    const float *norm = p.norm + static_cast<uint64_t>(kvh) * p.m_total + tok0 * G;
-    const uint16_t *q0 = p.q + tok0 * p.q_tok_stride + static_cast<uint64_t>(kvh * G) * D + half * 8;
-    const uint32_t m_begin = (first_seen & ~31u) + 32 * turn;
-    if (m_begin < s.m_rows && p0 < total) {
-        RowCursor cursor(m_begin + col, G);
-        uint4 next[KS];
-        // a tile's query rows are requested one tile ahead (rows past the end repeat the last one)
-        auto request = [&](uint32_t m0) __attribute__((always_inline)) {
-            const bool in = m0 + col < s.m_rows;
-            const uint32_t r = in ? cursor.r : (s.m_rows - 1) / G, h = in ? cursor.h : G - 1;
-            const uint16_t *src = q0 + static_cast<uint64_t>(r) * p.q_tok_stride + h * D;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                next[ks] = *reinterpret_cast<const uint4 *>(src + ks * 16);
-            }
-        };
-        request(m_begin);
-        for (uint32_t m0 = m_begin; m0 < s.m_rows; m0 += 64) {
-            uint4 qop[KS];
-            float n[16];
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                qop[ks] = next[ks];
-            }
-            // this tile's normalisers ahead of the next tile's rows: memory answers in order
-            if (m0 + 32 <= s.m_rows) {
-                typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const f4 x = *reinterpret_cast<const f4 *>(norm + m0 + g * 8 + half * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        n[4 * g + e] = x[e];
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    n[k] = norm[min(m0 + (k / 4) * 8 + half * 4 + (k % 4), s.m_rows - 1)];
-                }
-            }
-            if (m0 + 64 < s.m_rows) {
-                cursor.step();
-                cursor.step();
-                request(m0 + 64);
-            }
-            f32x16_t S[PT];
-#pragma unroll
-            for (int pt = 0; pt < PT; pt++) {
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    S[pt][k] = 0.f;
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-#pragma unroll
-                for (int pt = 0; pt < PT; pt++) {
-                    S[pt] = mfma32<T>(qop[ks], kreg[pt][ks], S[pt]);
-                }
-            }
-            const bool masked = m0 + 32 > s.m_rows || p0 + 32 * PT - 1 > s.cached + s.first + m0 / G;
-#pragma unroll
-            for (int pt = 0; pt < PT; pt++) {
-                float sum = 0.f;
-                if (masked) {
-                    const uint32_t t = p0 + pt * 32 + col;
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const uint32_t mk = m0 + (k / 4) * 8 + half * 4 + (k % 4);
-                        const float e = fast_exp2(__builtin_fmaf(S[pt][k], mul[pt], n[k]));
-                        sum += mk < s.m_rows && t <= s.cached + s.first + mk / G ? e : 0.f;
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        sum += fast_exp2(__builtin_fmaf(S[pt][k], mul[pt], n[k]));
-                    }
-                }
-                acc[pt] += sum;   // (a tile's sum first: 16 additions, then one per tile, not one chain over every row)
-            }
-        }
-    }
-#pragma unroll
-    for (int pt = 0; pt < PT; pt++) {
-        acc[pt] += __shfl_xor(acc[pt], 32);
-        if (turn == 1 && half == 0) {
-            other[mine][pt * 32 + col] = acc[pt];
-        }
-    }
-    __syncthreads();
-    if (turn == 0 && half == 0) {
-#pragma unroll
-        for (int pt = 0; pt < PT; pt++) {
-            const uint32_t t = p0 + pt * 32 + col;
-            if (t < total) {
-                const float sum = acc[pt] + other[mine][pt * 32 + col];
-                p.weights[at[pt]] = t < s.cached ? p.weights[at[pt]] + sum : sum;
-            }
-        }
-    }
-}
-
-// The same for head_dim 64 and 128 with the query rows copied straight into LDS, 32 M rows for each turn (four waves, 64
-// positions each) at a time, and their normalisers with them. As many turns as the registers hold waves: the exponentials of
+// Query rows copied straight into LDS, 32 M rows for each turn (four waves, 64 positions each, 32 of head_dim 256) at a time, and
+// their normalisers with them. As many turns as the registers hold waves: the exponentials of
 // a tile (96 vector instructions, 300 cycles with four waves on a SIMD, 410 with one) run beside the products of the others.
 template <int D>
-constexpr int kTurns = D == 128 ? 3 : 4;
+constexpr int kTurns = D == 256 ? 2 : D == 128 ? 3 : 4;
+template <int D>
+constexpr int kColumnTiles = D == 256 ? 1 : 2;   // tiles of 32 positions of a wave
 
 template <typename T, int D, int KVF>
 __global__ void __launch_bounds__(kTurns<D> * kThreads)
-column_sums_staged_kernel(const WeightsParams p)
+column_sums_kernel(const WeightsParams p)
 {
-    constexpr int KS = D / 16, PT = 2, STAGES = 3, TURNS = kTurns<D>, ROWS = 32 * TURNS;
+    constexpr int KS = D / 16, PT = kColumnTiles<D>, STAGES = 3, TURNS = kTurns<D>, ROWS = 32 * TURNS;
     constexpr uint32_t ROWB = D * (KVF == XLITE_HIP_KV_SAME ? 2 : 1), QROWB = D * 2;
     constexpr uint32_t QBYTES = ROWS * QROWB, STAGE = QBYTES + 4 * TURNS * 256;   // the rows, then each wave's normalisers
     constexpr int RPC = 1024 / QROWB, CPW = 8 / RPC;                    // rows per copy, copies per wave
@@ -721,8 +572,7 @@ column_sums_staged_kernel(const WeightsParams p)
         stage::copy_lanes_4(st + QBYTES + wave * 256, norm + min(m_ahead + 32 * turn + (lane & 31u), rows - 1));
         m_ahead += ROWS;
     };
-    const uint32_t row_off = D == 128 ? col * 256 : (col >> 1) * 256;
-    const uint32_t x = D == 128 ? (half ^ stage::pattern<D>(col)) << 4 : ((((col & 1) << 3) | half) ^ stage::pattern<D>(col >> 1)) << 4;
+    const uint32_t row_off = stage::row_offset<D>(col), x = stage::row_swizzle<D>(col, half);
     uint32_t slot = 0;
     issue(0);
     issue(1);
@@ -741,7 +591,7 @@ column_sums_staged_kernel(const WeightsParams p)
         const unsigned char *base = st + turn * 32 * QROWB + row_off;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
-            qop[ks] = *reinterpret_cast<const uint4 *>(base + (((2 * ks) << 4) ^ x));
+            qop[ks] = *reinterpret_cast<const uint4 *>(base + stage::chunk_offset(ks, x));
         }
         float n[16];
         const float *nl = reinterpret_cast<const float *>(st + QBYTES + wave * 256) + half * 4;
@@ -1189,11 +1039,11 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
             store_scores_kernel<T, D, KVF><<<dim3(ceil_div(plan.splits, kStoredWaves / heads) * ceil_div(n_kv_heads, heads), batch),
                                              64 * kStoredWaves, lds, s>>>(p);
         } else {
-            // K through LDS: 16-bit caches whose copies (four positions of 128 elements, eight of 64) lie in one block, and a
+            // K through LDS: 16-bit caches whose copies (two positions of 256 elements, four of 128, eight of 64) lie in one block, and a
             // split's block-table entries behind the stages
             bool staged = false;
-            if constexpr (D != 256 && KVF == XLITE_HIP_KV_SAME) {
-                const size_t lds = 3 * 64 * D * 2 + (static_cast<size_t>(plan.split_len / block_size) + 2) * sizeof(uint32_t);
+            if constexpr (KVF == XLITE_HIP_KV_SAME) {
+                const size_t lds = 3 * kStagedPositions<D> * D * 2 + (static_cast<size_t>(plan.split_len / block_size) + 2) * sizeof(uint32_t);
                 staged = block_size % (512 / D) == 0 && p.block_magic != 0 && lds <= 64 * 1024;
                 if (staged) {
                     if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(row_stats_staged_kernel<T, D>), lds)) {
@@ -1221,15 +1071,11 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
             const uint32_t z = std::max(1u, std::min(n_kv_heads, 512u / std::max(1u, tiles * batch)));   // few positions: the heads side by side
             sum_scores_kernel<<<dim3(tiles, batch, z), kThreads, 0, s>>>(p);
         } else {
-            if constexpr (D == 256) {
-                column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 128u), batch, n_kv_heads), 2 * kThreads, 0, s>>>(p);
-            } else {
-                const size_t lds = 3 * kTurns<D> * (32 * D * 2 + 4 * 256);
-                if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(column_sums_staged_kernel<T, D, KVF>), lds)) {
-                    return rc;
-                }
-                column_sums_staged_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 256u), batch, n_kv_heads), kTurns<D> * kThreads, lds, s>>>(p);
+            const size_t lds = 3 * kTurns<D> * (32 * D * 2 + 4 * 256);
+            if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(column_sums_kernel<T, D, KVF>), lds)) {
+                return rc;
             }
+            column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 128u * kColumnTiles<D>), batch, n_kv_heads), kTurns<D> * kThreads, lds, s>>>(p);
         }
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;

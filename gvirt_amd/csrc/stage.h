@@ -48,28 +48,38 @@ __device__ __forceinline__ uint32_t lds_address(const void *p)
         static_cast<uint32_t>((size_t)((__attribute__((address_space(3))) const unsigned char *)p)))));
 }
 
-// Tiles of rows of D 16-bit elements (64 or 128), 16-byte chunks XOR-swizzled by the row so that 32 rows of one chunk (the
-// operand of a product) are read without bank conflicts. A 256-byte bank window holds one row of 128 elements or two of 64.
+// Tiles of rows of D 16-bit elements (64, 128 or 256), 16-byte chunks XOR-swizzled by the row so that 32 rows of one chunk (the
+// operand of a product) are read without bank conflicts. A 256-byte bank window holds two rows of 64 elements, one of 128 or
+// half a row of 256 (whose halves have the row's pattern).
 template <int D>
 __device__ __forceinline__ uint32_t pattern(uint32_t window)
 {
-    static_assert(D == 128 || D == 64, "tiles exist for rows of 128 and 64 elements");
-    return D == 128 ? (((window & 3) << 2) | ((window >> 2) & 3)) : (((window & 1) << 2) | ((window >> 1) & 3));
+    static_assert(D == 256 || D == 128 || D == 64, "tiles exist for rows of 64, 128 and 256 elements");
+    return D >= 128 ? (((window & 3) << 2) | ((window >> 2) & 3)) : (((window & 1) << 2) | ((window >> 1) & 3));
+}
+// byte offset of chunk 2 ks + half of row `row`: row_offset + chunk_offset(ks)
+template <int D>
+__device__ __forceinline__ uint32_t row_offset(uint32_t row)
+{
+    return D == 64 ? (row >> 1) * 256 : row * (D * 2);
 }
 template <int D>
-__device__ __forceinline__ uint32_t tile_off(uint32_t row, uint32_t chunk)
+__device__ __forceinline__ uint32_t row_swizzle(uint32_t row, uint32_t half)
 {
-    if constexpr (D == 128) {
-        return row * 256 + ((chunk ^ pattern<D>(row)) << 4);
-    } else {
-        return (row >> 1) * 256 + (((((row & 1) << 3) | chunk) ^ pattern<D>(row >> 1)) << 4);
-    }
+    return D == 64 ? ((((row & 1) << 3) | half) ^ pattern<D>(row >> 1)) << 4 : (half ^ pattern<D>(row)) << 4;
+}
+__device__ __forceinline__ uint32_t chunk_offset(uint32_t ks, uint32_t swizzle)
+{
+    return (((2 * (ks & 7u)) << 4) ^ swizzle) + (ks >> 3) * 256;
 }
 // what lane `lane` of the copy that fills rows first .. first + 1024 / (2 D) - 1 has to fetch: its row of them and chunk
 template <int D>
 __device__ __forceinline__ void copy_source(uint32_t lane, uint32_t first, uint32_t *row, uint32_t *chunk)
 {
-    if constexpr (D == 128) {
+    if constexpr (D == 256) {
+        *row = lane >> 5;
+        *chunk = ((lane & 15u) ^ pattern<D>(first + (lane >> 5))) | ((lane >> 4) & 1u) << 4;
+    } else if constexpr (D == 128) {
         *row = lane >> 4;
         *chunk = (lane & 15u) ^ pattern<D>(first + (lane >> 4));
     } else {
