@@ -45,11 +45,11 @@ constexpr uint32_t kStages = 4;
 template <int NH>
 constexpr uint32_t kRows = 32 * kWaves / NH;     // M rows of a workgroup, per kv head
 constexpr uint32_t kStage = 2 * kHalf;
-constexpr uint32_t kWaveRaw = 2 * 1024 + 256;    // caches of bytes: what a wave copies in a step, 8 rows of K and of V and their scales
+constexpr uint32_t kWaveRaw = 2 * 1024 + 256;    // short rows: what a wave copies in a step, 8 rows of K and of V and their scales
 constexpr uint32_t kRawStage = kWaves * kWaveRaw;
 constexpr uint32_t kScales = 3 * 64 * 4;         // of a widened stage: three numbers per (kv head, position)
-template <bool KV8>
-constexpr uint32_t kStageBytes = KV8 ? 2 * (kStage + kScales) + kStages * kRawStage : kStages * kStage;
+template <bool RAW>
+constexpr uint32_t kStageBytes = RAW ? 2 * (kStage + kScales) + kStages * kRawStage : kStages * kStage;
 constexpr float kLeastScale = 0x1p-100f;         // of a V row, in the arithmetic of its logarithm and reciprocal
 constexpr uint32_t kTblCap = 2048;               // block-table entries staged per segment
 constexpr uint32_t kSeqCap = 1024;               // sequences whose prefix sums fit
@@ -101,13 +101,15 @@ __device__ __forceinline__ uint32_t uni(uint32_t x)
 }
 
 // NH: kv heads of a workgroup. T: the type of the products; TIO: of the query rows and the output (the same, or bf16 with fp16
-// products over caches of bytes, KVF). D: 128, or 64 over caches of bytes (half of a row in LDS is not used then).
+// products over caches of bytes, KVF). Rows shorter than
+// 256 bytes (caches of bytes, D = 64) are copied as they are and laid out by the wave that copied them; of D = 64, half of a
+// row in LDS is not used.
 template <typename T, int NH, int KVF, typename TIO, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_stream_kernel(const StreamParams p)
 {
-    constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME;
-    static_assert(D == 128 || (D == 64 && KV8), "head_dim 128, or 64 over caches of bytes");
+    constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME, RAW = KV8 || D == 64;
+    static_assert(D == 128 || D == 64, "head_dim 64 or 128");
     constexpr int KS = D / 16, DT = D / 32;
     constexpr uint32_t ROWS = kRows<NH>;
     constexpr uint32_t POSB = NH * 256;          // LDS bytes of a position
@@ -115,7 +117,7 @@ tree_stream_kernel(const StreamParams p)
     constexpr uint32_t PPI = 1024 / POSB;        // positions of a copy
     constexpr int CPW = 2;                       // copies per wave, step and tensor
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    uint32_t *tbl = reinterpret_cast<uint32_t *>(smem + kStageBytes<KV8>);
+    uint32_t *tbl = reinterpret_cast<uint32_t *>(smem + kStageBytes<RAW>);
     uint32_t *mask_lds = tbl + kTblCap;
     uint32_t *pref = mask_lds + kMaskCap;        // batch + 1 words
     const uint32_t smem_addr = stage::lds_address(smem);
@@ -327,41 +329,49 @@ tree_stream_kernel(const StreamParams p)
                 }
             };
 
-            // Caches of bytes: a wave copies the bytes of 8 (position, kv head) rows and their scales of K and of V per step, four
-            // steps ahead, and widens what it copied itself into fp16 rows of one of two stages: no barrier in between. The
-            // bytes' values are exact in fp16 and the scales stay in fp32: K's multiplies the scores, V's goes into the
+            // Short rows: a wave copies 8 (position, kv head) rows of K and of V (and the scales of bytes) per step, four steps
+            // ahead, and lays out what it copied itself as the rows of one of two stages, bytes widened to fp16: no barrier in
+            // between. The bytes' values are exact in fp16 and the scales stay in fp32: K's multiplies the scores, V's goes into the
             // exponents (p vs = 2^(x + log2 vs), rounded once, in range whatever the scales) and out of the normaliser.
             constexpr uint32_t RP = 8 / NH;                 // positions of a wave
-            constexpr uint32_t COPIES = D / 64;             // of 1 KiB: K and V, or both in one
+            constexpr uint32_t ROWM = KV8 ? D : 2 * D;      // bytes of a row in memory: 64 or 128 here
+            constexpr uint32_t COPIES = ROWM == 64 ? 1 : 2; // of 1 KiB: both tensors in one, or one each
+            constexpr uint32_t OPS = COPIES + (KV8 ? 1 : 0);
             auto row8 = [&](uint32_t s, uint32_t r) __attribute__((always_inline)) {
                 const uint32_t pos = min(t0 + s * SP + wave * RP + r / NH, t1 - 1), blk = __umulhi(pos, p.block_magic);
                 return (static_cast<uint64_t>(tbl[blk - blk0]) * p.block_size + (pos - blk * p.block_size)) * p.n_kv_heads + blockIdx.y * NH + r % NH;
             };
-            constexpr uint32_t RAW = 2 * (kStage + kScales);
+            constexpr uint32_t RING = 2 * (kStage + kScales);
             auto issue8 = [&](uint32_t s) __attribute__((always_inline)) {
-                const uint32_t st = smem_addr + RAW + (s % kStages) * kRawStage + wave * kWaveRaw;
-                if constexpr (D == 128) {
-                    const uint64_t off = row8(s, lane >> 3) * D + (lane & 7u) * 16;
+                const uint32_t st = smem_addr + RING + (s % kStages) * kRawStage + wave * kWaveRaw;
+                if constexpr (COPIES == 2) {
+                    const uint64_t off = row8(s, lane >> 3) * ROWM + (lane & 7u) * 16;
                     stage::copy_lanes_16_once(st, p.k_cache + off);
                     stage::copy_lanes_16_once(st + 1024, p.v_cache + off);
                 } else {
-                    stage::copy_lanes_16_once(st, (half != 0 ? p.v_cache : p.k_cache) + row8(s, (lane >> 2) & 7u) * D + (lane & 3u) * 16);
+                    stage::copy_lanes_16_once(st, (half != 0 ? p.v_cache : p.k_cache) + row8(s, (lane >> 2) & 7u) * ROWM + (lane & 3u) * 16);
                 }
-                stage::copy_lanes_4(st + 2048, ((lane & 8u) != 0 ? p.v_scale : p.k_scale) + row8(s, lane & 7u));   // K: words 0 .. 7, V: 8 .. 15
+                if constexpr (KV8) {   // K: words 0 .. 7, V: 8 .. 15
+                    stage::copy_lanes_4(st + 2048, ((lane & 8u) != 0 ? p.v_scale : p.k_scale) + row8(s, lane & 7u));
+                }
             };
-            auto widen = [&](uint32_t s) __attribute__((always_inline)) {
-                const unsigned char *raw = smem + RAW + (s % kStages) * kRawStage + wave * kWaveRaw;
+            auto lay_out = [&](uint32_t s) __attribute__((always_inline)) {
+                const unsigned char *raw = smem + RING + (s % kStages) * kRawStage + wave * kWaveRaw;
                 unsigned char *st = smem + (s % 2) * kStage;
-                const uint32_t r = D == 128 ? lane >> 3 : (lane >> 2) & 7u, c = 2 * (D == 128 ? lane & 7u : lane & 3u);
+                const uint32_t r = COPIES == 2 ? lane >> 3 : (lane >> 2) & 7u, c = COPIES == 2 ? lane & 7u : lane & 3u;   // row, 16 bytes of it
                 const uint32_t pos = wave * RP + r / NH, x = stage::pattern<kRow>(pos);
-                unsigned char *dst = st + pos * POSB + (r % NH) * 256 + (D == 128 ? 0u : half * kHalf);
+                unsigned char *dst = st + pos * POSB + (r % NH) * 256 + (COPIES == 2 ? 0u : half * kHalf);
 #pragma unroll
                 for (uint32_t v = 0; v < COPIES; v++) {
                     const uint4 bytes = *reinterpret_cast<const uint4 *>(raw + v * 1024 + lane * 16);
-                    *reinterpret_cast<uint4 *>(dst + v * kHalf + ((c ^ x) << 4)) = widen8<KVF>(make_uint2(bytes.x, bytes.y));
-                    *reinterpret_cast<uint4 *>(dst + v * kHalf + (((c + 1) ^ x) << 4)) = widen8<KVF>(make_uint2(bytes.z, bytes.w));
+                    if constexpr (KV8) {
+                        *reinterpret_cast<uint4 *>(dst + v * kHalf + (((2 * c) ^ x) << 4)) = widen8<KVF>(make_uint2(bytes.x, bytes.y));
+                        *reinterpret_cast<uint4 *>(dst + v * kHalf + (((2 * c + 1) ^ x) << 4)) = widen8<KVF>(make_uint2(bytes.z, bytes.w));
+                    } else {
+                        *reinterpret_cast<uint4 *>(dst + v * kHalf + ((c ^ x) << 4)) = bytes;
+                    }
                 }
-                if (lane < 16) {
+                if (KV8 && lane < 16) {
                     const float scale = *reinterpret_cast<const float *>(raw + 2048 + lane * 4);
                     const uint32_t rs = lane & 7u;
                     float *to = reinterpret_cast<float *>(smem + 2 * kStage + (s % 2) * kScales) + (rs % NH) * SP + wave * RP + rs / NH;
@@ -385,7 +395,7 @@ tree_stream_kernel(const StreamParams p)
             auto compute = [&](uint32_t s, uint32_t h) __attribute__((always_inline)) {
                 const uint32_t j0 = t0 + s * SP + 32 * h;
                 const bool masked = j0 + 32 > cached;   // (positions below the cached length are seen by every row)
-                const unsigned char *st = smem + (s % (KV8 ? 2 : kStages)) * kStage + h * 32 * POSB;
+                const unsigned char *st = smem + (s % (RAW ? 2 : kStages)) * kStage + h * 32 * POSB;
                 uint4 kop[KS];
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
@@ -514,7 +524,7 @@ tree_stream_kernel(const StreamParams p)
             };
 
             const uint32_t n_steps = b - a, last = n_steps - 1;
-            if constexpr (KV8) {
+            if constexpr (RAW) {
                 for (uint32_t s = 0; s < min(n_steps, kStages); s++) {
                     issue8(s);
                 }
@@ -534,18 +544,18 @@ tree_stream_kernel(const StreamParams p)
                 qreg[ks] = convert8<TIO, T>(qreg[ks]);
             }
             for (uint32_t s = 0; s < n_steps; s++) {
-                if constexpr (KV8) {
-                    // this wave's share of step s has landed: COPIES + 1 of each of the next three steps are out
+                if constexpr (RAW) {
+                    // this wave's share of step s has landed: OPS of each of the next three steps are out
                     if (s + 3 <= last) {
-                        stage::wait<3 * (COPIES + 1)>();
+                        stage::wait<3 * OPS>();
                     } else if (s + 2 <= last) {
-                        stage::wait<2 * (COPIES + 1)>();
+                        stage::wait<2 * OPS>();
                     } else if (s + 1 <= last) {
-                        stage::wait<COPIES + 1>();
+                        stage::wait<OPS>();
                     } else {
                         stage::wait<0>();
                     }
-                    widen(s);          // (the stage of step s - 2: everybody was past it at the barrier of step s - 1)
+                    lay_out(s);          // (the stage of step s - 2: everybody was past it at the barrier of step s - 1)
                     __syncthreads();
                     if (s + 4 <= last) {
                         issue8(s + 4);
@@ -636,12 +646,16 @@ tree_stream_kernel(const StreamParams p)
     }
 }
 
-// Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), D / 8 threads of 8 columns (a piece of the stored layout) per row.
-template <typename T, int NH, int D>
-__global__ void __launch_bounds__(2 * D)
+// Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), D / 8 threads of 8 columns (a piece of the stored
+// layout) per row, and TURNS such sets that take the segments in turn.
+template <typename T, int NH, int D, int TURNS>
+__global__ void __launch_bounds__(2 * D * TURNS)
 tree_merge_kernel(const StreamParams p)
 {
+    constexpr int U = TURNS > 1 ? 8 : 4;   // segments of a set at a time
+    __shared__ float part[TURNS > 1 ? TURNS - 1 : 1][10][2 * D];
     const uint32_t id = blockIdx.x, kvh = blockIdx.y, G = p.group;
+    const uint32_t turn = threadIdx.x / (2 * D), in_set = threadIdx.x % (2 * D);
     uint32_t seq = 0;   // the last sequence whose ids start at or before `id`
     int32_t n;
     uint32_t start;
@@ -666,27 +680,39 @@ tree_merge_kernel(const StreamParams p)
         n = p.lens[seq];
         start = static_cast<uint32_t>(p.query_start_loc[seq]);
     }
-    const uint32_t mt = id - first_id<NH>(p, start, seq);
-    const uint32_t in_tile = blockIdx.z * 16 + threadIdx.x % 16, m = mt * kRows<NH> + in_tile;
-    if (n <= 0 || m >= static_cast<uint32_t>(n) * G) {
+    const uint32_t mt = id - first_id<NH>(p, start, seq), m_rows = static_cast<uint32_t>(max(n, 0)) * G;
+    const uint32_t m_first = mt * kRows<NH> + blockIdx.z * 16;
+    if (m_first >= m_rows) {   // (the whole workgroup)
         return;
     }
     const uint32_t segments = static_cast<uint32_t>(meta.x);
-    if (segments == 0) {
+    const bool shared = TURNS > 1 && segments > U;   // by the sets
+    if (segments == 0 || (turn != 0 && !shared)) {
         return;
     }
-    const uint32_t c0 = static_cast<uint32_t>(meta.y), first = static_cast<uint32_t>(meta.z), piece = threadIdx.x / 16;
+    const uint32_t in_tile = blockIdx.z * 16 + in_set % 16, m = mt * kRows<NH> + in_tile;   // (rows past the end: partials of no row, unstored)
+    const uint32_t c0 = static_cast<uint32_t>(meta.y), first = static_cast<uint32_t>(meta.z), piece = in_set / 16;
     const uint64_t group0 = static_cast<uint64_t>(kvh / NH) * p.slots;
     auto row_of = [&](uint32_t s) {
         const uint64_t slot = group0 + (s == 0 ? 2 * c0 + (1 - first) : 2 * (c0 + s));
         return (slot * NH + kvh % NH) * kRows<NH> + in_tile;
     };
     float m_all = -INFINITY, l = 0.f, o[8] = {};
-    for (uint32_t i0 = 0; i0 < segments; i0 += 4) {
-        float2 ml[4];
-        float4 x[4][2];
+    auto join = [&](float m_part, float l_part, const float (&x)[8]) __attribute__((always_inline)) {
+        const float m_new = fmaxf(m_all, m_part), safe = m_new == -INFINITY ? 0.f : m_new;
+        const float wa = fast_exp2(m_all - safe), wb = fast_exp2(m_part - safe);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {   // (all loads on their way; past the end: the last one again, weighted zero)
+        for (int e = 0; e < 8; e++) {
+            o[e] = o[e] * wa + (wb != 0.f ? x[e] * wb : 0.f);   // (a part of weight zero that saw nothing holds zeros)
+        }
+        l = l * wa + l_part * wb;
+        m_all = m_new;
+    };
+    for (uint32_t i0 = U * turn; i0 < segments; i0 += U * TURNS) {
+        float2 ml[U];
+        float4 x[U][2];
+#pragma unroll
+        for (int u = 0; u < U; u++) {   // (all loads on their way; past the end: the last one again, left out)
             const uint64_t row = row_of(min(i0 + u, segments - 1));
             ml[u] = *reinterpret_cast<const float2 *>(p.ml + row * 2);
             const float4 *src = reinterpret_cast<const float4 *>(p.acc + (row & ~31ull) * D) + piece * 64 + (row & 31);
@@ -694,21 +720,38 @@ tree_merge_kernel(const StreamParams p)
             x[u][1] = src[32];   // columns 8 piece + 4 .. + 7
         }
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const bool in = i0 + u < segments;
-            const float m_new = in ? fmaxf(m_all, ml[u].x) : m_all;
-            const float safe = m_new == -INFINITY ? 0.f : m_new;
-            const float wa = fast_exp2(m_all - safe), wb = fast_exp2(ml[u].x - safe);
-            if (in) {
-                const float *f = reinterpret_cast<const float *>(&x[u][0]);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    o[e] = o[e] * wa + (wb != 0.f ? f[e] * wb : 0.f);   // (a part of weight zero that saw nothing holds zeros)
-                }
-                l = l * wa + ml[u].y * wb;
-                m_all = m_new;
+        for (int u = 0; u < U; u++) {
+            if (i0 + u < segments) {
+                const float f[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
+                join(ml[u].x, ml[u].y, f);
             }
         }
+    }
+    if (shared) {
+        if (turn != 0) {
+            part[turn - 1][8][in_set] = m_all;
+            part[turn - 1][9][in_set] = l;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                part[turn - 1][e][in_set] = o[e];
+            }
+        }
+        __syncthreads();
+        if (turn != 0) {
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < TURNS - 1; u++) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f[e] = part[u][e][in_set];
+            }
+            join(part[u][8][in_set], part[u][9][in_set], f);
+        }
+    }
+    if (m >= m_rows) {
+        return;
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const float scale = l != l ? l : inv;
@@ -750,12 +793,13 @@ StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
 
 }  // namespace
 
-// head_dim 128, or 64 over caches of bytes; a copy's positions share a block (16-bit caches: four of them; bytes are copied from an address per lane); every
+// head_dim 64 or 128; a copy's positions share a block (rows of 256 bytes: four of them; short rows have an address per lane); every
 // block that a step can reach has its table entry in LDS
 bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
                            uint32_t max_num_block, int kv_dtype)
 {
-    return (head_dim == 128 || (head_dim == 64 && kv_dtype != XLITE_HIP_KV_SAME)) && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && (block_size % 4 == 0 || kv_dtype != XLITE_HIP_KV_SAME) &&
+    return (head_dim == 128 || head_dim == 64) && n_kv_heads > 0 && n_heads % n_kv_heads == 0 &&
+           (block_size % 4 == 0 || head_dim == 64 || kv_dtype != XLITE_HIP_KV_SAME) &&
            batch <= kSeqCap && static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32);
 }
 
@@ -810,13 +854,20 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
         using TIO = decltype(io);
         constexpr int NH = decltype(n)::value, KVF = decltype(kvf)::value, D = decltype(d)::value;
         auto kernel = tree_stream_kernel<T, NH, KVF, TIO, D>;
-        const size_t lds = kStageBytes<KVF != XLITE_HIP_KV_SAME> + (kTblCap + kMaskCap + a.batch + 1) * sizeof(uint32_t);
+        const size_t lds = kStageBytes<KVF != XLITE_HIP_KV_SAME || D == 64> + (kTblCap + kMaskCap + a.batch + 1) * sizeof(uint32_t);
         if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds)) {
             return rc;
         }
         kernel<<<grid, kThreads, lds, stream>>>(p);
         XL_LAUNCH_CHECK();
-        tree_merge_kernel<TIO, NH, D><<<merge_grid, 2 * D, 0, stream>>>(p);
+        // few sequences: their tiles have a segment in (nearly) every workgroup; 250 segments of one tile took 64 us one set
+        // after the other. Many: five segments are joined as fast by one set (8 us for 16 sequences, 10 with four sets)
+        constexpr int SETS = 512 / D;
+        if (grid.x >= 16 * a.batch) {
+            tree_merge_kernel<TIO, NH, D, SETS><<<merge_grid, 2 * D * SETS, 0, stream>>>(p);
+        } else {
+            tree_merge_kernel<TIO, NH, D, 1><<<merge_grid, 2 * D, 0, stream>>>(p);
+        }
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;
     };
@@ -825,17 +876,17 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     };
     using D64 = std::integral_constant<int, 64>;
     using D128 = std::integral_constant<int, 128>;
-    auto with_dim = [&](auto kvf, auto io) -> int {
-        return a.head_dim == 128 ? with_heads(FP16{}, kvf, io, D128{}) : with_heads(FP16{}, kvf, io, D64{});
+    auto with_dim = [&](auto t, auto kvf, auto io) -> int {
+        return a.head_dim == 128 ? with_heads(t, kvf, io, D128{}) : with_heads(t, kvf, io, D64{});
     };
-    auto with_bytes = [&](auto kvf) -> int { return a.dtype == XLITE_HIP_BF16 ? with_dim(kvf, BF16{}) : with_dim(kvf, FP16{}); };
+    auto with_bytes = [&](auto kvf) -> int { return a.dtype == XLITE_HIP_BF16 ? with_dim(FP16{}, kvf, BF16{}) : with_dim(FP16{}, kvf, FP16{}); };
     switch (a.kv_dtype) {
     case XLITE_HIP_KV_INT8: return with_bytes(std::integral_constant<int, XLITE_HIP_KV_INT8>{});
     case XLITE_HIP_KV_FP8: return with_bytes(std::integral_constant<int, XLITE_HIP_KV_FP8>{});
     default: break;
     }
     using Same = std::integral_constant<int, XLITE_HIP_KV_SAME>;
-    return a.dtype == XLITE_HIP_BF16 ? with_heads(BF16{}, Same{}, BF16{}, D128{}) : with_heads(FP16{}, Same{}, FP16{}, D128{});
+    return a.dtype == XLITE_HIP_BF16 ? with_dim(BF16{}, Same{}, BF16{}) : with_dim(FP16{}, Same{}, FP16{});
 }
 
 }  // namespace xlite
