@@ -268,7 +268,8 @@ walk_rows_kernel(const VerifyParams p)
 }
 
 // Up to so many rows all of them are read, by as many workgroups as there is room for; beyond, each sequence's workgroup
-// reads the rows of its path one after the other (384 rows of 131072 logits are 100 MB, 16 us, as long as a path of three).
+// reads the rows of its path one after the other (131072 fp32 logits, trees of 32, paths of up to 8: 12 trees all read 40 us, 13
+// walked 55).
 constexpr uint32_t kAllRows = 384;
 uint32_t parts_per_row(uint32_t rows)
 {
