@@ -2,7 +2,7 @@
 // nodes of one drafted tree per sequence, already written to the cache behind the cached positions; a row sees every
 // cached position and those nodes whose bit its mask has:
 //     out_r = sum_j [seen(r, j)] exp(q_r . k_j) v_j / sum_j [seen(r, j)] exp(q_r . k_j),   0 where nothing is seen.
-// head_dim 64 and 128: a kernel of its own that streams the cache past all rows of a tree (tree_stream.hip).
+// A kernel of its own streams the cache past all rows of a tree (tree_stream.hip).
 // Other shapes: the walk is that of a prefill chunk with another mask, and only tiles that reach into the tree look at it, so
 // the prefill kernels serve them with a mask of their own (prefill_mfma.hip, mfma_attention.hip: TREE).
 #include <algorithm>

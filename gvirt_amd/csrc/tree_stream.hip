@@ -1,4 +1,4 @@
-// Attention over drafted trees for head_dim 64 and 128: the cache streamed once, past all rows of a tree.
+// Attention over drafted trees: the cache streamed once, past all rows of a tree.
 //
 // A tree has few rows (nodes x query heads of a kv head: an M row each), so its attention is bound by reading K and V. The
 // prefill kernel gives a workgroup one kv head: its copies are 256-byte rows up to two kilobytes apart, which memory serves
@@ -19,6 +19,7 @@
 // step of 16 KiB, the chain of widening, barrier, operands, scores, softmax and products of two waves a SIMD. Half the vector
 // instructions for widening, or the products of one half of the waves beside the widening of the other: the same time. head_dim
 // 64, 16 bits: a tree of 8 over 700 positions 10 and 4 us (the prefill kernel 15), 64 ragged trees of 4 over 2000 25 us (31).
+// head_dim 256: 32 ragged trees of 8 over 4000 positions of 4 heads, 330 MB, 74 us with the merge (the generic kernel 237).
 //
 // Work split: a sequence owns ceil(len G / rows) M tiles of ceil((cached + len) / step) steps each; the steps of all M tiles laid
 // end to end are cut into equal chunks, one per workgroup, whatever the sequences' lengths (they live in device memory: every
@@ -105,13 +106,16 @@ __device__ __forceinline__ uint32_t uni(uint32_t x)
 // products over caches of bytes, KVF). Rows shorter than
 // 256 bytes (caches of bytes, D = 64) are copied as they are and laid out by the wave that copied them; of D = 64, half of a
 // row in LDS is not used.
-template <typename T, int NH, int KVF, typename TIO, int D>
+// WIDE: head_dim 256, as two heads of 128 in memory whose scores are added: a wave forms the scores of both halves and the
+// results of one.
+template <typename T, int NH, int KVF, typename TIO, int D, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
 tree_stream_kernel(const StreamParams p)
 {
+    static_assert(!WIDE || (NH == 2 && D == 128 && KVF == XLITE_HIP_KV_SAME), "two halves of 128 elements, 16-bit caches");
     constexpr bool KV8 = KVF != XLITE_HIP_KV_SAME, RAW = KV8 || D == 64;
     static_assert(D == 128 || D == 64, "head_dim 64 or 128");
-    constexpr int KS = D / 16, DT = D / 32;
+    constexpr int KS = D / 16, DT = D / 32, HALVES = WIDE ? 2 : 1;
     constexpr uint32_t ROWS = kRows<NH>;
     constexpr uint32_t POSB = NH * 256;          // LDS bytes of a position
     constexpr uint32_t SP = kHalf / POSB;        // positions of a step
@@ -188,7 +192,7 @@ tree_stream_kernel(const StreamParams p)
     const uint32_t n_chunks = ceil_div(total, chunk);
 
     // ---- read roles (the pattern of position p + 32 is that of p)
-    const uint32_t k_off = col * POSB + hsel * 256;
+    const uint32_t k_off = col * POSB + (WIDE ? 0u : hsel * 256);
     const uint32_t kx = (half ^ stage::pattern<kRow>(col)) << 4;
     uint32_t v_off;
     {
@@ -238,7 +242,7 @@ tree_stream_kernel(const StreamParams p)
             const bool has_rows = m_first < m_rows;
             const uint32_t m = min(m_first + col, m_rows - 1);       // (rows past the end repeat the last one, unstored)
             const uint64_t tok = start + m / G;
-            const uint32_t head = kvh * G + m % G;
+            const uint32_t head = (WIDE ? blockIdx.y : kvh) * G + m % G;
             const uint32_t t0 = a * SP, t1 = min(range, b * SP);
             const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
             const uint32_t blk0 = t0 / p.block_size, blk1 = (t1 - 1) / p.block_size;
@@ -254,10 +258,10 @@ tree_stream_kernel(const StreamParams p)
             const uint32_t *words_src = p.tree_mask + static_cast<uint64_t>(start + tok_first) * p.mask_words;
             const uint32_t word = words_src[words_in_lds ? min(threadIdx.x, n_words - 1) : 0u];
             const uint32_t entry = static_cast<uint32_t>(table[blk0 + min(threadIdx.x, n_blk - 1)]);
-            uint4 qreg[KS];
-            const uint16_t *src = p.q + tok * p.q_tok_stride + static_cast<uint64_t>(head) * D;
+            uint4 qreg[HALVES * KS];
+            const uint16_t *src = p.q + tok * p.q_tok_stride + static_cast<uint64_t>(head) * (HALVES * D);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
+            for (int ks = 0; ks < HALVES * KS; ks++) {
                 qreg[ks] = *reinterpret_cast<const uint4 *>(src + ks * 16 + half * 8);
             }
             // (this wait leaves the query rows on their way)
@@ -397,19 +401,25 @@ tree_stream_kernel(const StreamParams p)
                 const uint32_t j0 = t0 + s * SP + 32 * h;
                 const bool masked = j0 + 32 > cached;   // (positions below the cached length are seen by every row)
                 const unsigned char *st = smem + (s % (RAW ? 2 : kStages)) * kStage + h * 32 * POSB;
-                uint4 kop[KS];
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    kop[ks] = *reinterpret_cast<const uint4 *>(st + k_off + (((2 * ks) << 4) ^ kx));
-                }
                 f32x16_t S;
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
                     S[k] = 0.f;
                 }
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    S = mfma32<T>(kop[ks], qreg[ks], S);
+                for (int w = 0; w < HALVES; w++) {
+                    uint4 kop[KS];
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        kop[ks] = *reinterpret_cast<const uint4 *>(st + k_off + w * 256 + (((2 * ks) << 4) ^ kx));
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) {
+                        S = mfma32<T>(kop[ks], qreg[w * KS + ks], S);
+                    }
+                    if (WIDE) {
+                        __builtin_amdgcn_sched_barrier(0);   // (the operands of one half at a time: the registers hold no more)
+                    }
                 }
                 // V^T operands: on their way during the softmax
                 typedef s16x4_t __attribute__((address_space(3))) * lds_tr_ptr;
@@ -540,7 +550,7 @@ tree_stream_kernel(const StreamParams p)
             }
             // (the query rows were requested before the copies; their wait is for both)
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
+            for (int ks = 0; ks < HALVES * KS; ks++) {
                 asm volatile("" : "+v"(qreg[ks].x), "+v"(qreg[ks].y), "+v"(qreg[ks].z), "+v"(qreg[ks].w));
                 qreg[ks] = convert8<TIO, T>(qreg[ks]);
             }
@@ -611,7 +621,7 @@ tree_stream_kernel(const StreamParams p)
                 if (whole) {
                     const float inv = l_tot > 0.f ? 1.0f / l_tot : 0.f;   // (NaN is not above 0 ...)
                     const float scale = l_tot != l_tot ? l_tot : inv;     // (... and stays NaN)
-                    uint16_t *dst = p.out + (tok * p.n_heads + head) * D;
+                    uint16_t *dst = p.out + (tok * p.n_heads + head) * (HALVES * D) + (WIDE ? hsel * D : 0u);
 #pragma unroll
                     for (int dt = 0; dt < DT; dt++) {
 #pragma unroll
@@ -649,7 +659,7 @@ tree_stream_kernel(const StreamParams p)
 
 // Joins the partials of an M tile: a workgroup per (M tile, kv head, 16 rows), D / 8 threads of 8 columns (a piece of the stored
 // layout) per row, and TURNS such sets that take the segments in turn.
-template <typename T, int NH, int D, int TURNS>
+template <typename T, int NH, int D, int TURNS, bool WIDE>
 __global__ void __launch_bounds__(2 * D * TURNS)
 tree_merge_kernel(const StreamParams p)
 {
@@ -761,7 +771,8 @@ tree_merge_kernel(const StreamParams p)
     w.y = T::pack(o[2] * scale, o[3] * scale);
     w.z = T::pack(o[4] * scale, o[5] * scale);
     w.w = T::pack(o[6] * scale, o[7] * scale);
-    *reinterpret_cast<uint4 *>(p.out + (static_cast<uint64_t>(start + m / G) * p.n_heads + kvh * G + m % G) * D + piece * 8) = w;
+    const uint64_t head = static_cast<uint64_t>(start + m / G) * p.n_heads + (WIDE ? kvh / 2 : kvh) * G + m % G;
+    *reinterpret_cast<uint4 *>(p.out + (WIDE ? head * 2 + kvh % 2 : head) * D + piece * 8) = w;
 }
 
 // The kv heads of a workgroup: as many as divide the model's and leave it the rows of a typical M tile (twice the average of
@@ -795,12 +806,12 @@ StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
 
 }  // namespace
 
-// head_dim 64 or 128; a copy's positions share a block (rows of 256 bytes: four of them; short rows have an address per lane); every
+// head_dim 64, 128 or 256 (16-bit caches); a copy's positions share a block (rows of 256 bytes: four of them; short rows have an address per lane); every
 // block that a step can reach has its table entry in LDS
 bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
                            uint32_t max_num_block, int kv_dtype)
 {
-    return (head_dim == 128 || head_dim == 64) && n_kv_heads > 0 && n_heads % n_kv_heads == 0 &&
+    return (head_dim == 128 || head_dim == 64 || (head_dim == 256 && kv_dtype == XLITE_HIP_KV_SAME)) && n_kv_heads > 0 && n_heads % n_kv_heads == 0 &&
            (block_size % 4 == 0 || head_dim == 64 || kv_dtype != XLITE_HIP_KV_SAME) &&
            batch <= kSeqCap && static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32);
 }
@@ -808,6 +819,9 @@ bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_
 size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t batch,
                                    uint32_t block_size, uint32_t max_num_block)
 {
+    if (head_dim == 256) {   // as twice the heads of 128
+        return plan_of(total_tokens, 2 * n_heads, 2 * n_kv_heads, 128, batch, block_size, max_num_block, 2).bytes;
+    }
     size_t need = 0;   // whatever heads_of will say
     for (uint32_t nh : {1u, 2u}) {
         if (n_kv_heads % nh == 0) {
@@ -819,8 +833,10 @@ size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint
 
 int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
 {
-    const StreamPlan plan = plan_of(a.total_tokens, a.n_heads, a.n_kv_heads, a.head_dim, a.batch, a.block_size, a.max_num_block,
-                                    heads_of(a.total_tokens, a.n_heads / a.n_kv_heads, a.n_kv_heads, a.batch, a.mask_words));
+    const bool wide = a.head_dim == 256;
+    const uint32_t split = wide ? 2u : 1u, n_kv_heads = split * a.n_kv_heads, head_dim = a.head_dim / split;   // as they lie in memory
+    const StreamPlan plan = plan_of(a.total_tokens, split * a.n_heads, n_kv_heads, head_dim, a.batch, a.block_size, a.max_num_block,
+                                    wide ? 2u : heads_of(a.total_tokens, a.n_heads / a.n_kv_heads, a.n_kv_heads, a.batch, a.mask_words));
     if (a.workspace == nullptr || a.workspace_bytes < plan.bytes) {
         return fail(XLITE_HIP_ENOSPC, __func__, "workspace too small: need " + std::to_string(plan.bytes) + " bytes, have " +
                                                     std::to_string(a.workspace == nullptr ? 0 : a.workspace_bytes));
@@ -839,7 +855,7 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     p.block_tables = a.block_tables;
     p.q_tok_stride = (a.n_heads + 2 * a.n_kv_heads) * a.head_dim;
     p.n_heads = a.n_heads;
-    p.n_kv_heads = a.n_kv_heads;
+    p.n_kv_heads = n_kv_heads;
     p.group = a.n_heads / a.n_kv_heads;
     p.batch = a.batch;
     p.block_size = a.block_size;
@@ -849,13 +865,14 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     p.slots = plan.slots;
     p.meta = static_cast<int4 *>(a.workspace);
     p.acc = reinterpret_cast<float *>(p.meta + plan.tiles);
-    p.ml = p.acc + static_cast<uint64_t>(plan.groups) * plan.slots * 32 * kWaves * a.head_dim;
-    const dim3 grid(std::max(1u, kComputeUnits / plan.groups), plan.groups), merge_grid(plan.tiles, a.n_kv_heads, 32 * kWaves / plan.nh / 16);
-    auto launch = [&](auto t, auto n, auto kvf, auto io, auto d) -> int {
+    p.ml = p.acc + static_cast<uint64_t>(plan.groups) * plan.slots * 32 * kWaves * head_dim;
+    const dim3 grid(std::max(1u, kComputeUnits / plan.groups), plan.groups), merge_grid(plan.tiles, n_kv_heads, 32 * kWaves / plan.nh / 16);
+    auto launch = [&](auto t, auto n, auto kvf, auto io, auto d, auto w) -> int {
         using T = decltype(t);
         using TIO = decltype(io);
         constexpr int NH = decltype(n)::value, KVF = decltype(kvf)::value, D = decltype(d)::value;
-        auto kernel = tree_stream_kernel<T, NH, KVF, TIO, D>;
+        constexpr bool WIDE = decltype(w)::value;
+        auto kernel = tree_stream_kernel<T, NH, KVF, TIO, D, WIDE>;
         const size_t lds = kStageBytes<KVF != XLITE_HIP_KV_SAME || D == 64> + (kTblCap + kMaskCap + a.batch + 1) * sizeof(uint32_t);
         if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(kernel), lds)) {
             return rc;
@@ -866,15 +883,16 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
         // after the other. Many: five segments are joined as fast by one set (8 us for 16 sequences, 10 with four sets)
         constexpr int SETS = 512 / D;
         if (grid.x >= 16 * a.batch) {
-            tree_merge_kernel<TIO, NH, D, SETS><<<merge_grid, 2 * D * SETS, 0, stream>>>(p);
+            tree_merge_kernel<TIO, NH, D, SETS, WIDE><<<merge_grid, 2 * D * SETS, 0, stream>>>(p);
         } else {
-            tree_merge_kernel<TIO, NH, D, 1><<<merge_grid, 2 * D, 0, stream>>>(p);
+            tree_merge_kernel<TIO, NH, D, 1, WIDE><<<merge_grid, 2 * D, 0, stream>>>(p);
         }
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;
     };
     auto with_heads = [&](auto t, auto kvf, auto io, auto d) -> int {
-        return plan.nh == 2 ? launch(t, std::integral_constant<int, 2>{}, kvf, io, d) : launch(t, std::integral_constant<int, 1>{}, kvf, io, d);
+        return plan.nh == 2 ? launch(t, std::integral_constant<int, 2>{}, kvf, io, d, std::false_type{})
+                            : launch(t, std::integral_constant<int, 1>{}, kvf, io, d, std::false_type{});
     };
     using D64 = std::integral_constant<int, 64>;
     using D128 = std::integral_constant<int, 128>;
@@ -888,6 +906,11 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     default: break;
     }
     using Same = std::integral_constant<int, XLITE_HIP_KV_SAME>;
+    if (wide) {
+        using Two = std::integral_constant<int, 2>;
+        return a.dtype == XLITE_HIP_BF16 ? launch(BF16{}, Two{}, Same{}, BF16{}, D128{}, std::true_type{})
+                                         : launch(FP16{}, Two{}, Same{}, FP16{}, D128{}, std::true_type{});
+    }
     return a.dtype == XLITE_HIP_BF16 ? with_dim(BF16{}, Same{}, BF16{}) : with_dim(FP16{}, Same{}, FP16{});
 }
 

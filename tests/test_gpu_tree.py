@@ -141,6 +141,14 @@ def test_many_sequences_and_many_rows(rt, H, KV, lens, clens, cache):
     check(run(rt, w), w)
 
 
+@pytest.mark.parametrize("lens,clens", BATCHES + [([100, 1, 1, 1, 1, 1, 1, 1], [70, 0, 33, 5, 64, 1, 127, 300]), ([30], [5000]),
+                                                  ([2] * 70, [17 * i % 90 for i in range(70)])])
+@pytest.mark.parametrize("H,KV,bs", [(16, 4, 64), (4, 1, 12), (6, 3, 7)])
+def test_heads_of_256(rt, H, KV, bs, lens, clens):
+    w = make(16, lens, clens, H, KV, 256, bs, torch.bfloat16 if bs % 2 else torch.float16)
+    check(run(rt, w), w)
+
+
 @pytest.mark.parametrize("cache", ["int8", "fp8"])
 @pytest.mark.parametrize("H,KV,D,bs", [(14, 2, 64, 16), (28, 4, 128, 24), (3, 3, 64, 7), (8, 2, 128, 64)])
 def test_bytes_are_widened_exactly(rt, H, KV, D, bs, cache):
@@ -218,7 +226,7 @@ def test_any_mask_and_rows_that_see_nothing(rt, D):
     check(run(rt, w), w)
 
 
-@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (256, 16), (128, 5)])
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (256, 16), (128, 5), (256, 6)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_values_that_are_not_finite_stay_where_they_are_seen(rt, D, bs, bad):
     """Node 2's K and V rows and everything behind the sequence hold `bad`; the rows that do not see node 2 are those of
