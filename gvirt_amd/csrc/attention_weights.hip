@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "attention_common.h"
+#include "block_magic.h"
 #include "kv8.h"
 #include "stage.h"
 
@@ -61,7 +62,7 @@ struct WeightsParams {
     uint32_t tiles_per_seq;        // row tiles of a sequence when a window bounds them (0: ids from the prefix sums)
     uint32_t m_total;              // total_tokens * G
     uint32_t splits, split_len;
-    uint32_t block_magic;          // floor(2^32 / block_size) + 1 while positions * block_size stay below 2^32, otherwise 0
+    uint32_t block_magic;          // see block_magic()
     float *scores;                 // stored scores: [kv head][M row][pitch], in units of log2
     uint32_t pitch;                // positions of a stored row, a multiple of 64
 };
@@ -1020,7 +1021,7 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
     p.tiles_per_seq = plan.tiles_per_seq;
     p.splits = plan.splits;
     p.split_len = plan.split_len;
-    p.block_magic = static_cast<uint64_t>(max_ctx) * block_size < (1ull << 32) ? static_cast<uint32_t>((1ull << 32) / block_size) + 1 : 0u;
+    p.block_magic = block_magic(block_size, max_ctx);
     const uint32_t rows = plan.rows * n_kv_heads;
     p.norm = static_cast<float *>(workspace);
     if (plan.stored) {

@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "attention_common.h"
+#include "block_magic.h"
 
 namespace xlite {
 
@@ -41,7 +42,7 @@ struct SelectParams {
     const int32_t *context_lens;
     const int32_t *block_tables;
     uint32_t n_kv_heads, block_size, max_num_block, budget, recent, sink, batch;
-    uint32_t block_magic;   // floor(2^32 / block_size) + 1 while positions * block_size stay below 2^32, otherwise 0
+    uint32_t block_magic;   // see block_magic()
 };
 
 // The n-th largest of the keys (n > 0, at least n of them) and how many of those equal to it are among the n largest.
@@ -432,11 +433,6 @@ compact_kernel(const CompactParams p)
     }
 }
 
-uint32_t magic_of(uint32_t block_size, uint32_t max_num_block)
-{
-    return static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32) ? static_cast<uint32_t>((1ull << 32) / block_size) + 1 : 0u;
-}
-
 }  // namespace
 
 }  // namespace xlite
@@ -460,7 +456,7 @@ extern "C" int xlite_hip_select_kept(void *stream, const float *weights, int32_t
     // (the list of one head is written while the others still read the lengths)
     XL_REQUIRE(kept_lens != context_lens, "kept_lens must not be context_lens");
     SelectParams p{weights, kept, kept_lens, context_lens, block_tables, n_kv_heads, block_size, max_num_block,
-                   budget, recent, sink, batch, magic_of(block_size, max_num_block)};
+                   budget, recent, sink, batch, block_magic(block_size, static_cast<uint64_t>(max_num_block) * block_size)};
     const uint64_t grid = (static_cast<uint64_t>(batch) + kXcds - 1) / kXcds * kXcds * n_kv_heads;
     const uint32_t judged = max_num_block * block_size - std::min(max_num_block * block_size, sink + recent);   // at most
     hipStream_t s = as_stream(stream);
@@ -520,7 +516,7 @@ extern "C" int xlite_hip_compact_kv_cache(void *stream, void *k_cache, void *v_c
     const uint64_t row = head_bytes * (per_head ? 1u : n_kv_heads);
     XL_REQUIRE(row < (1ull << 31), "a position's row is too long");
     p.row_bytes = static_cast<uint32_t>(row);
-    p.block_magic = magic_of(block_size, max_num_block);
+    p.block_magic = block_magic(block_size, static_cast<uint64_t>(max_num_block) * block_size);
     // slices of 256 bytes, or the largest power of two below that divides the row
     p.slice_bytes = std::min(256u, p.row_bytes & (~p.row_bytes + 1u));
     p.slices = p.row_bytes / p.slice_bytes;

@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "attention_common.h"
+#include "block_magic.h"
 #include "kv8.h"
 #include "stage.h"
 
@@ -807,13 +808,13 @@ StreamPlan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads,
 }  // namespace
 
 // head_dim 64, 128 or 256 (16-bit caches); a copy's positions share a block (rows of 256 bytes: four of them; short rows have an address per lane); every
-// block that a step can reach has its table entry in LDS
+// block that a step can reach has its table entry in LDS; the kernel divides by the block size with its magic only (not blocks of 1)
 bool tree_stream_supported(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
                            uint32_t max_num_block, int kv_dtype)
 {
     return (head_dim == 128 || head_dim == 64 || (head_dim == 256 && kv_dtype == XLITE_HIP_KV_SAME)) && n_kv_heads > 0 && n_heads % n_kv_heads == 0 &&
            (block_size % 4 == 0 || head_dim == 64 || kv_dtype != XLITE_HIP_KV_SAME) &&
-           batch <= kSeqCap && static_cast<uint64_t>(max_num_block) * block_size * block_size < (1ull << 32);
+           batch <= kSeqCap && block_magic(block_size, static_cast<uint64_t>(max_num_block) * block_size) != 0;
 }
 
 size_t tree_stream_workspace_bytes(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t batch,
@@ -859,7 +860,7 @@ int launch_tree_stream(hipStream_t stream, const AttentionArgs &a)
     p.group = a.n_heads / a.n_kv_heads;
     p.batch = a.batch;
     p.block_size = a.block_size;
-    p.block_magic = static_cast<uint32_t>((1ull << 32) / a.block_size) + 1;
+    p.block_magic = block_magic(a.block_size, static_cast<uint64_t>(a.max_num_block) * a.block_size);
     p.max_num_block = a.max_num_block;
     p.mask_words = a.mask_words;
     p.slots = plan.slots;
