@@ -599,8 +599,10 @@ tree_stream_kernel(const StreamParams p)
                     }
                 }
             }
-            if (!KV8 && poisoned) {   // (rare, and not fast: the tree's V rows are read again, value by value)
-                for (uint32_t j = max(t0, cached); j < t1; j++) {
+            if (!KV8 && poisoned) {   // (rare, and not fast: the V rows of the masked steps are read again, value by value)
+                // from the first masked step on, whose positions below the cached length every row sees (segments begin at
+                // multiples of 32 positions, as the halves of a step do)
+                for (uint32_t j = max(t0, cached & ~31u); j < t1; j++) {
                     const uint32_t blk = j / p.block_size;
                     const uint64_t row = static_cast<uint64_t>(static_cast<uint32_t>(table[blk])) * p.block_size + (j - blk * p.block_size);
                     const uint16_t *v = reinterpret_cast<const uint16_t *>(p.v_cache) + (row * p.n_kv_heads + kvh) * D + 4 * half;
