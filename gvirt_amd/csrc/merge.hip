@@ -70,10 +70,12 @@ merge_kernel(uint16_t *__restrict__ out, const float *__restrict__ part_acc,
                 }
 #pragma unroll
                 for (uint32_t u = 0; u < 4; u++) {
-                    acc.x += x[u].x * w[u];
-                    acc.y += x[u].y * w[u];
-                    acc.z += x[u].z * w[u];
-                    acc.w += x[u].w * w[u];
+                    // (rows past the end repeat the last one: left out, not multiplied by zero, an infinity is a result too)
+                    const bool in = j + u < cnt;
+                    acc.x += in ? x[u].x * w[u] : 0.f;
+                    acc.y += in ? x[u].y * w[u] : 0.f;
+                    acc.z += in ? x[u].z * w[u] : 0.f;
+                    acc.w += in ? x[u].w * w[u] : 0.f;
                 }
             }
         }

@@ -9,7 +9,7 @@ DEV = "cuda:0"
 BF = torch.bfloat16
 
 
-@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (256, 16), (64, 5)])
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (256, 16), (64, 5), (128, 5), (256, 6)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_values_of_cached_positions_reach_every_row(rt, D, bs, bad):
     """One cached position's V row holds `bad` in some columns: the first or the last cached position of the 32 that the
