@@ -36,11 +36,21 @@ extern "C" size_t xlite_hip_tree_attention_workspace_bytes(uint32_t total_tokens
     if (total_tokens == 0 || batch == 0 || n_kv_heads == 0 || n_heads % n_kv_heads != 0 || head_dim < 8 || block_size == 0) {
         return 0;
     }
-    size_t need = tree_bytes_16(total_tokens, n_heads, n_kv_heads, head_dim, batch, max_num_block * block_size);
+    // the kernel that serves the shape, and nothing for those that would with less
     if (tree_stream_supported(n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, kv_dtype)) {
-        need = std::max(need, tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, head_dim, batch, block_size, max_num_block));
+        return tree_stream_workspace_bytes(total_tokens, n_heads, n_kv_heads, head_dim, batch, block_size, max_num_block);
     }
-    if (kv_dtype != XLITE_HIP_KV_SAME) {
+    size_t need = tree_bytes_16(total_tokens, n_heads, n_kv_heads, head_dim, batch, max_num_block * block_size);
+    AttentionArgs shape{};
+    const float scale = 1.f;
+    shape.n_heads = n_heads;
+    shape.n_kv_heads = n_kv_heads;
+    shape.head_dim = head_dim;
+    shape.block_size = block_size;
+    shape.max_num_block = max_num_block;
+    shape.kv_dtype = kv_dtype;
+    shape.k_scale = shape.v_scale = &scale;
+    if (kv_dtype != XLITE_HIP_KV_SAME && !prefill_kv8_supported(shape)) {
         need += kv_dequant_bytes(n_kv_heads, head_dim, block_size, batch, max_num_block);
         need += kv_dequant_f16_io_bytes(total_tokens, n_heads, n_kv_heads, head_dim);   // bf16 models (the size does not know)
     }

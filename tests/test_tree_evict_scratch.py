@@ -1,0 +1,25 @@
+"""How much scratch the operators on drafted trees and on caches kept to a budget ask for (host formulas)."""
+import pytest
+
+from gvirt_amd import _lib
+
+MB = 1 << 20
+
+
+def tree(tokens, heads, kv_heads, dim, block, batch, blocks, kv):
+    return _lib.load().xlite_hip_tree_attention_workspace_bytes(tokens, heads, kv_heads, dim, block, batch, blocks, kv)
+
+
+@pytest.mark.parametrize("kv", [1, 2])
+@pytest.mark.parametrize("shape", [(1024, 32, 8, 128, 128, 64, 256), (512, 14, 2, 64, 16, 64, 2048), (64, 28, 4, 128, 24, 8, 700), (8, 6, 1, 64, 7, 1, 1000)])
+def test_trees_over_bytes_need_no_copy_of_the_cache(shape, kv):
+    """The kernel that serves them widens rows on their way: the same scratch as over a 16-bit cache, which a copy would
+    exceed by the whole cache."""
+    assert tree(*shape, kv) <= tree(*shape, 0) < 200 * MB
+
+
+def test_trees_that_other_kernels_serve():
+    """More sequences than the streaming kernel takes: head_dim 128 is read as it is, head_dim 64 copied."""
+    copy = lambda dim, block, blocks: 2 * 2000 * blocks * block * 2 * dim * 2  # noqa: E731
+    assert tree(4000, 4, 2, 128, 16, 2000, 64, 1) < copy(128, 16, 64) // 4
+    assert tree(4000, 4, 2, 64, 16, 2000, 64, 1) >= copy(64, 16, 64)
