@@ -34,6 +34,15 @@ constexpr uint32_t kMinSplit = 256;           // positions a split of the row st
 // a position. 32 sequences of 6000 positions, 8 kv heads of 128, stored / formed twice: 48 rows 334 / 361 us, 64 rows 430 / 342;
 // one of 8000: 48 rows 30 / 30; 28 heads over 4: 56 rows 190 / 181. The scratch grows with the limit.
 constexpr uint32_t kStoredRows = 32;
+// ... and of one sequence: an average says nothing about a chunk beside decode rows. Sequences of more M rows than a tile of the
+// row statistics has go through the other kernels, in launches of their own. All stored / long ones apart: 100 decode rows and a
+// chunk of 300 rows behind 2000 positions (32 heads over 8) 2340 / 171 us, 300 and a chunk of 1000 (28 over 4) 12060 / 337; 64
+// sequences of 1 to 8 rows, none of them long, 159 / 170.
+constexpr uint32_t kLongRows = kRowTile;
+// Stored scores at a time: kv heads beyond it take turns, and where one head's do not fit they are formed twice. The rows are laid
+// out for the widest context that the block tables have room for, whatever the sequences' lengths. (A decode step of 64 sequences
+// over tables of 131072 positions: 1028 MB, 196 us; with a limit of 512 MB and so three heads at a time 408.)
+constexpr size_t kStoredBytes = 1536ull << 20;
 
 template <typename T>
 __device__ __forceinline__ f32x16_t mfma32(const uint4 &a, const uint4 &b, f32x16_t c)
@@ -63,8 +72,10 @@ struct WeightsParams {
     uint32_t m_total;              // total_tokens * G
     uint32_t splits, split_len;
     uint32_t block_magic;          // see block_magic()
-    float *scores;                 // stored scores: [kv head][M row][pitch], in units of log2
+    float *scores;                 // stored scores: [kv head - head0][M row][pitch], in units of log2
     uint32_t pitch;                // positions of a stored row, a multiple of 64
+    uint32_t head0, heads;         // stored scores: the kv heads of a launch
+    uint32_t long_rows;            // M rows of a sequence from which on its scores are formed twice (0: those of all, or of none, are)
 };
 
 // what a workgroup knows about its sequence
@@ -84,10 +95,79 @@ __device__ __forceinline__ Sequence sequence_of(const WeightsParams &p, uint32_t
     return q;
 }
 
+// the n-th sequence whose scores are formed twice, for a whole wave; `batch`: there are fewer
+__device__ __forceinline__ uint32_t long_sequence(const WeightsParams &p, uint32_t n, uint32_t lane)
+{
+    for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
+        const uint32_t i = i0 + lane;
+        uint64_t hits = __ballot(sequence_of(p, min(i, p.batch - 1)).m_rows > p.long_rows && i < p.batch);
+        const uint32_t here = static_cast<uint32_t>(__builtin_popcountll(hits));
+        if (n < here) {
+            for (; n != 0; n--) {
+                hits &= hits - 1;
+            }
+            return i0 + static_cast<uint32_t>(__builtin_ctzll(hits));
+        }
+        n -= here;
+    }
+    return p.batch;
+}
+
 __device__ __forceinline__ uint64_t slot_of(const WeightsParams &p, const int32_t *table, uint32_t pos)
 {
     const uint32_t b = p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size;
     return static_cast<uint64_t>(static_cast<uint32_t>(table[b])) * p.block_size + (pos - b * p.block_size);
+}
+
+// Row tile blockIdx.x of the row statistics, for a whole wave: its sequence and number inside it (which may lie behind its last
+// one). False: there is none. The tiles of a sequence are numbered from floor(start * G / TILE) + i (a formula of the prefix sums, at
+// least as many ids as it has tiles), or evenly when a window bounds the counted rows; beside stored scores those of the long
+// sequences are counted one after the other.
+template <uint32_t TILE>
+__device__ __forceinline__ bool row_tile_of(const WeightsParams &p, uint32_t lane, uint32_t *seq, uint32_t *mt)
+{
+    if (p.long_rows != 0) {
+        uint32_t left = blockIdx.x;
+        for (uint32_t i0 = 0; i0 < p.batch; i0 += 64) {
+            const uint32_t rows = sequence_of(p, min(i0 + lane, p.batch - 1)).m_rows;
+            const uint32_t tiles = i0 + lane < p.batch && rows > p.long_rows ? ceil_div(rows, TILE) : 0u;
+            uint32_t incl = tiles;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t up = __shfl_up(incl, d);
+                incl += lane >= static_cast<uint32_t>(d) ? up : 0u;
+            }
+            const uint64_t behind = __ballot(incl > left);   // the first of these holds the tile
+            if (behind != 0) {
+                const int at = __builtin_ctzll(behind);
+                *seq = i0 + static_cast<uint32_t>(at);
+                *mt = left - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(incl - tiles), at));
+                return true;
+            }
+            left -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(incl), 63));
+        }
+        return false;
+    }
+    if (p.tiles_per_seq != 0) {
+        *seq = blockIdx.x / p.tiles_per_seq;
+        *mt = blockIdx.x % p.tiles_per_seq;
+        return true;
+    }
+    auto first_id = [&](uint32_t i) {
+        return static_cast<uint32_t>(static_cast<uint64_t>(p.query_start_loc[i]) * p.group / TILE) + i;
+    };
+    uint32_t at = 0, hi = p.batch;
+    while (hi - at > 1) {
+        const uint32_t mid = (at + hi) >> 1;
+        if (first_id(mid) <= blockIdx.x) {
+            at = mid;
+        } else {
+            hi = mid;
+        }
+    }
+    *seq = at;
+    *mt = blockIdx.x - first_id(at);
+    return true;
 }
 
 // chunk c (eight elements) of a cache row as T; a byte cache's values exactly, without their scale
@@ -119,26 +199,9 @@ row_stats_kernel(const WeightsParams p)
     const uint32_t kvh = blockIdx.z, split = blockIdx.y, G = p.group;
     constexpr uint32_t TILE = 4 * 32 * RT;
 
-    // ---- which rows: the tiles of a sequence are numbered from floor(start * G / tile) + i (a formula of the prefix sums,
-    // at least as many ids as it has tiles), or evenly when a window bounds the counted rows
-    uint32_t seq = 0, mt;
-    if (p.tiles_per_seq != 0) {
-        seq = blockIdx.x / p.tiles_per_seq;
-        mt = blockIdx.x % p.tiles_per_seq;
-    } else {
-        auto first_id = [&](uint32_t i) {
-            return static_cast<uint32_t>(static_cast<uint64_t>(p.query_start_loc[i]) * G / TILE) + i;
-        };
-        uint32_t hi = p.batch;
-        while (hi - seq > 1) {
-            const uint32_t mid = (seq + hi) >> 1;
-            if (first_id(mid) <= blockIdx.x) {
-                seq = mid;
-            } else {
-                hi = mid;
-            }
-        }
-        mt = blockIdx.x - first_id(seq);
+    uint32_t seq, mt;
+    if (!row_tile_of<TILE>(p, lane, &seq, &mt)) {
+        return;
     }
     const Sequence s = sequence_of(p, seq);
     const uint32_t m_wave = mt * TILE + wave * 32 * RT;
@@ -282,24 +345,9 @@ row_stats_staged_kernel(const WeightsParams p)
     const uint32_t smem_addr = stage::lds_address(smem);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const uint32_t kvh = blockIdx.z, split = blockIdx.y, G = p.group;
-    uint32_t seq = 0, mt;
-    if (p.tiles_per_seq != 0) {
-        seq = blockIdx.x / p.tiles_per_seq;
-        mt = blockIdx.x % p.tiles_per_seq;
-    } else {
-        auto first_id = [&](uint32_t i) {
-            return static_cast<uint32_t>(static_cast<uint64_t>(p.query_start_loc[i]) * G / TILE) + i;
-        };
-        uint32_t hi = p.batch;
-        while (hi - seq > 1) {
-            const uint32_t mid = (seq + hi) >> 1;
-            if (first_id(mid) <= blockIdx.x) {
-                seq = mid;
-            } else {
-                hi = mid;
-            }
-        }
-        mt = blockIdx.x - first_id(seq);
+    uint32_t seq, mt;
+    if (!row_tile_of<TILE>(p, lane, &seq, &mt)) {
+        return;
     }
     const Sequence s = sequence_of(p, seq);
     const uint32_t m_first = mt * TILE;
@@ -505,7 +553,11 @@ column_sums_kernel(const WeightsParams p)
     __shared__ float other[TURNS][4][32 * PT];
     const uint32_t smem_addr = stage::lds_address(smem);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    const uint32_t kvh = blockIdx.z, seq = blockIdx.y, G = p.group;
+    const uint32_t kvh = blockIdx.z, G = p.group;
+    const uint32_t seq = p.long_rows == 0 ? blockIdx.y : long_sequence(p, blockIdx.y, lane);
+    if (seq >= p.batch) {
+        return;
+    }
     const uint32_t mine = wave & 3u, turn = wave >> 2;   // which 64 positions, and which 32 of the staged rows
     const Sequence s = sequence_of(p, seq);
     const uint32_t total = s.cached + s.nodes;
@@ -726,14 +778,15 @@ store_scores_kernel(const WeightsParams p)
     constexpr int KS = D / 32, NT = Tile::BN / 16, S = Tile::STAGES, C = Tile::C;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, jq = lane >> 4;
-    const uint32_t heads = min(p.n_kv_heads, kStoredWaves), per_wg = kStoredWaves / heads;   // kv heads and chunks of a workgroup
-    const uint32_t parts = ceil_div(p.n_kv_heads, heads);
-    const uint32_t kvh = blockIdx.x % parts * heads + wave % heads, chunk = blockIdx.x / parts * per_wg + wave / heads;
+    const uint32_t heads = min(p.heads, kStoredWaves), per_wg = kStoredWaves / heads;   // kv heads and chunks of a workgroup
+    const uint32_t parts = ceil_div(p.heads, heads);
+    const uint32_t local = blockIdx.x % parts * heads + wave % heads, chunk = blockIdx.x / parts * per_wg + wave / heads;
+    const uint32_t kvh = p.head0 + local;
     const uint32_t seq = blockIdx.y, G = p.group;
     const Sequence s = sequence_of(p, seq);
     const uint32_t total = s.cached + s.nodes;
     const uint32_t begin = chunk * p.split_len, end = min(total, begin + p.split_len);
-    if (wave >= heads * per_wg || kvh >= p.n_kv_heads || s.nodes == 0 || chunk >= p.splits) {
+    if (wave >= heads * per_wg || local >= p.heads || s.nodes == 0 || chunk >= p.splits || (p.long_rows != 0 && s.m_rows > p.long_rows)) {
         return;
     }
     const uint32_t entries = stored_table(p.split_len, p.block_size);
@@ -741,7 +794,7 @@ store_scores_kernel(const WeightsParams p)
     uint32_t *tbl = reinterpret_cast<uint32_t *>(ring + Tile::RING);
     const uint32_t ring_addr = stage::lds_address(smem) + wave * (Tile::RING + entries * 4);
     const uint32_t base = stored_base(p, seq, s);
-    const uint64_t rows0 = static_cast<uint64_t>(kvh) * p.m_total + base;
+    const uint64_t rows0 = static_cast<uint64_t>(local) * p.m_total + base;
     auto block_of = [&](uint32_t pos) __attribute__((always_inline)) { return p.block_magic != 0 ? __umulhi(pos, p.block_magic) : pos / p.block_size; };
     const uint32_t blk0 = block_of(begin);
     if (begin < end) {
@@ -861,7 +914,7 @@ store_scores_kernel(const WeightsParams p)
             m_run = m_all;
         }
         if (jq == 0 && m0 + col < s.m_rows) {
-            *reinterpret_cast<float2 *>(p.stats + (static_cast<uint64_t>(chunk) * p.n_kv_heads * p.m_total + rows0 + m0 + col) * 2) =
+            *reinterpret_cast<float2 *>(p.stats + (static_cast<uint64_t>(chunk) * p.heads * p.m_total + rows0 + m0 + col) * 2) =
                 make_float2(m_run, l_run);
         }
     }
@@ -874,15 +927,15 @@ sum_scores_kernel(const WeightsParams p)
     const uint32_t seq = blockIdx.y, G = p.group;
     const Sequence s = sequence_of(p, seq);
     const uint32_t total = s.cached + s.nodes, t = blockIdx.x * kThreads + threadIdx.x;
-    if (s.nodes == 0 || t >= total) {
+    if (s.nodes == 0 || t >= total || (p.long_rows != 0 && s.m_rows > p.long_rows)) {
         return;
     }
     const int32_t *table = p.block_tables + static_cast<uint64_t>(seq) * p.max_num_block;
-    float *w = p.weights + slot_of(p, table, t) * p.n_kv_heads;
+    float *w = p.weights + slot_of(p, table, t) * p.n_kv_heads + p.head0;
     const uint32_t base = stored_base(p, seq, s);
     // rows that see the position: from the first counted row r with s.cached + r >= t on
     const uint32_t m_first = t > s.cached + s.first ? (t - s.cached - s.first) * G : 0u;
-    for (uint32_t kvh = blockIdx.z; kvh < p.n_kv_heads; kvh += gridDim.z) {
+    for (uint32_t kvh = blockIdx.z; kvh < p.heads; kvh += gridDim.z) {   // (from head0 on)
         const uint64_t rows0 = static_cast<uint64_t>(kvh) * p.m_total + base;
         const float *norm = p.norm + rows0;
         const float *score = p.scores + rows0 * p.pitch + t;
@@ -907,11 +960,19 @@ sum_scores_kernel(const WeightsParams p)
 }
 
 // ---- the plan of a call: which kernels, how many pieces, how much scratch -----------------------------------------------------
+// Scores stored (`heads` kv heads at a time), formed twice, or the one for the short and the other for the long sequences of a batch.
 struct Plan {
-    bool stored;                 // the scores are stored
-    uint32_t rows;               // M rows of a kv head that the scratch is laid out for
-    uint32_t tiles, tiles_per_seq, splits, split_len, pitch, window;
-    size_t bytes;
+    uint32_t window, long_rows;
+    struct Stored {
+        uint32_t heads;          // 0: none
+        uint32_t rows;           // M rows of a kv head that the scratch is laid out for
+        uint32_t splits, split_len, pitch;
+    } stored;
+    struct Formed {
+        uint32_t sequences;      // that may be formed twice (0: none)
+        uint32_t rows, tiles, tiles_per_seq, splits, split_len;
+    } formed;
+    size_t bytes;                // (the parts of a call take turns in the same scratch)
 };
 
 Plan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t batch,
@@ -923,35 +984,49 @@ Plan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint3
     // counted rows: at most `window` per sequence, at most every row
     const uint64_t bounded = window == 0 ? total_tokens : static_cast<uint64_t>(window) * batch;
     const uint64_t counted = std::min<uint64_t>(bounded, total_tokens);
-    plan.stored = counted * G <= static_cast<uint64_t>(kStoredRows) * batch && bounded * n_heads < (1ull << 31);
-    if (plan.stored) {
-        plan.rows = static_cast<uint32_t>(bounded) * G;
-        plan.pitch = ceil_div(max_ctx, 64u) * 64u;
-        // chunks of 64 to 512 positions: the longest that leave 4096 waves (16 per compute unit; 12 fit)
-        const uint64_t waves64 = static_cast<uint64_t>(batch) * ceil_div(max_ctx, 64u) * n_kv_heads;
-        plan.split_len = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(8, waves64 / 4096))) * 64u;
-        plan.splits = ceil_div(max_ctx, plan.split_len);
-        const size_t rows = static_cast<size_t>(plan.rows) * n_kv_heads;
-        plan.bytes = ((rows + 3) / 4 * 4 + rows * plan.pitch + 2 * rows * plan.splits) * sizeof(float);
-        return plan;
+    if (counted * G <= static_cast<uint64_t>(kStoredRows) * batch && bounded * n_heads < (1ull << 31)) {
+        const uint32_t rows = static_cast<uint32_t>(bounded) * G;
+        const uint32_t pitch = ceil_div(max_ctx, 64u) * 64u;
+        // what a kv head takes: a normaliser and a score a position for every row, two statistics for every 64 positions at the most
+        const size_t of_head = static_cast<size_t>(rows) * (pitch + pitch / 32 + 1) * sizeof(float);
+        uint32_t heads = static_cast<uint32_t>(std::min<size_t>(n_kv_heads, kStoredBytes / of_head));
+        heads = heads < n_kv_heads && heads > kStoredWaves ? heads / kStoredWaves * kStoredWaves : heads;
+        if (heads != 0) {
+            plan.stored = {heads, rows, 0, 0, pitch};
+            // chunks of 64 to 512 positions: the longest that leave 4096 waves (16 per compute unit; 12 fit)
+            const uint64_t waves64 = static_cast<uint64_t>(batch) * ceil_div(max_ctx, 64u) * heads;
+            plan.stored.split_len = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(8, waves64 / 4096))) * 64u;
+            plan.stored.splits = ceil_div(max_ctx, plan.stored.split_len);
+            const size_t all = static_cast<size_t>(rows) * heads;
+            plan.bytes = ((all + 3) / 4 * 4 + all * pitch + 2 * all * plan.stored.splits) * sizeof(float);
+            // how long a sequence may be while each of the others has a row. (Beside empty ones a longer one is possible: its scores
+            // are stored like the others'. A call of one row a sequence must not pay for launches that find nothing to do.)
+            const uint64_t others = batch - 1u, longest = total_tokens > others ? total_tokens - others : 1u;
+            if ((window == 0 ? longest : std::min<uint64_t>(longest, window)) * G <= kLongRows) {
+                return plan;
+            }
+            plan.long_rows = kLongRows;
+        }
     }
-    plan.rows = total_tokens * G;
+    Plan::Formed &f = plan.formed;
+    f.sequences = plan.long_rows == 0 ? batch : static_cast<uint32_t>(counted * G / (plan.long_rows + 1));   // (fewer than the batch: see the average)
+    f.rows = total_tokens * G;
     const uint32_t tile = head_dim == 256 ? kRowTile / 2 : kRowTile;
     const uint64_t of_window = window == 0 ? 0 : static_cast<uint64_t>(std::min(window, total_tokens)) * G;
-    plan.tiles_per_seq = static_cast<uint32_t>((of_window + tile - 1) / tile);
-    const uint32_t by_prefix = ceil_div(total_tokens * G, tile) + batch;
-    if (plan.tiles_per_seq != 0 && static_cast<uint64_t>(plan.tiles_per_seq) * batch <= by_prefix) {
-        plan.tiles = plan.tiles_per_seq * batch;
+    f.tiles_per_seq = static_cast<uint32_t>((of_window + tile - 1) / tile);
+    const uint32_t by_prefix = ceil_div(total_tokens * G, tile) + f.sequences;
+    if (plan.long_rows == 0 && f.tiles_per_seq != 0 && static_cast<uint64_t>(f.tiles_per_seq) * batch <= by_prefix) {
+        f.tiles = f.tiles_per_seq * batch;
     } else {
-        plan.tiles_per_seq = 0;
-        plan.tiles = by_prefix;
+        f.tiles_per_seq = 0;
+        f.tiles = by_prefix;
     }
     // splits of the row statistics: enough workgroups (of four waves) for four per compute unit
-    const uint32_t want = ceil_div(2048u, std::max(1u, plan.tiles * n_kv_heads));
-    plan.splits = std::max(1u, std::min(want, max_ctx / kMinSplit));
-    plan.split_len = ceil_div(ceil_div(max_ctx, plan.splits), 32u) * 32u;
+    const uint32_t want = ceil_div(2048u, std::max(1u, f.tiles * n_kv_heads));
+    f.splits = std::max(1u, std::min(want, max_ctx / kMinSplit));
+    f.split_len = ceil_div(ceil_div(max_ctx, f.splits), 32u) * 32u;
     const size_t rows = static_cast<size_t>(total_tokens) * n_heads;
-    plan.bytes = (rows + (plan.splits > 1 ? 2 * plan.splits * rows : 0)) * sizeof(float);
+    plan.bytes = std::max(plan.bytes, (rows + (f.splits > 1 ? 2 * f.splits * rows : 0)) * sizeof(float));
     return plan;
 }
 
@@ -1017,72 +1092,95 @@ extern "C" int xlite_hip_attention_weights(void *stream, const void *qkv, const 
     p.block_size = block_size;
     p.max_num_block = max_num_block;
     p.window = plan.window;
-    p.m_total = plan.rows;
-    p.tiles_per_seq = plan.tiles_per_seq;
-    p.splits = plan.splits;
-    p.split_len = plan.split_len;
+    p.long_rows = plan.long_rows;
     p.block_magic = block_magic(block_size, max_ctx);
-    const uint32_t rows = plan.rows * n_kv_heads;
     p.norm = static_cast<float *>(workspace);
-    if (plan.stored) {
-        p.scores = p.norm + (static_cast<size_t>(rows) + 3) / 4 * 4;   // (16-byte stores)
-        p.pitch = plan.pitch;
-        p.stats = p.scores + static_cast<size_t>(rows) * plan.pitch;
-    } else {
-        p.stats = p.norm + rows;
-    }
-    auto launch = [&](auto t, auto d, auto kvf) -> int {
-        using T = decltype(t);
-        constexpr int D = decltype(d)::value, KVF = decltype(kvf)::value;
-        if (plan.stored) {
-            const uint32_t heads = std::min(n_kv_heads, kStoredWaves);
-            const size_t lds = kStoredWaves * (StoredTile<D, KVF != XLITE_HIP_KV_SAME>::RING + stored_table(plan.split_len, block_size) * sizeof(uint32_t));
-            if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(store_scores_kernel<T, D, KVF>), lds)) {
-                return rc;
-            }
-            store_scores_kernel<T, D, KVF><<<dim3(ceil_div(plan.splits, kStoredWaves / heads) * ceil_div(n_kv_heads, heads), batch),
-                                             64 * kStoredWaves, lds, s>>>(p);
+    // (16 splits of 2048 rows: 4.7 us either way; 251 of 16 rows: 64 us with a lane a row)
+    auto join = [&](uint32_t rows, uint32_t splits) -> int {
+        if (splits < 16) {
+            join_stats_kernel<1><<<ceil_div(rows, 256u), 256, 0, s>>>(p.stats, p.norm, rows, splits);
         } else {
-            // K through LDS: 16-bit caches whose copies (two positions of 256 elements, four of 128, eight of 64) lie in one block, and a
-            // split's block-table entries behind the stages
-            bool staged = false;
-            if constexpr (KVF == XLITE_HIP_KV_SAME) {
-                const size_t lds = 3 * kStagedPositions<D> * D * 2 + (static_cast<size_t>(plan.split_len / block_size) + 2) * sizeof(uint32_t);
-                staged = block_size % (512 / D) == 0 && p.block_magic != 0 && lds <= 64 * 1024;
-                if (staged) {
-                    if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(row_stats_staged_kernel<T, D>), lds)) {
-                        return rc;
-                    }
-                    row_stats_staged_kernel<T, D><<<dim3(plan.tiles, plan.splits, n_kv_heads), kThreads, lds, s>>>(p);
-                }
-            }
-            if (!staged) {
-                row_stats_kernel<T, D, KVF><<<dim3(plan.tiles, plan.splits, n_kv_heads), kThreads, 0, s>>>(p);
-            }
-        }
-        XL_LAUNCH_CHECK();
-        if (plan.stored || plan.splits > 1) {
-            // (16 splits of 2048 rows: 4.7 us either way; 251 of 16 rows: 64 us with a lane a row)
-            if (plan.splits < 16) {
-                join_stats_kernel<1><<<ceil_div(rows, 256u), 256, 0, s>>>(p.stats, p.norm, rows, plan.splits);
-            } else {
-                join_stats_kernel<16><<<ceil_div(rows, 16u), 256, 0, s>>>(p.stats, p.norm, rows, plan.splits);
-            }
-            XL_LAUNCH_CHECK();
-        }
-        if (plan.stored) {
-            const uint32_t tiles = ceil_div(max_ctx, static_cast<uint32_t>(kThreads));
-            const uint32_t z = std::max(1u, std::min(n_kv_heads, 512u / std::max(1u, tiles * batch)));   // few positions: the heads side by side
-            sum_scores_kernel<<<dim3(tiles, batch, z), kThreads, 0, s>>>(p);
-        } else {
-            const size_t lds = 3 * kTurns<D> * (32 * D * 2 + 4 * 256);
-            if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(column_sums_kernel<T, D, KVF>), lds)) {
-                return rc;
-            }
-            column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 128u * kColumnTiles<D>), batch, n_kv_heads), kTurns<D> * kThreads, lds, s>>>(p);
+            join_stats_kernel<16><<<ceil_div(rows, 16u), 256, 0, s>>>(p.stats, p.norm, rows, splits);
         }
         XL_LAUNCH_CHECK();
         return XLITE_HIP_OK;
+    };
+    auto stored = [&](auto t, auto d, auto kvf) -> int {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value, KVF = decltype(kvf)::value;
+        p.m_total = plan.stored.rows;
+        p.splits = plan.stored.splits;
+        p.split_len = plan.stored.split_len;
+        p.pitch = plan.stored.pitch;
+        const size_t lds = kStoredWaves * (StoredTile<D, KVF != XLITE_HIP_KV_SAME>::RING + stored_table(p.split_len, block_size) * sizeof(uint32_t));
+        if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(store_scores_kernel<T, D, KVF>), lds)) {
+            return rc;
+        }
+        for (p.head0 = 0; p.head0 < n_kv_heads; p.head0 += plan.stored.heads) {
+            p.heads = std::min(plan.stored.heads, n_kv_heads - p.head0);
+            const uint32_t rows = p.m_total * p.heads, heads = std::min(p.heads, kStoredWaves);
+            p.scores = p.norm + (static_cast<size_t>(rows) + 3) / 4 * 4;   // (16-byte stores)
+            p.stats = p.scores + static_cast<size_t>(rows) * p.pitch;
+            store_scores_kernel<T, D, KVF><<<dim3(ceil_div(p.splits, kStoredWaves / heads) * ceil_div(p.heads, heads), batch),
+                                             64 * kStoredWaves, lds, s>>>(p);
+            XL_LAUNCH_CHECK();
+            if (const int rc = join(rows, p.splits)) {
+                return rc;
+            }
+            const uint32_t tiles = ceil_div(max_ctx, static_cast<uint32_t>(kThreads));
+            const uint32_t z = std::max(1u, std::min(p.heads, 512u / std::max(1u, tiles * batch)));   // few positions: the heads side by side
+            sum_scores_kernel<<<dim3(tiles, batch, z), kThreads, 0, s>>>(p);
+            XL_LAUNCH_CHECK();
+        }
+        return XLITE_HIP_OK;
+    };
+    auto formed = [&](auto t, auto d, auto kvf) -> int {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value, KVF = decltype(kvf)::value;
+        const Plan::Formed &f = plan.formed;
+        const uint32_t rows = f.rows * n_kv_heads;
+        p.m_total = f.rows;
+        p.tiles_per_seq = f.tiles_per_seq;
+        p.splits = f.splits;
+        p.split_len = f.split_len;
+        p.stats = p.norm + rows;
+        // K through LDS: 16-bit caches whose copies (two positions of 256 elements, four of 128, eight of 64) lie in one block, and a
+        // split's block-table entries behind the stages
+        bool staged = false;
+        if constexpr (KVF == XLITE_HIP_KV_SAME) {
+            const size_t lds = 3 * kStagedPositions<D> * D * 2 + (static_cast<size_t>(p.split_len / block_size) + 2) * sizeof(uint32_t);
+            staged = block_size % (512 / D) == 0 && p.block_magic != 0 && lds <= 64 * 1024;
+            if (staged) {
+                if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(row_stats_staged_kernel<T, D>), lds)) {
+                    return rc;
+                }
+                row_stats_staged_kernel<T, D><<<dim3(f.tiles, p.splits, n_kv_heads), kThreads, lds, s>>>(p);
+            }
+        }
+        if (!staged) {
+            row_stats_kernel<T, D, KVF><<<dim3(f.tiles, p.splits, n_kv_heads), kThreads, 0, s>>>(p);
+        }
+        XL_LAUNCH_CHECK();
+        if (p.splits > 1) {
+            if (const int rc = join(rows, p.splits)) {
+                return rc;
+            }
+        }
+        const size_t lds = 3 * kTurns<D> * (32 * D * 2 + 4 * 256);
+        if (const int rc = ensure_dynamic_lds(reinterpret_cast<const void *>(column_sums_kernel<T, D, KVF>), lds)) {
+            return rc;
+        }
+        column_sums_kernel<T, D, KVF><<<dim3(ceil_div(max_ctx, 128u * kColumnTiles<D>), f.sequences, n_kv_heads), kTurns<D> * kThreads, lds, s>>>(p);
+        XL_LAUNCH_CHECK();
+        return XLITE_HIP_OK;
+    };
+    auto launch = [&](auto t, auto d, auto kvf) -> int {
+        if (plan.stored.heads != 0) {
+            if (const int rc = stored(t, d, kvf)) {
+                return rc;
+            }
+        }
+        return plan.formed.sequences != 0 ? formed(t, d, kvf) : XLITE_HIP_OK;
     };
     auto with_dim = [&](auto t, auto kvf) -> int {
         using D64 = std::integral_constant<int, 64>;

@@ -23,3 +23,20 @@ def test_trees_that_other_kernels_serve():
     copy = lambda dim, block, blocks: 2 * 2000 * blocks * block * 2 * dim * 2  # noqa: E731
     assert tree(4000, 4, 2, 128, 16, 2000, 64, 1) < copy(128, 16, 64) // 4
     assert tree(4000, 4, 2, 64, 16, 2000, 64, 1) >= copy(64, 16, 64)
+
+
+def weights(tokens, heads, kv_heads, dim, block, batch, blocks, window=0):
+    return _lib.load().xlite_hip_attention_weights_workspace_bytes(tokens, heads, kv_heads, dim, block, batch, blocks, window)
+
+
+@pytest.mark.parametrize("shape", [(512, 32, 8, 128, 128, 512, 256), (64, 32, 8, 128, 16, 64, 8192), (512, 32, 8, 128, 128, 64, 256), (1300, 28, 4, 128, 128, 301, 64),
+                                   (64, 64, 1, 64, 16, 64, 1 << 20), (4096, 28, 4, 128, 128, 64, 256, 8)])
+def test_stored_scores_are_bounded(shape):
+    """Decode steps, short steps and chunks of wide tables: what is stored of the scores at a time stays below 1.5 GB,
+    the normalisers and statistics of scores that are not stored below 64 MB."""
+    assert 0 < weights(*shape) <= 1600 * MB
+
+
+def test_one_row_a_sequence_is_not_laid_out_for_more():
+    """64 rows of 32 heads over tables of 4096 positions: a score of 4 bytes each, and their statistics."""
+    assert weights(64, 32, 8, 128, 128, 64, 32) < 1.1 * 64 * 32 * 4096 * 4
