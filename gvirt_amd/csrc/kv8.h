@@ -10,6 +10,11 @@
 namespace xlite {
 
 __device__ __forceinline__ float clamp_f16(float x) { return fminf(fmaxf(x, -65504.f), 65504.f); }
+// the same for queries, whose NaNs stay NaNs
+__device__ __forceinline__ float saturate_f16(float x)
+{
+    return __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -65504.f), 65504.f);
+}
 
 template <typename T, int KVF>
 __device__ __forceinline__ uint4 dequant8(const uint2 &raw, float scale)
@@ -60,7 +65,7 @@ __device__ __forceinline__ uint4 widen8(const uint2 &raw)
     }
 }
 
-// eight 16-bit values of storage type FROM as type TO
+// eight 16-bit values (of a query) of storage type FROM as type TO
 template <typename FROM, typename TO>
 __device__ __forceinline__ uint4 convert8(const uint4 &x)
 {
@@ -68,7 +73,7 @@ __device__ __forceinline__ uint4 convert8(const uint4 &x)
         return x;
     } else {
         auto one = [](uint32_t w) {
-            return TO::pack(fminf(fmaxf(FROM::lo(w), -65504.f), 65504.f), fminf(fmaxf(FROM::hi(w), -65504.f), 65504.f));
+            return TO::pack(saturate_f16(FROM::lo(w)), saturate_f16(FROM::hi(w)));
         };
         return make_uint4(one(x.x), one(x.y), one(x.z), one(x.w));
     }

@@ -84,7 +84,7 @@ dequant_blocks_kernel(const unsigned char *__restrict__ k_cache, const unsigned 
 __global__ void __launch_bounds__(256)
 rows_bf16_to_f16_kernel(const uint16_t *__restrict__ src, uint16_t *__restrict__ dst, uint64_t n_oct)
 {
-    auto one = [](uint32_t w) { return FP16::pack(clamp_f16(BF16::lo(w)), clamp_f16(BF16::hi(w))); };
+    auto one = [](uint32_t w) { return FP16::pack(saturate_f16(BF16::lo(w)), saturate_f16(BF16::hi(w))); };
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n_oct; i += gridDim.x * 256ull) {
         const uint4 w = reinterpret_cast<const uint4 *>(src)[i];
         reinterpret_cast<uint4 *>(dst)[i] = make_uint4(one(w.x), one(w.y), one(w.z), one(w.w));

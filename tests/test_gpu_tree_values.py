@@ -1,12 +1,13 @@
-"""Infinities and NaNs that the rows of a tree see."""
+"""Infinities and NaNs that the rows of a tree see, and queries that are NaN."""
 import pytest
 import torch
 
+from gvirt_amd import workloads as W
 from test_gpu_tree import make, run
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
-BF = torch.bfloat16
+BF, FP = torch.bfloat16, torch.float16
 
 
 @pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (256, 16), (64, 5), (128, 5), (256, 6)])
@@ -40,3 +41,29 @@ def test_values_that_some_rows_see_beside_values_that_all_see(rt):
                 assert (x[r] != x[r]).all()
             else:
                 assert (x[r] == float("inf")).all()
+
+
+@pytest.mark.parametrize("cache", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (64, 1)])     # (blocks of one: through the 16-bit copy)
+def test_queries_that_are_nan_over_caches_of_bytes(rt, D, bs, dtype, cache):
+    clean, dirty = (make(12, [9, 40], [70, 5], 4, 2, D, bs, dtype, cache) for _ in range(2))
+    dirty["qkv"].view(-1, 8, D)[11, 1, 7] = float("nan")
+    a, b = run(rt, clean).view(-1, 4, D), run(rt, dirty).view(-1, 4, D)
+    assert (b[11, 1] != b[11, 1]).all()
+    b[11, 1] = a[11, 1]
+    assert torch.equal(a, b)
+
+
+def test_queries_that_are_nan_in_the_causal_kernel(rt):
+    """The same conversion of queries serves chunks over a cache of bytes."""
+    from gvirt_amd._C import attention
+    for limit in (None, 64):     # through the 16-bit copy, and read on the fly
+        w = make(12, [40], [70], 4, 2, 128, 16, BF, "int8", spare=0)
+        w["qkv"].view(-1, 8, 128)[11, 1, 7] = float("nan")
+        d = W.to_device({k: v for k, v in w.items() if isinstance(v, torch.Tensor)}, DEV)
+        out = torch.zeros(40, 4 * 128, dtype=BF, device=DEV)
+        attention(rt, d["qkv"], d["k"], d["v"], out, d["qsl"], d["lens"], d["clens"], d["tables"], 4, 2, 128, 16, 1, w["mb"], k_scale=d["ks"],
+                  v_scale=d["vs"], workspace_limit=limit)
+        bad = torch.isnan(out.float().view(40, 4, 128)).cpu()
+        assert bad[11, 1].all() and bad.sum() == 128
