@@ -53,7 +53,9 @@ constexpr uint32_t kRawStage = kWaves * kWaveRaw;
 constexpr uint32_t kScales = 3 * 64 * 4;         // of a widened stage: three numbers per (kv head, position)
 template <bool RAW>
 constexpr uint32_t kStageBytes = RAW ? 2 * (kStage + kScales) + kStages * kRawStage : kStages * kStage;
-constexpr float kLeastScale = 0x1p-100f;         // of a V row, in the arithmetic of its logarithm and reciprocal
+// Of a V row, in the arithmetic of its logarithm and reciprocal; the largest is its inverse. A row of the least scale beside one of the
+// largest has its probability times 2^-100 in the exponential, which fp32 holds down to 2^-126, and gets the normaliser's share back.
+constexpr float kLeastScale = 0x1p-50f;
 constexpr uint32_t kTblCap = 2048;               // block-table entries staged per segment
 constexpr uint32_t kSeqCap = 1024;               // sequences whose prefix sums fit
 constexpr uint32_t kMaskCap = kThreads;          // mask words of an M tile kept in LDS: 128 rows of 4 heads and 512 nodes

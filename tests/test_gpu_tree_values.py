@@ -1,9 +1,10 @@
-"""Infinities and NaNs that the rows of a tree see, and queries that are NaN."""
+"""What does not have ordinary values: infinities and NaNs that the rows of a tree see, queries that are NaN, and V scales
+of a cache of bytes from nothing to the largest."""
 import pytest
 import torch
 
 from gvirt_amd import workloads as W
-from test_gpu_tree import make, run
+from test_gpu_tree import check, make, run
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -67,3 +68,16 @@ def test_queries_that_are_nan_in_the_causal_kernel(rt):
                   v_scale=d["vs"], workspace_limit=limit)
         bad = torch.isnan(out.float().view(40, 4, 128)).cpu()
         assert bad[11, 1].all() and bad.sum() == 128
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cache", ["int8", "fp8"])
+def test_v_scales_from_nothing_to_the_largest(rt, D, cache):
+    """Positions of scale zero keep their weight in the normaliser beside positions of scale 2^50."""
+    w = make(14, [9, 3], [300, 40], 4, 2, D, 16, BF, cache)
+    g = torch.Generator().manual_seed(2)
+    w["vs"] = torch.full(w["vs"].shape, 2.0 ** 50)
+    w["vs"][torch.rand(w["vs"].shape, generator=g) < 0.5] = 0.0
+    check(run(rt, w), w)
+    w["vs"] *= 2.0 ** -80     # and of small ones
+    check(run(rt, w), w)
