@@ -387,7 +387,7 @@ tree_stream_kernel(const StreamParams p)
                         to[0] = scale * kLog2e;
                     } else {
                         const float vs = fminf(fmaxf(scale, kLeastScale), 1.0f / kLeastScale);
-                        to[64] = __log2f(vs);
+                        to[64] = scale != scale ? scale : __log2f(vs);   // (a NaN: of the scores, so that only rows that see it get it)
                         to[128] = 1.0f / vs;
                     }
                 }

@@ -458,9 +458,9 @@ int xlite_hip_prepare_tree(const uint32_t *lens, const uint32_t *cached_lens, co
  * ancestors; bits from lens[i] on are ignored, nodes from 32 * mask_words on are seen by nobody).
  * mask_words <= 2^22. A row that sees nothing gets zeros. Infinities and NaNs in rows that a row does not see do not
  * reach it. Everything else as in xlite_hip_attention (quantised caches: head_dim 64 or 128;
- * v_scale is not negative, and counts as 2^-50 below and as 2^50 above; shapes that go through a
+ * v_scale is not negative, and counts as 2^-50 below and as 2^50 above, a NaN stays one; shapes that go through a
  * widened copy - blocks of one position, more than 1024 sequences, less workspace - saturate
- * values at 65504 there, as xlite_hip_attention does).
+ * values at 65504 there and take NaNs for -65504, as xlite_hip_attention does).
  * workspace: xlite_hip_tree_attention_workspace_bytes(); with less another kernel serves the
  * batch, in the end without splitting the KV axis (one over a quantised cache that needs a 16-bit
  * copy fails with XLITE_HIP_ENOSPC). qkv, caches, output and workspace: aligned to 16 bytes.

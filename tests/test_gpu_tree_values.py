@@ -72,6 +72,20 @@ def test_queries_that_are_nan_in_the_causal_kernel(rt):
 
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("cache", ["int8", "fp8"])
+def test_v_scales_that_are_nan_reach_the_rows_that_see_them(rt, D, cache):
+    for node in (2, -3):     # a node, a cached position of the tile that the tree begins in
+        clean, dirty = (make(13, [6], [21], 4, 2, D, 16, FP, cache) for _ in range(2))
+        p = 21 + node
+        dirty["vs"][int(dirty["tables"][p // 16]), p % 16, 1] = float("nan")
+        a, b = run(rt, clean).view(-1, 4, D), run(rt, dirty).view(-1, 4, D)
+        for r in range(6):
+            sees = node < 0 or int(clean["mask"][r, 0]) >> node & 1
+            assert torch.isnan(b[r, 2:]).all() if sees else torch.equal(a[r], b[r])
+            assert torch.equal(a[r, :2], b[r, :2])     # (the other kv head's)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cache", ["int8", "fp8"])
 def test_v_scales_from_nothing_to_the_largest(rt, D, cache):
     """Positions of scale zero keep their weight in the normaliser beside positions of scale 2^50."""
     w = make(14, [9, 3], [300, 40], 4, 2, D, 16, BF, cache)
