@@ -8,18 +8,18 @@ namespace xlite {
 namespace stage {
 
 // One wave-wide copy of 1 KiB into LDS at `lds_addr` + 16 * lane, from base + voff (a lane's own). The compiler sees neither
-// the LDS write nor the memory counter: completion is awaited with wait<N> (at most N later copies outstanding). The scalar
-// base must come out of scalar arithmetic: a register that a readlane wrote needs five wait states before a memory
-// instruction reads it, which nobody inserts here.
+// the LDS write nor the memory counter: completion is awaited with wait<N> (at most N later copies outstanding). A register that
+// a lane read wrote (the base itself, or a spilled half of it) needs five wait states before a memory instruction reads it, which
+// the compiler does not insert in front of what it does not see: the copy brings them.
 __device__ __forceinline__ void copy_1k(uint32_t lds_addr, uint32_t voff, const void *base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
                  :: "s"(lds_addr), "v"(voff), "s"(base) : "memory", "m0");
 }
 // the same for bytes that nobody reads again: they displace nothing on their way through the caches
 __device__ __forceinline__ void copy_1k_once(uint32_t lds_addr, uint32_t voff, const void *base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\t"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\t"
                  :: "s"(lds_addr), "v"(voff), "s"(base) : "memory", "m0");
 }
 // the same from an address per lane, 16 or 4 bytes each
