@@ -198,7 +198,10 @@ def generate_tree(model: DecoderModel, prompt_tokens: List[List[int]], draft: Ca
     if model.is_mla:
         raise RuntimeError("generate_tree: drafted trees need multi-head attention layers")
     out: List[List[int]] = [[] for _ in range(n)]
-    cached, live = [len(t) for t in prompt_tokens], [True] * n
+    cached = [len(t) for t in prompt_tokens]
+    live = [c > 0 for c in cached]               # (nothing follows an empty prompt, as in generate_ragged)
+    if not any(live) or max_new_tokens <= 0:
+        return out, 0
     flat = torch.tensor([t for p in prompt_tokens for t in p], dtype=torch.int32, device=dev)
     last = model.forward_tokens(flat, cached, [0] * n).argmax(dim=-1).tolist()     # not in the cache yet
     step = 1
@@ -213,7 +216,7 @@ def generate_tree(model: DecoderModel, prompt_tokens: List[List[int]], draft: Ca
         live[i] = len(out[i]) < max_new_tokens
 
     for i in range(n):      # (a token that the cache has no room for is not taken, as in generate_ragged)
-        live[i] = cached[i] + 1 <= model.max_seq_len
+        live[i] = live[i] and cached[i] + 1 <= model.max_seq_len
         take(i, last[i])
     while any(live):
         tokens, parents = [], []
