@@ -12,8 +12,8 @@
 //   column sums: a wave owns 64 positions as the columns of S = Q K^T and walks the M rows, so a position's sum lives in one
 //     lane pair: no atomics, one owner per weight, the same order of additions in every run.
 // Measured, 2 chunks of 2048 rows behind 6144 positions, 28 heads over 4 of 128 elements (210 GFLOP of scores, formed twice): row
-// statistics 245 us, column sums 300, together 0.77 PFLOP/s (a large bf16 product reaches 1.28): the matrix instructions share
-// the SIMDs with 0.8 G exponentials a pass.
+// statistics 227-247 us, column sums 258-291 (settled, after a pause), together 0.78-0.87 PFLOP/s (a large bf16 product reaches 1.28):
+// the matrix instructions share the SIMDs with 0.8 G exponentials a pass.
 #include <algorithm>
 #include <type_traits>
 

@@ -18,10 +18,11 @@ namespace {
 // A weight's neighbours in memory belong to the other kv heads: the heads of a sequence run on one XCD, at the same time, so
 // that its lines come from memory once and from that XCD's L2 for the other heads.
 // Measured, 64 sequences x 8 heads, an eighth kept: 16 us over 4000 positions, 32 over 16000, 58 over 32000, 114 over 64000;
-// one sequence of 32000 34 us. The weights of 64 x 32768 positions are 67 MB, 13 us at the rate of a copy. What bounds it: a wave's
-// keys lie 32 bytes apart, so that a list takes eight times its bytes out of L2 (27 us of the 58 with two lists a compute unit);
-// the histograms take 11, the ballots 3, the output 5, and only two lists' keys fit a compute unit's registers. Two heads a
-// workgroup in neighbouring lanes fetch half the lines: 57 us, but 47 instead of 34 for one sequence.
+// one sequence of 32000 34 us. The weights of 64 x 32768 positions are 67 MB, 13 us at the rate of a copy. What bounds it: the loads,
+// 27 us of the 58. A quarter's keys are converted in the loop that loads them, and the compiler has 16 loads under way only in the first
+// two quarters of 64 keys: in the others every load is awaited before the next, 32 trips to memory in a row (48 with 1024 threads). It
+// is not the bytes out of L2, eight times the list's because a wave's keys lie 32 bytes apart: two heads a workgroup in neighbouring
+// lanes fetch half the lines and took 57 us (and 47 instead of 34 for one sequence). The histograms take 11, the ballots 3, the output 5.
 constexpr uint32_t kXcds = 8;
 constexpr uint32_t kSelTable = 4096;   // block-table entries in LDS
 constexpr int kAhead = 16;   // loads a thread has under way
@@ -316,10 +317,11 @@ select_kept_kernel(const SelectParams p)
 // Position start + i of a sequence receives the row of position start + kept[i], kept[i] >= i, in place. The columns of a
 // row are independent, so a workgroup owns a slice of the rows' bytes (or one fp32 per row: scales, weights) and walks the
 // list in order, a batch of entries at a time: all of a batch is read before any of it is written (a barrier), and what later
-// batches read lies above everything written so far (kept[i] >= i), so the next batch is read ahead of that barrier. Bound
-// by memory: every moved row is read and written once. Measured: 16 sequences of 8192 positions cut to 2048 per head of 8 (128
-// elements of 16 bits, and the weights), 135 MB moved: 61 us, 4.4 TB/s read and written; 64 paths of 6 rows 6 us. Rows of 256
-// bytes of one head are scattered over pages: a plain copy of as many bytes takes 52 us.
+// batches read lies above everything written so far (kept[i] >= i), so the next batch may be read ahead of that barrier. Measured: 16
+// sequences of 8192 positions cut to 2048 per head of 8 (128 elements of 16 bits, and the weights), 135 MB moved: 60 us, 4.5 TB/s
+// read and written (a plain copy of as many bytes takes 52); 64 paths of 6 rows 5.5 us. What bounds it beside the bytes: the table entry
+// comes from LDS or from memory by a choice of addresses, a load that the compiler awaits together with everything else, so that
+// the rows of a batch are fetched one after the other; a path's few rows pay for whole batches of them.
 constexpr int kMoveUnroll = 4;
 constexpr uint32_t kMoveTable = 4096;   // block-table entries kept in LDS (longer tables are read from memory)
 

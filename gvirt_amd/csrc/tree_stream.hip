@@ -8,18 +8,20 @@
 //     S^T[pos][m]  = K[pos][:] . Q[m][:]           v_mfma_f32_32x32x16 (A = K rows, ds_read_b128; B = Q)
 //     O^T[d][m]   += V^T[d][pos] . P^T[pos][m]     v_mfma_f32_32x32x16 (A = V^T, ds_read_b64_tr_b16; B = P)
 // Four stages of 32 KiB: one is consumed while three are on their way (with two of 64 KiB half of what memory delivers in a
-// round trip was not asked for: 447 against 385-405 us for 64 trees of 32 over 8192 positions).
+// round trip was not asked for: a tenth slower for 64 trees of 32 over 8192 positions).
 // Rows of less than 256 bytes: copied as they stand four steps ahead (caches of bytes: 18 KiB a step with their scales) and laid
 // out in one of two stages, bytes widened to fp16; the scales join the scores. With the scales multiplied into fp16 rows an fp16 result was off by 5.5-8 e-4 of its size
 // instead of 2.1 e-4 (its own rounding).
 //
 // Bound by memory where trees are small next to their contexts. Measured: 64 trees of 32 nodes over 8192 positions, 8 kv heads of
-// 4, 2.19 GB: 385-405 us, 5.4-5.7 TB/s (the prefill kernel 514); 16 ragged trees of up to 27 over up to 4096, 170 MB: 49 us and
-// 8 of merging. 8 trees of up to 16 over up to 16384 int8 positions, 97 MB: 57 us and 8 of merging (the prefill kernel 80): 2 us a
-// step of 16 KiB, the chain of widening, barrier, operands, scores, softmax and products of two waves a SIMD. Half the vector
-// instructions for widening, or the products of one half of the waves beside the widening of the other: the same time. head_dim
-// 64, 16 bits: a tree of 8 over 700 positions 10 and 4 us (the prefill kernel 15), 64 ragged trees of 4 over 2000 25 us (31).
-// head_dim 256: 32 ragged trees of 8 over 4000 positions of 4 heads, 330 MB, 74 us with the merge (the generic kernel 237).
+// 4, 2.19 GB: 402 us in the first calls after a pause, 440 once the clocks have settled under load (up to 640 on the way there), 5.4
+// and 5.0 TB/s; 16 ragged trees of up to 27 over up to 4096, 170 MB: 49 us and 8 of merging. 8 trees of up to 16 over up to 16384
+// int8 positions, 97 MB: 58 us and 8 of merging (the prefill kernel 80): 2 us a step of 16 KiB, the chain of widening, barrier,
+// operands, scores, softmax and products. These trees fill two of the four row tiles of a head: the waves of the others only
+// copy, so that one wave a SIMD computes. Half the vector instructions for widening, or the products of one half of the waves beside
+// the widening of the other: the same time. head_dim 64, 16 bits: a tree of 8 over 700 positions 10 and 4 us (the prefill kernel
+// 15), 64 ragged trees of 4 over 2000 25 us (31). head_dim 256: 32 ragged trees of 8 over 4000 positions of 4 heads, 330 MB: 64 us after a
+// pause, 74 settled, and 5 of merging (the generic kernel 237).
 //
 // Work split: a sequence owns ceil(len G / rows) M tiles of ceil((cached + len) / step) steps each; the steps of all M tiles laid
 // end to end are cut into equal chunks, one per workgroup, whatever the sequences' lengths (they live in device memory: every

@@ -458,9 +458,10 @@ int xlite_hip_prepare_tree(const uint32_t *lens, const uint32_t *cached_lens, co
  * ancestors; bits from lens[i] on are ignored, nodes from 32 * mask_words on are seen by nobody).
  * mask_words <= 2^22. A row that sees nothing gets zeros. Infinities and NaNs in rows that a row does not see do not
  * reach it. Everything else as in xlite_hip_attention (quantised caches: head_dim 64 or 128;
- * v_scale is not negative, and counts as 2^-50 below and as 2^50 above, a NaN stays one; shapes that go through a
- * widened copy - blocks of one position, more than 1024 sequences, less workspace - saturate
- * values at 65504 there and take NaNs for -65504, as xlite_hip_attention does).
+ * v_scale is not negative, and counts as 2^-50 below and as 2^50 above, a NaN stays one, an e4m3
+ * NaN counts as -65504; shapes that another kernel serves - blocks of one position, more than 1024
+ * sequences, less workspace - saturate values times scales at 65504 and take NaNs for -65504, as
+ * xlite_hip_attention does).
  * workspace: xlite_hip_tree_attention_workspace_bytes(); with less another kernel serves the
  * batch, in the end without splitting the KV axis (one over a quantised cache that needs a 16-bit
  * copy fails with XLITE_HIP_ENOSPC). qkv, caches, output and workspace: aligned to 16 bytes.
@@ -506,7 +507,8 @@ int xlite_hip_verify_tree(void *stream, const void *logits, const int32_t *token
  * appended the position. window: only the last `window` rows of every sequence count (0: all).
  * Sums are fp32, in the same order in every run. A block may stand in one sequence's table only.
  * Sequences without rows are left as they are. 16-bit caches, or quantised ones (K bytes and
- * k_scale, head_dim 64 or 128). workspace: xlite_hip_attention_weights_workspace_bytes() (required).
+ * k_scale, head_dim 64 or 128). workspace: xlite_hip_attention_weights_workspace_bytes() (required;
+ * grows with the block tables' width, scores that are stored take 1.5 GB at the most).
  * qkv, k_cache and workspace: aligned to 16 bytes.
  * ---------------------------------------------------------------------- */
 size_t xlite_hip_attention_weights_workspace_bytes(uint32_t total_tokens, uint32_t n_heads,
