@@ -6,6 +6,8 @@ import subprocess
 
 import pytest
 
+from gvirt_amd.build import FLAGS
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 PROGRAM = r"""
@@ -37,7 +39,7 @@ __global__ void kernel(const uint32_t *where)
 def test_copies_wait_for_their_base(tmp_path):
     source = tmp_path / "copies.hip"
     source.write_text(PROGRAM)
-    text = subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "--offload-device-only", "-S", "-I",
+    text = subprocess.run([HIPCC] + FLAGS + ["--offload-device-only", "-S", "-I",
                            os.path.join(ROOT, "gvirt_amd", "csrc"), str(source), "-o", "-"], capture_output=True, text=True, check=True).stdout
     waited, since, copies = {}, 0, 0
     for line in text.splitlines():
