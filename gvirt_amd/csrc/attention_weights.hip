@@ -988,7 +988,7 @@ Plan plan_of(uint32_t total_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint3
         const uint32_t rows = static_cast<uint32_t>(bounded) * G;
         const uint32_t pitch = ceil_div(max_ctx, 64u) * 64u;
         // what a kv head takes: a normaliser and a score a position for every row, two statistics for every 64 positions at the most
-        const size_t of_head = static_cast<size_t>(rows) * (pitch + pitch / 32 + 1) * sizeof(float);
+        const size_t of_head = rows * (static_cast<size_t>(pitch) + pitch / 32 + 1) * sizeof(float);
         uint32_t heads = static_cast<uint32_t>(std::min<size_t>(n_kv_heads, kStoredBytes / of_head));
         heads = heads < n_kv_heads && heads > kStoredWaves ? heads / kStoredWaves * kStoredWaves : heads;
         if (heads != 0) {
@@ -1040,7 +1040,7 @@ extern "C" size_t xlite_hip_attention_weights_workspace_bytes(uint32_t total_tok
                                                               uint32_t head_dim, uint32_t block_size, uint32_t batch,
                                                               uint32_t max_num_block, uint32_t window)
 {
-    if (total_tokens == 0 || batch == 0 || n_kv_heads == 0 || n_heads % n_kv_heads != 0) {
+    if (total_tokens == 0 || batch == 0 || n_kv_heads == 0 || n_heads == 0 || n_heads % n_kv_heads != 0) {
         return 0;
     }
     return plan_of(total_tokens, n_heads, n_kv_heads, head_dim, block_size, batch, max_num_block, window).bytes;

@@ -40,3 +40,11 @@ def test_stored_scores_are_bounded(shape):
 def test_one_row_a_sequence_is_not_laid_out_for_more():
     """64 rows of 32 heads over tables of 4096 positions: a score of 4 bytes each, and their statistics."""
     assert weights(64, 32, 8, 128, 128, 64, 32) < 1.1 * 64 * 32 * 4096 * 4
+
+
+def test_sizes_of_shapes_that_do_not_exist():
+    """The size functions answer whatever they are asked (the calls themselves refuse such shapes)."""
+    for heads, kv_heads, block, blocks in ((0, 2, 16, 4), (4, 0, 16, 4), (3, 2, 16, 4), (4, 2, 16, 0), (4, 2, 1 << 16, (1 << 16) - 1)):
+        weights(8, heads, kv_heads, 64, block, 2, blocks)
+        tree(8, heads, kv_heads, 64, block, 2, blocks, 0)
+    assert weights(8, 0, 2, 64, 16, 2, 4) == 0
